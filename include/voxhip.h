@@ -103,6 +103,88 @@ int vox_paged_attention_of(vox_ctx* ctx, void* stream, const void* q, const void
  * more than 32 tokens with a page table), else rows that read q and their pages. */
 int vox_attention_form(int decode, int n_rows, int n_req, int Hq, int Hkv, int D, int page_size, int max_kvlen);
 
+/* ---- long contexts: a paged cache whose blocks are chosen per query ---------------------------------------------------
+ * A cache layer is the one of vox_kv_append / vox_paged_attention, in bf16 or fp16.  A page is page_size / block blocks of `block`
+ * tokens; of every complete block, per kv head, `bounds` holds the largest and the smallest key of each channel as whole numbers of
+ * steps (rounded outward: ceil and floor, -127..127) and `steps` the step, a power of two: the smallest one of which 127 reach the
+ * block's largest finite |key|, and at least 2^-100.  NaN keys are passed over, infinite ones count as 127 steps; a channel of NaN is 0.
+ * The four calls below are the three operators of such a cache (rotate + append, choose, attend) and the bounds alone.  Rows whose page
+ * (append, bounds) or q_kvlen (choose, attend) is not positive enough to exist - page < 0, page >= n_pages, slot outside the page, q_kvlen <= 0,
+ * q_req outside the requests - are passed over: what the call would have written for them stays as it was.  Page ids outside the cache and blocks
+ * behind a request's pages are passed over too (such a block is as if it were not listed).  kv_indptr is the caller's word for how long kv_indices is. */
+enum { VOX_DTYPE_BF16 = 0, VOX_DTYPE_F16 = 1 };
+typedef struct {
+    void* kv;            /* [n_pages,2,page_size,kv_heads,head_dim], on 16 bytes */
+    int8_t* bounds;      /* [n_pages,kv_heads,page_size/block,2,head_dim]: largest, smallest; on 16 bytes */
+    float* steps;        /* [n_pages,kv_heads,page_size/block] */
+    int32_t n_pages, page_size, block, kv_heads, head_dim, dtype; /* block 16, 32, 64 or 128; head_dim 64 or 128 */
+} vox_block_cache;
+typedef struct { /* rows of one ragged call (the plan arrays of vox_paged_attention) */
+    const int32_t *q_req, *q_kvlen, *kv_indptr, *kv_indices;
+    int32_t n_rows, n_req;  /* n_req: entries of kv_indptr minus one */
+    int32_t n_own;          /* how many requests have rows here (0: not known; the launch goes by it, the results do not) */
+    int32_t heads;          /* query heads: kv_heads times 1..64 */
+    int32_t max_kvlen;      /* bounds q_kvlen (a longer row is taken as this long) */
+} vox_block_rows;
+
+/* RoPE of q and k and the append of k and v in one call: apply_rope_pos_ids + set_kv_cache (flashinfer_utils.py:134-145, 270-324), bit for
+ * bit vox_rope + vox_kv_append.  Rows of q, k, v may lie apart (strides in elements, so the slices of one projection's output serve as they
+ * are); q_out [n_rows,heads,head_dim] contiguous, may be q itself if that is.  Positions are clamped to the table as in vox_rope (fp32
+ * [table_max_pos, rot/2, 2], vox_rope_table_host); rot even, 0 (no table) .. head_dim; interleave: pairs (2i, 2i+1), else (i, i + rot/2).
+ * cache.bounds not NULL: also the bounds of the blocks that these rows complete.  n_own: how many requests have rows here (0: not known); n_own ==
+ * n_rows says that no two rows share a request, hence a block, and the bounds come in the same launch.  No two rows may have the same page and slot. */
+typedef struct {
+    vox_block_cache cache;
+    const void *q, *k, *v;
+    void* q_out;
+    const int32_t *pos, *page, *slot;
+    const float* table;
+    int64_t q_stride, k_stride, v_stride;
+    int32_t n_rows, n_own, heads, rot, interleave, table_max_pos;
+} vox_rope_append_args;
+int vox_rope_append(vox_ctx* ctx, void* stream, const vox_rope_append_args* a);
+/* The bounds of the blocks whose last slot is one of (page, slot): behind any other way of filling the cache (vox_kv_append, a copied prefix). */
+int vox_block_bounds(vox_ctx* ctx, void* stream, const vox_block_cache* cache, const int32_t* page, const int32_t* slot, int n_rows);
+
+/* Blocks that each row reads, per kv head: blocks[n_rows,kv_heads,top], ascending, -1 behind the last.  A row of n tokens has ceil(n / block)
+ * blocks; its first `first` and its last `last` >= 1 are always taken (the newest is part filled and has no bounds), of the others the
+ * top - first - last with the largest scores, the lower index where scores are equal:
+ *   score = fp32(sum over the kv head's query heads and channels of max(a * hi, a * lo)) * step,
+ *   a = q rounded to the nearest whole number (to even) of the smallest power of two of which 127 reach the largest finite |q| of the kv head's query heads (at
+ * least 2^-100), clamped to +-127, NaN 0.  Sums of whole numbers: the choice depends on no order, batch or launch.  At most
+ * VOX_BLOCK_SELECT_MAX blocks a row.  workspace: vox_block_select_workspace_bytes(), nothing in it outlives the call. */
+#define VOX_BLOCK_SELECT_MAX 32768
+#define VOX_BLOCK_TOP_MAX 1024
+typedef struct {
+    vox_block_cache cache;
+    vox_block_rows rows;
+    const void* q;       /* [n_rows, heads, head_dim], rows q_stride elements apart */
+    int32_t* blocks;
+    void* workspace;
+    int64_t workspace_bytes, q_stride;
+    int32_t top, first, last;
+} vox_block_select_args;
+int64_t vox_block_select_workspace_bytes(const vox_block_select_args* a);
+int vox_block_select(vox_ctx* ctx, void* stream, const vox_block_select_args* a);
+
+/* out[i, h] = softmax(scale q . K) V over the tokens < q_kvlen[i] of the blocks in row i's list of h's kv head; out [n_rows,heads,head_dim] contiguous.  An entry
+ * counts if it is a block of the row and larger than every entry before it.  A row without any such entry is zero.  Scores, sums and
+ * the output are fp32 until its one rounding (the softmax weights enter the matrix cores as two 16-bit terms).  What a masked or unlisted
+ * token holds, NaN and infinities included, does not reach a row. */
+typedef struct {
+    vox_block_cache cache;   /* bounds and steps are not read */
+    vox_block_rows rows;
+    const void* q;
+    const int32_t* blocks;
+    void* out;
+    void* workspace;
+    int64_t workspace_bytes, q_stride;
+    int32_t top;
+    float scale;
+} vox_block_attention_args;
+int64_t vox_block_attention_workspace_bytes(const vox_block_attention_args* a);
+int vox_block_attention(vox_ctx* ctx, void* stream, const vox_block_attention_args* a);
+
 /* nn.Linear on bf16 (qwen3_tts.py:562-601): y[b,n] = bf16(dot(W[n,:],x[b,:]) + bias[n]);
  * residual != NULL: y = bf16(residual + y).  act: 0 none, 1 SiLU applied to the rounded output. */
 int vox_linear(vox_ctx* ctx, void* stream, const void* W, const void* bias, const void* x, const void* residual,

@@ -1,0 +1,146 @@
+"""What block_attention refuses, before anything reaches a GPU: by the C entry points (the argument structs with one field wrong at a time) and by the
+Python functions; and that the packed structs are the header's."""
+import os
+import shutil
+import subprocess
+
+import pytest
+import torch
+
+from vox_serve_amd import _native as N
+from vox_serve_amd import block_attention as B
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+AT = 4096           # an address for the checks to look at; nothing reads it
+CACHE = dict(kv=AT, bounds=AT, steps=AT, n_pages=4, page_size=128, block=32, kv_heads=2, head_dim=128, dtype=0)
+ROWS = dict(q_req=AT, q_kvlen=AT, kv_indptr=AT, kv_indices=AT, n_rows=3, n_req=2, n_own=0, heads=16, max_kvlen=400, pad=0)
+APPEND = dict(CACHE, q=AT, k=AT, v=AT, q_out=AT, pos=AT, page=AT, slot=AT, table=AT, q_stride=2048, k_stride=256, v_stride=256, n_rows=3, n_own=0, heads=16, rot=128,
+              interleave=0, table_max_pos=100)
+SELECT = dict(CACHE, **ROWS, q=AT, blocks=AT, workspace=AT, workspace_bytes=1 << 40, q_stride=2048, top=8, first=1, last=2)
+ATTEND = dict(CACHE, **ROWS, q=AT, blocks=AT, out=AT, workspace=AT, workspace_bytes=1 << 40, q_stride=2048, top=8, scale=0.1)
+
+
+def call(fn, packer, fields, **wrong):
+    return getattr(N.lib(), fn)(None, None, packer.pack(*dict(fields, **wrong).values()))
+
+
+BAD_CACHE = [dict(kv=0), dict(kv=AT + 8), dict(n_pages=0), dict(page_size=0), dict(kv_heads=0), dict(kv_heads=-2), dict(dtype=2), dict(block=8), dict(block=0), dict(block=96),
+             dict(page_size=100), dict(page_size=16), dict(head_dim=96), dict(head_dim=0)]
+BAD_BOUNDS = [dict(steps=0), dict(bounds=AT + 4), dict(steps=AT + 2)]
+BAD_ROWS = [dict(n_rows=-1), dict(n_req=-1), dict(n_own=-1), dict(heads=0), dict(heads=15), dict(heads=130), dict(max_kvlen=-1), dict(q_req=0), dict(q_kvlen=0), dict(kv_indptr=0),
+            dict(kv_indices=0), dict(q=0), dict(q=AT + 1), dict(q_stride=-1), dict(blocks=0)]
+
+
+@pytest.mark.parametrize("wrong", BAD_CACHE + BAD_BOUNDS + [dict(q=0), dict(k=0), dict(v=0), dict(q_out=0), dict(page=0), dict(slot=0), dict(pos=0), dict(table=0), dict(table=AT + 2),
+                                                             dict(table_max_pos=0), dict(rot=130), dict(rot=3), dict(rot=-2), dict(n_rows=-1), dict(n_own=-1), dict(heads=0), dict(q=AT + 1),
+                                                             dict(q_stride=-5), dict(head_dim=127, bounds=0), dict(head_dim=514, bounds=0)], ids=str)
+def test_rope_append_refuses(wrong):
+    assert call("vox_rope_append", B._APPEND, APPEND, **wrong) == 1
+    assert b"rope_append" in N.lib().vox_last_error()
+
+
+@pytest.mark.parametrize("wrong", BAD_BOUNDS + BAD_ROWS + [w for w in BAD_CACHE if "kv" not in w]
+                         + [dict(bounds=0), dict(top=2), dict(top=1025), dict(first=-1), dict(last=0), dict(first=7), dict(first=2 ** 31 - 1), dict(max_kvlen=32 * 32768 + 1)], ids=str)
+def test_block_select_refuses(wrong):
+    assert call("vox_block_select", B._SELECT, SELECT, **wrong) == 1
+    assert b"block_select" in N.lib().vox_last_error()
+
+
+@pytest.mark.parametrize("wrong", BAD_CACHE + BAD_ROWS + [dict(out=0), dict(out=AT + 1), dict(top=-1), dict(top=1025)], ids=str)
+def test_block_attention_refuses(wrong):
+    assert call("vox_block_attention", B._ATTEND, ATTEND, **wrong) == 1
+    assert b"block_attention" in N.lib().vox_last_error()
+
+
+@pytest.mark.parametrize("wrong", BAD_CACHE + BAD_BOUNDS + [dict(bounds=0)], ids=str)
+def test_block_bounds_refuses(wrong):
+    fields = B._BOUNDS.pack(*dict(CACHE, **wrong).values())
+    assert N.lib().vox_block_bounds(None, None, fields, AT, AT, 3) == 1
+    assert b"block_bounds" in N.lib().vox_last_error()
+
+
+def test_missing_arguments_and_nothing_to_do():
+    L = N.lib()
+    for fn in ("vox_rope_append", "vox_block_select", "vox_block_attention"):
+        assert getattr(L, fn)(None, None, None) == 1
+    assert L.vox_block_bounds(None, None, None, AT, AT, 1) == 1
+    assert L.vox_block_bounds(None, None, B._BOUNDS.pack(*CACHE.values()), None, AT, 1) == 1
+    assert L.vox_block_bounds(None, None, B._BOUNDS.pack(*CACHE.values()), AT, AT, -1) == 1
+    assert L.vox_block_select_workspace_bytes(B._SELECT.pack(*dict(SELECT, top=2).values())) == -1
+    assert L.vox_block_attention_workspace_bytes(B._ATTEND.pack(*dict(ATTEND, top=-1).values())) == -1
+    # no rows: done, and no pointer is asked for
+    assert call("vox_rope_append", B._APPEND, APPEND, n_rows=0, q=0, k=0, v=0, page=0) == 0
+    assert call("vox_block_select", B._SELECT, SELECT, n_rows=0, q=0, q_req=0) == 0
+    assert call("vox_block_attention", B._ATTEND, ATTEND, n_rows=0, q=0, out=0, q_req=0) == 0
+    assert L.vox_block_bounds(None, None, B._BOUNDS.pack(*CACHE.values()), None, None, 0) == 0
+
+
+def test_packed_structs_are_the_headers(tmp_path):
+    cc = shutil.which("cc") or shutil.which("gcc")
+    if cc is None:
+        pytest.skip("no C compiler")
+    src = tmp_path / "s.c"
+    src.write_text('#include "voxhip.h"\n#include <stdio.h>\n#include <stddef.h>\n#define P(t, f) printf("%zu ", offsetof(t, f))\n#define Z(t) printf("%zu\\n", sizeof(t))\nint main(void) {\n'
+                   + "".join(f"P({t}, {f});" for t, f in (("vox_rope_append_args", "q_stride"), ("vox_rope_append_args", "table_max_pos"))) + "Z(vox_rope_append_args);"
+                   + "P(vox_block_cache, dtype); Z(vox_block_cache);"
+                   + "".join(f"P(vox_block_select_args, {f});" for f in ("rows.max_kvlen", "q", "q_stride", "last")) + "Z(vox_block_select_args);"
+                   + "".join(f"P(vox_block_attention_args, {f});" for f in ("rows.heads", "out", "top", "scale")) + "Z(vox_block_attention_args);\nreturn 0;\n}\n")
+    subprocess.check_call([cc, "-I", os.path.join(ROOT, "include"), str(src), "-o", str(tmp_path / "s")])
+    lines = [[int(x) for x in line.split()] for line in subprocess.check_output([str(tmp_path / "s")], text=True).splitlines()]
+
+    def at(packer, fields, *names):
+        """Where a field's bytes lie: what changes when it does."""
+        out = []
+        for n in names:
+            a, b = (packer.pack(*dict(fields, **{n: v}).values()) for v in ((1, 2) if n != "scale" else (1.0, -1.0)))
+            out.append(min(i for i in range(len(a)) if a[i] != b[i]) // 4 * 4)
+        return out + [packer.size]
+
+    assert lines == [at(B._APPEND, APPEND, "q_stride", "table_max_pos"), at(B._BOUNDS, CACHE, "dtype"), at(B._SELECT, SELECT, "max_kvlen", "q", "q_stride", "last"),
+                     at(B._ATTEND, ATTEND, "heads", "out", "top", "scale")]
+
+
+def test_python_functions_refuse():
+    """Shapes, types and places, on the CPU; the C entry points' own refusals come behind these."""
+    kv = torch.zeros(2, 2, 32, 2, 64, dtype=torch.bfloat16)
+    q, k = torch.zeros(3, 4, 64, dtype=torch.bfloat16), torch.zeros(3, 2, 64, dtype=torch.bfloat16)
+    one = torch.zeros(3, dtype=torch.int32)
+    bounds, steps = B.new_bounds(kv, 16)
+    assert bounds.shape == (2, 2, 2, 2, 64) and bounds.dtype is torch.int8 and steps.shape == (2, 2, 2)
+    with pytest.raises(ValueError, match="whole blocks"):
+        B.new_bounds(kv, 24)
+    with pytest.raises(ValueError, match="HIP device"):
+        B.rope_append(q, k, k, kv, None, one, one, one)
+    with pytest.raises(ValueError, match="HIP device"):
+        B.block_attention(q, kv, torch.zeros(3, 2, 2, dtype=torch.int32), one, one, one, one, block=16)
+    with pytest.raises(ValueError, match="HIP device"):
+        B.select_blocks(q, bounds, steps, one, one, one, one, block=16, top=4, max_kvlen=32)
+    with pytest.raises(ValueError, match="HIP device"):
+        B.update_bounds(kv, bounds, steps, one, one)
+    with pytest.raises(ValueError, match="kv_cache has shape"):
+        B.rope_append(q, k, k, kv[:, :1], None, one, one, one)
+    with pytest.raises(ValueError, match="kv_cache has shape"):
+        B.update_bounds(kv.transpose(2, 3), bounds, steps, one, one)
+    with pytest.raises(TypeError, match="kv_cache is"):
+        B.block_attention(q, kv.float(), torch.zeros(3, 2, 2, dtype=torch.int32), one, one, one, one, block=16)
+    # the checks behind the device's, on their own
+    with pytest.raises(ValueError, match="pages has shape"):
+        B._ints(one, (4,), one.device, "pages")
+    with pytest.raises(TypeError, match="int32 or int64"):
+        B._ints(one.float(), (3,), one.device, "pages")
+    assert B._ints(one.long(), (3,), one.device, "pages").dtype is torch.int32
+    with pytest.raises(ValueError, match="q has shape"):
+        B._heads(q, 3, 128, kv, "q")
+    with pytest.raises(ValueError, match="q is torch.float16"):
+        B._heads(q.half(), 3, 64, kv, "q")
+    assert B._heads(q.transpose(0, 1).contiguous().transpose(0, 1), 3, 64, kv, "q").is_contiguous()       # heads apart: laid together
+    wide = torch.zeros(3, 512, dtype=torch.bfloat16)[:, 64:320].unflatten(1, (4, 64))
+    assert B._heads(wide, 3, 64, kv, "q") is wide                                                          # rows apart: taken as they are
+    with pytest.raises(ValueError, match="not those of a cache"):
+        B._bounds_of(kv, bounds[:1].contiguous(), steps[:1].contiguous())
+    with pytest.raises(ValueError, match="steps is"):
+        B._bounds_of(kv, bounds, steps.double())
+    with pytest.raises(ValueError, match="bounds is"):
+        B._bounds_of(kv, bounds.int(), steps)
+    with pytest.raises(ValueError, match="out is"):
+        B._out(torch.zeros(3, 4, 64), q.shape, torch.bfloat16, q.device)

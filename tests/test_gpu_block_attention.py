@@ -1,0 +1,603 @@
+"""block_attention's operators on an MI355X against their definition in 64 bits (oracle/block_attn_ref.py): integers equal, the append bit for bit what
+apply_rope_pos_ids and set_kv_cache write, attention within the output's half step and the bound that the oracle derives for fp32 work."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import block_attn_ref as R
+
+pytestmark = pytest.mark.gpu
+TYPES = {"bf16": torch.bfloat16, "f16": torch.float16}
+
+
+@pytest.fixture(scope="module")
+def dev():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    from vox_serve_amd import _native as N
+    N.ctx()
+    return torch.device("cuda", torch.cuda.current_device())
+
+
+def f64(t):
+    return t.detach().cpu().double().numpy()
+
+
+class Paged:
+    """Requests of the given lengths on shuffled pages, new rows at their ends, a page that is nobody's."""
+
+    def __init__(self, dev, dtype, h, d, page, kv_lens, q_lens, seed=0, spare=1):
+        g = torch.Generator().manual_seed(seed)
+        self.kv_lens, self.page = kv_lens, page
+        need = [-(-n // page) for n in kv_lens]
+        total = sum(need) + spare
+        order = torch.randperm(total, generator=g).tolist()
+        self.pages, at = [], 0
+        for n in need:
+            self.pages.append(order[at:at + n])
+            at += n
+        self.indptr = torch.tensor([0] + list(np.cumsum(need)), dtype=torch.int32, device=dev)
+        self.indices = torch.tensor(order[:max(at, 1)], dtype=torch.int32, device=dev)
+        self.req = [r for r, m in enumerate(q_lens) for _ in range(m)]
+        self.kvlen = [kv_lens[r] - m + i + 1 for r, m in enumerate(q_lens) for i in range(m)]
+        self.n = len(self.req)
+        self.q_req = torch.tensor(self.req, dtype=torch.int32, device=dev)
+        self.q_kvlen = torch.tensor(self.kvlen, dtype=torch.int32, device=dev)
+        self.row_page = torch.tensor([self.pages[r][(n - 1) // page] for r, n in zip(self.req, self.kvlen)], dtype=torch.int32, device=dev)
+        self.row_slot = torch.tensor([(n - 1) % page for n in self.kvlen], dtype=torch.int32, device=dev)
+        self.kv = torch.randn(total, 2, page, h, d, generator=g).to(dtype).to(dev)
+        self.gen, self.dtype, self.dev, self.h, self.d = g, dtype, dev, h, d
+
+    def rnd(self, *shape, s=1.0):
+        return (s * torch.randn(*shape, generator=self.gen)).to(self.dtype).to(self.dev)
+
+    @property
+    def plan(self):
+        return self.q_req, self.q_kvlen, self.indptr, self.indices
+
+    def bounds(self, block):
+        """Of every complete block, by the oracle."""
+        k = f64(self.kv)[:, 0]
+        total, page, h, d = k.shape
+        per = page // block
+        b, s = np.zeros((total, h, per, 2, d), np.int8), np.zeros((total, h, per), np.float32)
+        for p in range(total):
+            for g in range(h):
+                for j in range(per):
+                    b[p, g, j], s[p, g, j] = R.bounds(k[p, j * block:(j + 1) * block, g])
+        return torch.from_numpy(b).to(self.dev), torch.from_numpy(s).to(self.dev)
+
+
+def table(dev, length, half, theta=1e4):
+    a = torch.arange(length, dtype=torch.float64)[:, None] * theta ** (-torch.arange(half, dtype=torch.float64) / max(half, 1))
+    return torch.stack([a.cos(), a.sin()], -1).float().to(dev)
+
+
+# ---------------------------------------------------------------- append
+APPEND = [  # heads, kv heads, dim, page, block, rot, pairs interleaved, kv lengths, new rows
+    (16, 8, 128, 128, 64, 128, False, [200, 64, 128, 1], [1, 1, 1, 1]),
+    (32, 2, 128, 64, 64, 64, True, [64, 63, 65], [1, 1, 1]),
+    (14, 2, 64, 48, 16, 64, False, [48, 100, 17, 3], [48, 37, 17, 1]),
+    (8, 8, 64, 16, 16, 32, True, [33, 16], [33, 1]),
+    (12, 4, 128, 32, 32, 0, False, [70, 32], [70, 32]),
+    (4, 1, 128, 128, 128, 128, True, [300], [300]),
+    (4, 2, 64, 32, 16, 18, False, [40], [40]),           # an odd number of pairs: no vector of eight fits
+    (4, 2, 64, 32, 16, 6, True, [40, 2], [40, 2]),
+]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("hq,h,d,page,block,rot,interleave,kv_lens,q_lens", APPEND)
+def test_rope_append(dev, dtype, hq, h, d, page, block, rot, interleave, kv_lens, q_lens):
+    from vox_serve_amd import block_attention as B
+    s = Paged(dev, TYPES[dtype], h, d, page, kv_lens, q_lens, seed=hq + rot)
+    qkv = s.rnd(s.n, (hq + 2 * h) * d)
+    q, k, v = (x.unflatten(1, (-1, d)) for x in qkv.split([hq * d, h * d, h * d], 1))
+    pos = torch.tensor([n - 1 for n in s.kvlen], dtype=torch.int32, device=dev)
+    cs = table(dev, 64, rot // 2) if rot else None        # shorter than some positions: those take the last row
+    before = s.kv.clone()
+    for n_req in (0, len(q_lens)):
+        s.kv.copy_(before)
+        bounds, steps = B.new_bounds(s.kv, block)
+        got = B.rope_append(q, k, v, s.kv, cs, pos, s.row_page, s.row_slot, interleave=interleave, bounds=bounds, steps=steps, n_req=n_req)
+        tab = cs.cpu().numpy() if rot else np.zeros((1, 0, 2), np.float32)
+        half_step = torch.finfo(TYPES[dtype]).eps / 2
+        tiny = torch.finfo(TYPES[dtype]).smallest_normal * half_step
+        for x, y in ((q, got), (k, None)):
+            want = R.rotate(f64(x), tab, pos.cpu().numpy(), interleave)
+            have = f64(got) if y is not None else f64(s.kv[s.row_page.long(), 0, s.row_slot.long()])
+            # two products in fp32, each off by 2^-24 of |x| + |y| <= 2 max|x| at most, then one rounding
+            far = np.abs(have - want)
+            assert (far <= half_step * np.abs(want) * (1 + half_step) + 2.0 ** -22 * np.abs(f64(x)).max(-1, keepdims=True) + tiny).all()
+        assert torch.equal(s.kv[s.row_page.long(), 1, s.row_slot.long()], v)
+        # nothing else of the cache has changed
+        mask = torch.zeros(s.kv.shape[0], page, dtype=torch.bool, device=dev)
+        mask[s.row_page.long(), s.row_slot.long()] = True
+        assert torch.equal(s.kv.transpose(1, 2)[~mask], before.transpose(1, 2)[~mask])
+        # bounds: of the blocks that were completed, of no others
+        want_b, want_s = s.bounds(block)
+        done = torch.zeros(s.kv.shape[0], page // block, dtype=torch.bool, device=dev)
+        last = (s.row_slot.long() + 1) % block == 0
+        done[s.row_page.long()[last], s.row_slot.long()[last] // block] = True
+        assert torch.equal(bounds.transpose(1, 2)[done], want_b.transpose(1, 2)[done]) and torch.equal(steps.transpose(1, 2)[done], want_s.transpose(1, 2)[done])
+        assert not bounds.transpose(1, 2)[~done].any() and not steps.transpose(1, 2)[~done].any()
+
+
+@pytest.mark.parametrize("hq,h,d,rot,interleave,n", [(16, 8, 128, 128, False, 3), (32, 2, 128, 64, True, 70), (14, 2, 64, 64, False, 150), (4, 2, 16, 8, True, 5), (4, 2, 24, 22, False, 9),
+                                                     (16, 8, 128, 64, False, 33)])
+def test_rope_append_is_rope_then_append(dev, hq, h, d, rot, interleave, n):
+    from vox_serve_amd import block_attention as B
+    from vox_serve_amd.flashinfer_utils import FlashInferPrefillWrapper, _rope_table, apply_rope_pos_ids
+    page = 32
+    need = -(-n // page)
+    g = torch.Generator().manual_seed(n)
+    r = lambda *s: torch.randn(*s, generator=g).bfloat16().to(dev)
+    q, k, v = r(n, hq, d), r(n, h, d), r(n, h, d)
+    w = FlashInferPrefillWrapper(None, hq, h, hq * d, page, device=dev)
+    w.plan(torch.tensor([0, n]), torch.tensor([0, need]), torch.randperm(need, generator=g).int(), torch.tensor([n - (need - 1) * page]), torch.bfloat16)
+    pos = torch.arange(n, dtype=torch.int32, device=dev) * 37
+    qr, kr = apply_rope_pos_ids(q, k, pos, interleave=interleave, rope_theta=1e6, rotary_dim=rot)
+    want, have = torch.zeros(need, 2, page, h, d, dtype=torch.bfloat16, device=dev), torch.zeros(need, 2, page, h, d, dtype=torch.bfloat16, device=dev)
+    w.set_kv_cache(want, kr, v)
+    cs = _rope_table(dev, 8192, rot, 1e6, 1.0, None).view(8192, rot // 2, 2)
+    assert torch.equal(w.set_kv_cache_rope(have, q, k, v, pos, cs, interleave=interleave), qr)
+    assert torch.equal(have, want)
+    # q turned where it is
+    have.zero_()
+    q2 = q.clone()
+    assert B.rope_append(q2, k, v, have, cs, pos.long(), w.token_to_page, w.token_to_cache, interleave=interleave, out=q2) is q2
+    assert torch.equal(q2, qr) and torch.equal(have, want)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("d,rot,interleave", [(128, 128, False), (64, 64, True), (128, 64, False)])
+def test_rope_append_rounds_where_it_says(dev, dtype, d, rot, interleave):
+    """x cos rounded to 32 bits, the fused sum rounded to 32, then to the type: the bits of that, over enough values that another order would show."""
+    from vox_serve_amd import block_attention as B
+    n, hq, h, page = 600, 16, 8, 64
+    s = Paged(dev, TYPES[dtype], h, d, page, [n], [n], seed=d)
+    q, k = s.rnd(n, hq, d), s.rnd(n, h, d)
+    cs = table(dev, n, rot // 2)
+    got = B.rope_append(q, k, k, s.kv, cs, s.q_kvlen - 1, s.row_page, s.row_slot, interleave=interleave)
+    c, sn = (cs[:, None, :, i].cpu().numpy() for i in (0, 1))
+    for x, y in ((q, got), (k, s.kv[s.row_page.long(), 0, s.row_slot.long()])):
+        f = x.float().cpu().numpy()
+        a, b = (f[..., 0:rot:2], f[..., 1:rot:2]) if interleave else (f[..., :rot // 2], f[..., rot // 2:rot])
+        u = ((a * c).astype(np.float64) - b.astype(np.float64) * sn).astype(np.float32)       # (products of 8 or 11 by 24 bits are exact in 64)
+        v = ((b * c).astype(np.float64) + a.astype(np.float64) * sn).astype(np.float32)
+        turned = np.stack([u, v], -1).reshape(n, x.shape[1], rot) if interleave else np.concatenate([u, v], -1)
+        want = torch.cat([torch.from_numpy(turned).to(TYPES[dtype]), x[..., rot:].cpu()], -1)
+        assert torch.equal(y.cpu(), want)
+
+
+def test_rope_append_passes_rows_over(dev):
+    from vox_serve_amd import block_attention as B
+    n, hq, h, d, page = 6, 4, 2, 64, 16
+    q, k, v = (torch.randn(n, x, d, device=dev, dtype=torch.bfloat16) for x in (hq, h, h))
+    kv = torch.zeros(3, 2, page, h, d, dtype=torch.bfloat16, device=dev)
+    pages, slots = torch.tensor([0, -1, 3, 1, 2, 2], device=dev), torch.tensor([15, 15, 15, -1, 16, 15], device=dev)
+    out = torch.full((n, hq, d), 7.0, dtype=torch.bfloat16, device=dev)
+    for n_req in (0, n):
+        bounds, steps = B.new_bounds(kv, 16)
+        B.rope_append(q, k, v, kv, None, torch.zeros(n, dtype=torch.int32, device=dev), pages, slots, bounds=bounds, steps=steps, out=out, n_req=n_req)
+        assert torch.equal(out[[0, 5]], q[[0, 5]]) and (out[1:5] == 7).all()
+        assert torch.equal(kv[[0, 2], 0, 15], k[[0, 5]]) and torch.equal(kv[[0, 2], 1, 15], v[[0, 5]])
+        assert not kv[1].any() and not kv[:, :, :15].any()
+        assert (steps[[0, 2]] > 0).all() and not steps[1].any()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("block", [16, 32, 64, 128])
+def test_bounds_of_odd_keys(dev, d, block):
+    """Zeros, subnormals, the type's largest and lowest, infinities and NaN; a channel of NaN; the same by update_bounds."""
+    from vox_serve_amd import block_attention as B
+    for dtype in (torch.bfloat16, torch.float16):
+        s = Paged(dev, dtype, 3, d, 2 * block, [2 * block * 8], [1], seed=d + block, spare=0)
+        k = s.kv[:, 0]
+        k[0] = 0
+        k[1, 3] = torch.finfo(dtype).max
+        k[2, 5, 1, 7] = float("inf")
+        k[2, 6, 1, 8] = float("-inf")
+        k[3, 0, 2] = float("nan")
+        k[4, :, 0, 9] = float("nan")
+        k[5] *= 2.0 ** -20
+        k[6, :, 1] = torch.finfo(dtype).smallest_normal / 4
+        k[7, :block] = 127.0 * 0.5
+        k[7, block:] = 1.0
+        k[7, block + 1] = -2.0
+        bounds, steps = B.new_bounds(s.kv, block)
+        pages = torch.arange(8, device=dev).repeat_interleave(2)
+        slots = torch.tensor([block - 1, 2 * block - 1], device=dev).repeat(8)
+        B.update_bounds(s.kv, bounds, steps, pages, slots)
+        want_b, want_s = s.bounds(block)
+        assert torch.equal(bounds, want_b) and torch.equal(steps, want_s)
+
+
+# ---------------------------------------------------------------- choose
+SELECT = [  # heads, kv heads, dim, page, block, top, first, last, kv lengths, new rows
+    (16, 8, 128, 128, 32, 8, 1, 2, [1000, 33, 600], [1, 1, 1]),
+    (32, 2, 128, 64, 64, 5, 1, 2, [2000, 64, 320, 321], [1, 1, 1, 1]),
+    (14, 2, 64, 48, 16, 9, 1, 2, [700, 150], [30, 21]),
+    (8, 8, 64, 16, 16, 3, 0, 1, [300], [130]),
+    (12, 4, 128, 32, 32, 7, 3, 4, [900, 260], [17, 3]),
+    (64, 1, 64, 16, 16, 12, 2, 1, [500, 1], [2, 1]),
+    (6, 2, 128, 128, 128, 4, 1, 1, [3000], [9]),
+    (4, 2, 64, 16, 16, 70, 1, 2, [2100, 5], [3, 2]),        # more than a wave's lanes to take
+]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("hq,h,d,page,block,top,first,last,kv_lens,q_lens", SELECT)
+def test_select_blocks(dev, dtype, hq, h, d, page, block, top, first, last, kv_lens, q_lens):
+    from vox_serve_amd import block_attention as B
+    s = Paged(dev, TYPES[dtype], h, d, page, kv_lens, q_lens, seed=top)
+    q = s.rnd(s.n, hq, d)
+    bounds, steps = s.bounds(block)
+    nb, ns = bounds.cpu().numpy(), steps.cpu().numpy()
+    want = np.stack([R.select(f64(q[i]), nb, ns, s.pages[s.req[i]], s.kvlen[i], block, top, first, last) for i in range(s.n)])
+    for n_req in (0, len(q_lens)):
+        for most in (max(kv_lens), 4 * max(kv_lens)):
+            got = B.select_blocks(q, bounds, steps, *s.plan, block=block, top=top, max_kvlen=most, first=first, last=last, n_req=n_req)
+            assert np.array_equal(got.cpu().numpy(), want)
+
+
+def test_select_ties_zeros_and_odd_queries(dev):
+    """Equal scores go to the older block; queries of zeros, NaN and infinities choose by the same rule."""
+    from vox_serve_amd import block_attention as B
+    s = Paged(dev, torch.bfloat16, 2, 64, 32, [32 * 40] * 6, [1] * 6, seed=4)
+    s.kv[:, 0] = s.kv[:1, :1, :1, :, :][:, 0]                # every key the same
+    q = s.rnd(6, 8, 64)
+    q[1] = 0
+    q[2, 3, 5] = float("nan")
+    q[3, 0, 0] = float("inf")
+    q[4] = float("nan")
+    q[5, :4] *= 2.0 ** 100
+    for mix in (False, True):
+        if mix:
+            s.kv[::3, 0] *= 2.0
+        bounds, steps = s.bounds(32)
+        nb, ns = bounds.cpu().numpy(), steps.cpu().numpy()
+        want = np.stack([R.select(f64(q[i]), nb, ns, s.pages[i], s.kvlen[i], 32, 11, 1, 2) for i in range(6)])
+        got = B.select_blocks(q, bounds, steps, *s.plan, block=32, top=11, max_kvlen=1280, n_req=6)
+        assert np.array_equal(got.cpu().numpy(), want)
+        if not mix:
+            assert got[0, 0].tolist() == [0, 1, 2, 3, 4, 5, 6, 7, 8, 38, 39]
+
+
+def test_select_passes_rows_over_and_missing_pages(dev):
+    from vox_serve_amd import block_attention as B
+    s = Paged(dev, torch.float16, 2, 64, 16, [400, 400, 400], [1, 1, 1], seed=2)
+    bounds, steps = s.bounds(16)
+    q = s.rnd(5, 4, 64)
+    req, lens = torch.tensor([0, 1, 2, 7, -1], device=dev), torch.tensor([400, 0, 400, 400, 400], device=dev)
+    indices = s.indices.clone()
+    indices[int(s.indptr[2]) + 3] = 10 ** 6
+    indices[int(s.indptr[2]) + 9] = -5
+    out = torch.full((5, 2, 6), 99, dtype=torch.int32, device=dev)
+    B.select_blocks(q, bounds, steps, req, lens, s.indptr, indices, block=16, top=6, max_kvlen=400, out=out)
+    pages = list(s.pages[2])
+    pages[3], pages[9] = 10 ** 6, -5
+    for i, p in ((0, s.pages[0]), (2, pages)):
+        assert np.array_equal(out[i].cpu().numpy(), R.select(f64(q[i]), bounds.cpu().numpy(), steps.cpu().numpy(), p, 400, 16, 6, 1, 2))
+    assert (out[[1, 3, 4]] == 99).all()
+    # a row that claims more tokens than its request has pages, and one longer than max_kvlen says
+    B.select_blocks(q[:2], bounds, steps, torch.tensor([2, 1], device=dev), torch.tensor([900, 400], device=dev), s.indptr, s.indices, block=16, top=6, max_kvlen=900, out=out[:2])
+    assert np.array_equal(out[0].cpu().numpy(), R.select(f64(q[0]), bounds.cpu().numpy(), steps.cpu().numpy(), s.pages[2], 900, 16, 6, 1, 2))
+    B.select_blocks(q[:2], bounds, steps, torch.tensor([2, 1], device=dev), torch.tensor([400, 400], device=dev), s.indptr, s.indices, block=16, top=6, max_kvlen=200, out=out[:2])
+    assert np.array_equal(out[1].cpu().numpy(), R.select(f64(q[1]), bounds.cpu().numpy(), steps.cpu().numpy(), s.pages[1], 200, 16, 6, 1, 2))
+
+
+# ---------------------------------------------------------------- attend
+def check_attend(s, q, got, blocks, block, scale, rows=None):
+    step = torch.finfo(s.dtype).eps / 2
+    kv, lists = f64(s.kv), blocks.cpu().numpy()
+    for i in rows if rows is not None else range(s.n):
+        want, off = R.attend(f64(q[i]), kv, lists[i], s.pages[s.req[i]], s.kvlen[i], block, scale)
+        far = np.abs(f64(got[i]) - want)
+        assert (far <= step * np.abs(want) + off + torch.finfo(s.dtype).smallest_normal * step).all(), (i, float((far / (step * np.abs(want) + off + 1e-30)).max()))
+
+
+def random_lists(s, h, block, top, seed):
+    """Ascending lists of different lengths, empty ones among them."""
+    r = np.random.default_rng(seed)
+    out = np.full((s.n, h, top), -1, np.int32)
+    for i, n in enumerate(s.kvlen):
+        for g in range(h):
+            have = -(-n // block)
+            m = min(have, int(r.integers(0, top + 1)))
+            out[i, g, :m] = np.sort(r.permutation(have)[:m])
+    return torch.from_numpy(out).to(s.dev)
+
+
+ATTEND = [  # heads, kv heads, dim, page, block, top, kv lengths, new rows
+    (16, 8, 128, 128, 32, 8, [500, 33, 1, 256], [1, 1, 1, 1]),
+    (32, 2, 128, 64, 64, 6, [700, 64, 65], [1, 1, 1]),
+    (14, 2, 64, 48, 16, 9, [300, 120], [40, 23]),
+    (8, 8, 64, 16, 16, 20, [400], [70]),
+    (12, 4, 128, 32, 32, 7, [500, 90], [33, 5]),
+    (64, 2, 64, 16, 16, 5, [100, 40], [7, 1]),
+    (40, 1, 128, 32, 16, 12, [200, 90], [3, 1]),
+    (6, 2, 128, 128, 128, 5, [1000], [19]),
+    (4, 4, 64, 128, 128, 3, [130, 127, 129], [1, 2, 3]),
+    (32, 2, 128, 256, 128, 40, [6000, 3000], [1, 1]),        # much to read for few rows
+    (4, 2, 64, 16, 16, 130, [2500, 1800], [1, 1]),
+    (10, 2, 128, 16, 16, 64, [900, 700], [50, 37]),
+]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("hq,h,d,page,block,top,kv_lens,q_lens", ATTEND)
+def test_block_attention(dev, dtype, hq, h, d, page, block, top, kv_lens, q_lens):
+    from vox_serve_amd import block_attention as B
+    s = Paged(dev, TYPES[dtype], h, d, page, kv_lens, q_lens, seed=block + top)
+    wide = s.rnd(s.n, (hq + 3) * d)
+    q = wide[:, d:(hq + 1) * d].unflatten(1, (hq, d))         # rows apart
+    blocks = random_lists(s, h, block, top, top)
+    scale = d ** -0.5
+    for n_req in (0, len(q_lens)):
+        got = B.block_attention(q, s.kv, blocks, *s.plan, block=block, n_req=n_req)
+        check_attend(s, q, got, blocks, block, scale)
+    sharp = B.block_attention(q, s.kv, blocks, *s.plan, block=block, scale=1.0, n_req=len(q_lens))
+    check_attend(s, q, sharp, blocks, block, 1.0)
+
+
+@pytest.mark.parametrize("q_lens", [[1, 1, 1], [20, 9, 2]])
+@pytest.mark.parametrize("hq,h,d", [(8, 2, 128), (16, 1, 64), (4, 2, 64)])
+def test_attention_masked_places(dev, hq, h, d, q_lens):
+    """NaN, infinities and the type's lowest value behind a row's last token, in blocks that it does not list, and in pages that are nobody's
+    reach no row; where a row does see an infinity, its output is what the formula gives."""
+    from vox_serve_amd import block_attention as B
+    for dtype in (torch.bfloat16, torch.float16):
+        s = Paged(dev, dtype, h, d, 32, [200, 90, 37], q_lens, seed=d)
+        q = s.rnd(s.n, hq, d)
+        blocks = random_lists(s, h, 16, 6, 5)
+        want = B.block_attention(q, s.kv, blocks, *s.plan, block=16, n_req=3)
+        check_attend(s, q, want, blocks, 16, d ** -0.5)
+        # per request: tokens that none of its rows may see (behind the longest), then one row's own view of another's tokens
+        bad = s.kv.clone()
+        for fill in (float("nan"), float("inf"), float("-inf"), torch.finfo(dtype).min):
+            b = bad.clone()
+            owned = {p for pages in s.pages for p in pages}
+            for p in range(b.shape[0]):
+                if p not in owned:
+                    b[p] = fill
+            for r, n in enumerate(s.kv_lens):
+                for t in range(n, len(s.pages[r]) * 32):
+                    b[s.pages[r][t // 32], :, t % 32] = fill
+            assert torch.equal(B.block_attention(q, b, blocks, *s.plan, block=16, n_req=3), want)
+            # a request's newest token holds the fill: rows that see it feel it, the others do not
+            b = s.kv.clone()
+            n = s.kv_lens[0]
+            b[s.pages[0][(n - 1) // 32], :, (n - 1) % 32] = fill
+            got = B.block_attention(q, b, blocks, *s.plan, block=16, n_req=3)
+            feel = torch.tensor([[s.req[i] == 0 and s.kvlen[i] == n and (n - 1) // 16 in blocks[i, g].tolist() for g in range(h)] for i in range(s.n)], device=dev)
+            feel = feel.repeat_interleave(hq // h, 1)
+            assert torch.equal(got[~feel], want[~feel])
+            # a block that only one row lists
+            if s.n > 6:
+                lists = blocks.clone()
+                lists[lists == 1] = 2
+                lists[3, :, :] = -1
+                lists[3, :, 0] = 1
+                clean = B.block_attention(q, s.kv, lists, *s.plan, block=16, n_req=3)
+                b = s.kv.clone()
+                b[s.pages[0][0], :, 16:32] = fill
+                got = B.block_attention(q, b, lists, *s.plan, block=16, n_req=3)
+                others = [i for i in range(s.n) if i != 3]
+                assert torch.equal(got[others], clean[others])
+
+
+def test_attention_infinite_value_seen(dev):
+    """One infinite value in a seen token: +inf in that channel, the others untouched; a NaN key poisons its row's heads only."""
+    from vox_serve_amd import block_attention as B
+    s = Paged(dev, torch.bfloat16, 2, 64, 32, [64], [8], seed=1)
+    q = s.rnd(8, 4, 64)
+    blocks = torch.tensor([0, 1, 2, 3], dtype=torch.int32, device=dev).repeat(8, 2, 1)
+    clean = B.block_attention(q, s.kv, blocks, *s.plan, block=16, n_req=1)
+    s.kv[s.pages[0][0], 1, 3, 0, 5] = float("inf")
+    got = B.block_attention(q, s.kv, blocks, *s.plan, block=16, n_req=1)
+    assert torch.isposinf(got[:, :2, 5]).all()
+    keep = torch.ones(64, dtype=torch.bool)
+    keep[5] = False
+    assert torch.equal(got[:, :2, keep], clean[:, :2, keep]) and torch.equal(got[:, 2:], clean[:, 2:])
+    s.kv[s.pages[0][1], 0, 28, 1, 0] = float("nan")          # token 60: seen by the last four rows
+    got = B.block_attention(q, s.kv, blocks, *s.plan, block=16, n_req=1)
+    assert torch.isnan(got[4:, 2:]).all() and torch.equal(got[:4, 2:], clean[:4, 2:])
+
+
+def test_attention_entries_that_do_not_count(dev):
+    """Equal and smaller entries, blocks behind the row, pages that do not exist: as if they were not listed; rows that see nothing stay."""
+    from vox_serve_amd import block_attention as B
+    s = Paged(dev, torch.float16, 1, 64, 16, [100, 100, 100, 100], [1, 1, 1, 1], seed=3)
+    q = s.rnd(6, 4, 64)
+    odd = torch.tensor([[0, 0, 3, 3, 5, 2], [4, 1, 2, 5, 5, 6], [0, 2, 6, 7, 2000000000, 6], [-1, -1, 1, -1, 0, 2], [0, 1, 2, 3, 4, 5], [0, 1, 2, 3, 4, 5]], dtype=torch.int32, device=dev)
+    plain = torch.tensor([[0, 3, 5, -1, -1, -1], [4, 5, 6, -1, -1, -1], [0, 2, 6, -1, -1, -1], [1, 2, -1, -1, -1, -1]], dtype=torch.int32, device=dev)
+    req, lens = torch.tensor([0, 1, 2, 3, 0, 9], device=dev), torch.tensor([100, 100, 100, 100, 0, 100], device=dev)
+    for n_req in (0, 4, 6):
+        out = torch.full((6, 4, 64), 5.0, dtype=torch.float16, device=dev)
+        B.block_attention(q, s.kv, odd[:, None], req, lens, s.indptr, s.indices, block=16, n_req=n_req, out=out)
+        assert (out[4:] == 5).all()
+        check_attend(s, q, out, plain[:, None], 16, 0.125)
+        indices = s.indices.clone()
+        indices[0], indices[int(s.indptr[1]) + 4] = -1, 10 ** 8
+        out = torch.empty_like(out)
+        B.block_attention(q[:4], s.kv, plain[:, None], s.q_req, s.q_kvlen, s.indptr, indices, block=16, n_req=n_req, out=out[:4])
+        few = torch.tensor([[3, 5, -1, -1, -1, -1], [5, 6, -1, -1, -1, -1], [0, 2, 6, -1, -1, -1], [1, 2, -1, -1, -1, -1]], dtype=torch.int32, device=dev)
+        check_attend(s, q, out, few[:, None], 16, 0.125)
+    empty = B.block_attention(q[:4], s.kv, torch.full((4, 1, 3), -1, device=dev), *s.plan, block=16)
+    assert not empty.any()
+    assert not B.block_attention(q[:4], s.kv, torch.empty(4, 1, 0, dtype=torch.int32, device=dev), *s.plan, block=16).any()
+    assert B.block_attention(q[:0], s.kv, plain[:0, None], s.q_req[:0], s.q_kvlen[:0], s.indptr, s.indices, block=16).shape == (0, 4, 64)
+
+
+def test_all_blocks_are_dense_attention(dev):
+    from vox_serve_amd.flashinfer_utils import FlashInferPrefillWrapper
+    hq, h, d, page, q_lens, kv_lens = 16, 8, 128, 32, [40, 1, 75], [140, 90, 75]
+    need = [-(-n // page) for n in kv_lens]
+    g = torch.Generator().manual_seed(8)
+    kv = torch.randn(sum(need), 2, page, h, d, generator=g).bfloat16().to(dev)
+    q = torch.randn(sum(q_lens), hq, d, generator=g).bfloat16().to(dev)
+    w = FlashInferPrefillWrapper(None, hq, h, hq * d, page, device=dev)
+    i32 = lambda a: torch.tensor(a, dtype=torch.int32)
+    w.plan(i32([0, 40, 41, 116]), i32([0] + list(np.cumsum(need))), torch.randperm(sum(need), generator=g).int(), i32([n - (m - 1) * page for n, m in zip(kv_lens, need)]), torch.bfloat16)
+    from vox_serve_amd import block_attention as B
+    bounds, steps = B.new_bounds(kv, 16)
+    blocks = w.select_blocks(q, bounds, steps, top=16)
+    a, b = w.run_blocks(q, kv, blocks, 16).double(), w.run(q, kv).double()
+    # both are within half a step of the same value, and fp32's share of it
+    assert ((a - b).abs() <= 2.0 ** -7 * torch.maximum(a.abs(), b.abs()) + 2.0 ** -13).all()
+
+
+# ---------------------------------------------------------------- together
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_a_session(dev, dtype):
+    """A prompt in two chunks and then decoded tokens: rotated and appended, blocks chosen, attended - every step against the oracle, on a cache
+    and bounds that only these calls have written."""
+    from vox_serve_amd import block_attention as B
+    from vox_serve_amd.flashinfer_utils import FlashInferDecodeWrapper, FlashInferPrefillWrapper
+    hq, h, d, page, block, top = 8, 2, 64, 32, 16, 6
+    t, g = TYPES[dtype], torch.Generator().manual_seed(9)
+    kv = torch.zeros(24, 2, page, h, d, dtype=t, device=dev)
+    bounds, steps = B.new_bounds(kv, block)
+    pages, have = [list(range(0, 12)), list(range(12, 24))], [0, 0]
+    cs = table(dev, 512, d // 2)
+    i32 = lambda a: torch.tensor(a, dtype=torch.int32)
+    s = Paged(dev, t, h, d, page, [1, 1], [1, 1])
+
+    def step(new, wrapper):
+        for r in range(2):
+            have[r] += new[r]
+        need = [-(-n // page) for n in have]
+        args = (i32([0] + list(np.cumsum(need))), i32([p for r in range(2) for p in pages[r][:need[r]]]), i32([n - (m - 1) * page for n, m in zip(have, need)]), t)
+        if wrapper is FlashInferPrefillWrapper:
+            args = (i32([0] + list(np.cumsum(new))),) + args
+        w = wrapper(None, hq, h, hq * d, page, device=dev)
+        w.plan(*args)
+        rows = sum(new)
+        qkv = torch.randn(rows, (hq + 2 * h) * d, generator=g).to(t).to(dev)
+        q, k, v = (x.unflatten(1, (-1, d)) for x in qkv.split([hq * d, h * d, h * d], 1))
+        kvlen = [have[r] - new[r] + i + 1 for r in range(2) for i in range(new[r])]
+        pos = torch.tensor(kvlen, device=dev) - 1
+        qr = w.set_kv_cache_rope(kv, q, k, v, pos, cs, bounds=bounds, steps=steps)
+        blocks = w.select_blocks(qr, bounds, steps, top)
+        out = w.run_blocks(qr, kv, blocks, block)
+        s.kv, s.req, s.kvlen, s.n, s.pages = kv, [r for r in range(2) for _ in range(new[r])], kvlen, rows, pages
+        for r in range(2):                                    # every complete block's bounds are those of its keys
+            for j in range(have[r] // block):
+                p = pages[r][j * block // page]
+                at = j * block % page
+                for gh in range(h):
+                    wb, ws = R.bounds(f64(kv[p, 0, at:at + block, gh]))
+                    assert np.array_equal(bounds[p, gh, at // block].cpu().numpy(), wb) and float(steps[p, gh, at // block]) == ws
+        nb, ns = bounds.cpu().numpy(), steps.cpu().numpy()
+        for i in range(rows):
+            assert np.array_equal(blocks[i].cpu().numpy(), R.select(f64(qr[i]), nb, ns, pages[s.req[i]], kvlen[i], block, top, 1, 2))
+        check_attend(s, qr, out, blocks, block, d ** -0.5)
+
+    step([70, 101], FlashInferPrefillWrapper)
+    step([90, 13], FlashInferPrefillWrapper)
+    for _ in range(20):
+        step([1, 1], FlashInferDecodeWrapper)
+
+
+@pytest.mark.parametrize("rows", [3, 64])
+def test_captured_steps(dev, rows):
+    """The three operators captured together, replayed with new inputs and eager calls of other sizes between: every replay is the eager result."""
+    from vox_serve_amd import _native as N
+    from vox_serve_amd import block_attention as B
+    hq, h, d, page, block, top = 16, 8, 128, 64, 16, 12
+    q_lens = [1] * 3 if rows == 3 else [60, 1, 3]
+    s = Paged(dev, torch.bfloat16, h, d, page, [600, 333, 128], q_lens, seed=rows)
+    qkv = s.rnd(s.n, (hq + 2 * h) * d)
+    q, k, v = (x.unflatten(1, (-1, d)) for x in qkv.split([hq * d, h * d, h * d], 1))
+    pos, cs = s.q_kvlen - 1, table(dev, 1024, d // 2)
+    bounds, steps = s.bounds(block)
+    qr, blocks, out = torch.empty(s.n, hq, d, dtype=s.dtype, device=dev), torch.empty(s.n, h, top, dtype=torch.int32, device=dev), torch.empty(s.n, hq, d, dtype=s.dtype, device=dev)
+
+    def calls(kv, b, st, qr, blocks, out):
+        B.rope_append(q, k, v, kv, cs, pos, s.row_page, s.row_slot, bounds=b, steps=st, n_req=3, out=qr)
+        B.select_blocks(qr, b, st, *s.plan, block=block, top=top, max_kvlen=600, n_req=3, out=blocks)
+        B.block_attention(qr, kv, blocks, *s.plan, block=block, n_req=3, out=out)
+
+    calls(s.kv, bounds, steps, qr, blocks, out)
+    graphs = []
+    for _ in range(2):
+        with N.graph_capture() as cap:
+            calls(s.kv, bounds, steps, qr, blocks, out)
+        graphs.append(cap.graph)
+    other = Paged(dev, torch.bfloat16, h, d, page, [2000], [1], seed=7)
+    ob, os_ = other.bounds(block)
+    oq = other.rnd(1, hq, d)
+    for i in range(6):
+        qkv.copy_(s.rnd(*qkv.shape))
+        kv2, b2, s2 = s.kv.clone(), bounds.clone(), steps.clone()
+        N.check(N.lib().vox_graph_launch(graphs[i % 2], N.stream()))
+        got = [x.clone() for x in (qr, blocks, out, s.kv, bounds, steps)]
+        B.block_attention(oq, other.kv, B.select_blocks(oq, ob, os_, *other.plan, block=block, top=100, max_kvlen=2000, n_req=1), *other.plan, block=block, n_req=1)
+        want = [torch.empty_like(x) for x in (qr, blocks, out)]
+        calls(kv2, b2, s2, *want)
+        torch.cuda.synchronize()
+        for x, y in zip(got, want + [kv2, b2, s2]):
+            assert torch.equal(x, y)
+    for gr in graphs:
+        N.lib().vox_graph_destroy(gr)
+
+
+def test_on_another_stream_and_two_at_once(dev):
+    from vox_serve_amd import block_attention as B
+    s = Paged(dev, torch.bfloat16, 2, 128, 128, [9000, 9000], [1, 1], seed=6)
+    q = s.rnd(2, 32, 128)
+    bounds, steps = B.new_bounds(s.kv, 128)
+    B.update_bounds(s.kv, bounds, steps, torch.arange(s.kv.shape[0], device=dev), torch.full((s.kv.shape[0],), 127, device=dev))
+    want_b = B.select_blocks(q, bounds, steps, *s.plan, block=128, top=60, max_kvlen=9000, n_req=2)
+    want = B.block_attention(q, s.kv, want_b, *s.plan, block=128, n_req=2)
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    for _ in range(4):
+        for st in streams:
+            with torch.cuda.stream(st):
+                b = B.select_blocks(q, bounds, steps, *s.plan, block=128, top=60, max_kvlen=9000, n_req=2)
+                got.append((b, B.block_attention(q, s.kv, b, *s.plan, block=128, n_req=2)))
+    torch.cuda.synchronize()
+    for b, o in got:
+        assert torch.equal(b, want_b) and torch.equal(o, want)
+
+
+def test_results_do_not_depend_on_the_batch(dev):
+    """The choice and the appended rows of a request are the same alone and among others."""
+    from vox_serve_amd import block_attention as B
+    s = Paged(dev, torch.bfloat16, 8, 128, 64, [3000, 1700, 900], [1, 1, 1], seed=12)
+    q = s.rnd(3, 16, 128)
+    bounds, steps = B.new_bounds(s.kv, 32)
+    where = torch.arange(s.kv.shape[0], device=dev).repeat_interleave(2), torch.tensor([31, 63], device=dev).repeat(s.kv.shape[0])
+    B.update_bounds(s.kv, bounds, steps, *where)
+    every = B.select_blocks(q, bounds, steps, *s.plan, block=32, top=20, max_kvlen=3000, n_req=3)
+    for i in range(3):
+        one = B.select_blocks(q[i:i + 1], bounds, steps, s.q_req[i:i + 1], s.q_kvlen[i:i + 1], s.indptr, s.indices, block=32, top=20, max_kvlen=s.kvlen[i], n_req=1)
+        assert torch.equal(one[0], every[i])
+
+
+def test_offsets_beyond_32_bits(dev):
+    """Pages whose elements lie more than 2^32 bytes, and 2^31 elements, behind the cache's start."""
+    from vox_serve_amd import block_attention as B
+    page, h, d = 128, 8, 128
+    total = 2 ** 31 // (2 * page * h * d) + 9
+    kv = torch.empty(total, 2, page, h, d, dtype=torch.bfloat16, device=dev)
+    s = Paged(dev, torch.bfloat16, h, d, page, [128 * 8], [1], seed=5, spare=0)
+    far = [total - 1 - i for i in range(8)]
+    for i, p in enumerate(far):
+        kv[p] = s.kv[s.pages[0][i]]
+    small_b, small_s = B.new_bounds(s.kv, 16)
+    slots = torch.arange(15, 128, 16, device=dev)
+    B.update_bounds(s.kv, small_b, small_s, torch.tensor(s.pages[0], device=dev).repeat_interleave(8), slots.repeat(8))
+    bounds, steps = B.new_bounds(kv, 16)
+    B.update_bounds(kv, bounds, steps, torch.tensor(far, device=dev).repeat_interleave(8), slots.repeat(8))
+    assert torch.equal(bounds[far], small_b[s.pages[0]]) and torch.equal(steps[far], small_s[s.pages[0]])
+    q, indices = s.rnd(1, 16, d), torch.tensor(far, dtype=torch.int32, device=dev)
+    want_b = B.select_blocks(q, small_b, small_s, *s.plan, block=16, top=20, max_kvlen=1024, n_req=1)
+    got_b = B.select_blocks(q, bounds, steps, s.q_req, s.q_kvlen, s.indptr, indices, block=16, top=20, max_kvlen=1024, n_req=1)
+    assert torch.equal(want_b, got_b)
+    assert torch.equal(B.block_attention(q, s.kv, want_b, *s.plan, block=16, n_req=1), B.block_attention(q, kv, got_b, s.q_req, s.q_kvlen, s.indptr, indices, block=16, n_req=1))
+    k = s.rnd(1, h, d)
+    B.rope_append(q, k, k, kv, None, s.q_kvlen, torch.tensor([total - 1], device=dev), torch.tensor([100], device=dev))
+    assert torch.equal(kv[total - 1, :, 100], k.expand(2, -1, -1))

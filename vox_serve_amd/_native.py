@@ -82,6 +82,12 @@ _SIGS = {
                                     c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float]),
     "vox_paged_attention_of": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                        c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int]),
+    "vox_rope_append": (c_int, [c_void_p, c_void_p, c_char_p]),             # (the argument structs travel as packed bytes: block_attention.py)
+    "vox_block_bounds": (c_int, [c_void_p, c_void_p, c_char_p, c_void_p, c_void_p, c_int]),
+    "vox_block_select_workspace_bytes": (c_int64, [c_char_p]),
+    "vox_block_select": (c_int, [c_void_p, c_void_p, c_char_p]),
+    "vox_block_attention_workspace_bytes": (c_int64, [c_char_p]),
+    "vox_block_attention": (c_int, [c_void_p, c_void_p, c_char_p]),
     "vox_attention_form": (c_int, [c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
     "vox_linear": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
                            c_int]),

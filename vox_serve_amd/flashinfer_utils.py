@@ -8,6 +8,9 @@ FlashInfer, no Triton.
                               .token_to_page, .token_to_cache, .head_dim)
   FlashInferDecodeWrapper     flashinfer_utils.py:149-244 (plan / run / set_kv_cache, .kv_cache_locations)
 
+Beyond the reference, both wrappers hand the same plan to the operators of `block_attention`: set_kv_cache_rope (rotate and append in one
+call), update_bounds, select_blocks and run_blocks (attention over the blocks that were chosen).
+
 plan() takes CPU int32 tensors like the reference and uploads them with an async copy; unlike the
 reference it needs no device synchronisation afterwards (the caller's `torch.cuda.synchronize()` is
 harmless but unnecessary).
@@ -17,6 +20,7 @@ from typing import Union
 import torch
 
 from . import _native as N
+from . import block_attention
 
 _ROPE_TABLES = {}
 
@@ -95,6 +99,27 @@ class _PagedBase:
         N.check(N.lib().vox_kv_append(N.ctx(), N.stream(), N.ptr(kv_cache), N.ptr(k), N.ptr(v), N.ptr(page),
                                       N.ptr(slot), k.shape[0], kv_cache.shape[2], self.n_kv_head, self.head_dim))
 
+    # ---- long contexts: the operators of block_attention, with this plan's rows
+    def set_kv_cache_rope(self, kv_cache, q, k, v, position_ids, cos_sin, interleave=False, bounds=None, steps=None, out=None):
+        """apply_rope_pos_ids and set_kv_cache in one call, from slices of one projection's output if need be; returns the rotated q."""
+        m = self._meta
+        return block_attention.rope_append(q, k, v, kv_cache, cos_sin, position_ids, m["page"], m["slot"], interleave=interleave, bounds=bounds, steps=steps,
+                                           n_req=m["n_own"], out=out)
+
+    def update_bounds(self, kv_cache, bounds, steps):
+        """The bounds of the blocks that the planned rows complete, behind set_kv_cache."""
+        block_attention.update_bounds(kv_cache, bounds, steps, self._meta["page"], self._meta["slot"])
+
+    def select_blocks(self, q, bounds, steps, top, first=1, last=2, out=None):
+        m = self._meta
+        return block_attention.select_blocks(q, bounds, steps, m["q_req"], m["q_kvlen"], m["indptr"], m["indices"], block=self.page_size // bounds.shape[2], top=top,
+                                             max_kvlen=m["max_kvlen"], first=first, last=last, n_req=m["n_own"], out=out)
+
+    def run_blocks(self, q, kv_cache, blocks, block, out=None):
+        """Attention as `run`, over the listed blocks of `block` tokens only."""
+        m = self._meta
+        return block_attention.block_attention(q, kv_cache, blocks, m["q_req"], m["q_kvlen"], m["indptr"], m["indices"], block=block, n_req=m["n_own"], out=out)
+
 
 class FlashInferPrefillWrapper(_PagedBase):
     def __init__(self, attn_buffer=None, n_qo_head=None, n_kv_head=None, n_state=None, page_size=None, batch_size=None,
@@ -143,7 +168,7 @@ class FlashInferPrefillWrapper(_PagedBase):
         self._meta = dict(q_req=q_req.to(dev), q_kvlen=q_kvlen.to(dev), page=page32, slot=slot32,
                           indptr=paged_kv_indptr.to(device=dev, dtype=torch.int32),
                           indices=paged_kv_indices.to(device=dev, dtype=torch.int32),
-                          max_kvlen=int(kv_len.max()) if n_req else 1, n_req=n_req)
+                          max_kvlen=int(kv_len.max()) if n_req else 1, n_req=n_req, n_own=int((lens > 0).sum()))
 
     def run(self, q, kv_cache):
         return self._run(q, kv_cache)
@@ -181,7 +206,7 @@ class FlashInferDecodeWrapper(_PagedBase):
                           page=page_idx.to(device=dev, dtype=torch.int32), slot=pos_idx.to(device=dev, dtype=torch.int32),
                           indptr=paged_kv_indptr.to(device=dev, dtype=torch.int32),
                           indices=paged_kv_indices.to(device=dev, dtype=torch.int32),
-                          max_kvlen=int(kv_len.max()) if b else 1, n_req=b)
+                          max_kvlen=int(kv_len.max()) if b else 1, n_req=b, n_own=b)
 
     def run(self, q, kv_cache):
         return self._run(q, kv_cache)

@@ -563,6 +563,33 @@ def test_on_another_stream_and_two_at_once(dev):
         assert torch.equal(b, want_b) and torch.equal(o, want)
 
 
+def test_two_graphs_at_once(dev):
+    """Two graphs of split calls, captured one behind the other and replayed on two streams beside eager calls: neither reaches the other's workspace."""
+    from vox_serve_amd import _native as N
+    from vox_serve_amd import block_attention as B
+    sets = []
+    for seed in (1, 2):
+        s = Paged(dev, torch.bfloat16, 2, 128, 128, [9000, 9000], [1, 1], seed=seed)
+        q, blocks = s.rnd(2, 32, 128), torch.arange(60, dtype=torch.int32, device=dev).repeat(2, 2, 1).contiguous()
+        out = torch.empty_like(q)
+        want = B.block_attention(q, s.kv, blocks, *s.plan, block=128, n_req=2)
+        torch.cuda.synchronize()
+        with N.graph_capture() as cap:
+            B.block_attention(q, s.kv, blocks, *s.plan, block=128, n_req=2, out=out)
+        sets.append((s, q, blocks, out, want, cap.graph, torch.cuda.Stream()))
+    for _ in range(10):
+        for s, q, blocks, out, want, graph, st in sets:
+            with torch.cuda.stream(st):
+                out.zero_()
+                N.check(N.lib().vox_graph_launch(graph, N.stream()))
+        eager = [B.block_attention(q, s.kv, blocks, *s.plan, block=128, n_req=2) for s, q, blocks, *_ in sets]
+        torch.cuda.synchronize()
+        for e, (_, _, _, out, want, *_) in zip(eager, sets):
+            assert torch.equal(out, want) and torch.equal(e, want)
+    for x in sets:
+        N.lib().vox_graph_destroy(x[5])
+
+
 def test_results_do_not_depend_on_the_batch(dev):
     """The choice and the appended rows of a request are the same alone and among others."""
     from vox_serve_amd import block_attention as B

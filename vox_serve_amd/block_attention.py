@@ -13,6 +13,7 @@ A cache layer is [pages, 2, page, kv heads, dim] in bf16 or fp16, dim 64 or 128,
 `steps` (fp32 [pages, kv heads, blocks a page], powers of two).  Integer plan arrays are int32 (int64 is converted).  Rows whose page is
 negative, or that see no token, are passed over: what would have been written for them stays as it was.
 """
+import functools
 import struct
 
 import torch
@@ -32,6 +33,26 @@ def _on(device):
     """Context and stream of the device that is current; tensors elsewhere are refused by the callers."""
     h = N._ctxs.get(device.index)
     return (h or N.ctx()), torch.cuda.current_stream().cuda_stream
+
+
+_kept = []                               # workspaces that captured graphs go back to
+
+
+@functools.lru_cache(maxsize=4096)
+def _attend_room(*sizes):
+    """Bytes of workspace that a call of these sizes asks for: a function of the sizes alone."""
+    rows, n_own, heads, kv_heads, dim, dtype, page, block, top = sizes
+    n = N.lib().vox_block_attention_workspace_bytes(_ATTEND.pack(16, 0, 0, 1, page, block, kv_heads, dim, dtype, 16, 16, 16, 16, rows, 1, n_own, heads, 1, 0, 16, 16, 16, 0, 0, 0, top, 1.0))
+    return max(n, 0)                    # (sizes that the call itself will refuse)
+
+
+def _workspace(n, device):
+    """A buffer for one call.  Eagerly the allocator's stream order makes it safe to let go of behind the call; a call that a `graph_capture` records keeps
+    its own for good, so that no two graphs, and no graph and eager call, ever share one (torch's own graphs keep theirs by their pool)."""
+    t = torch.empty(n, dtype=torch.uint8, device=device)
+    if device.index in N._capturing:
+        _kept.append(t)
+    return t
 
 
 def _device(t, name):
@@ -210,8 +231,10 @@ def block_attention(q, kv_cache, blocks, q_req, q_kvlen, kv_indptr, kv_indices, 
     plan = _plan(q_req, q_kvlen, kv_indptr, kv_indices, rows, device)
     out = _out(out, q.shape, kv_cache.dtype, device)
     ctx, stream = _on(device)
+    room = _attend_room(rows, n_req, q.shape[1], h, d, _DTYPES[kv_cache.dtype], page, block, top)
+    ws = _workspace(room, device) if room else None
     N.check(N.lib().vox_block_attention(ctx, stream, _ATTEND.pack(
         kv_cache.data_ptr(), 0, 0, n_pages, page, block, h, d, _DTYPES[kv_cache.dtype], plan[0].data_ptr(), plan[1].data_ptr(), plan[2].data_ptr(),
-        plan[3].data_ptr(), rows, plan[2].shape[0] - 1, n_req, q.shape[1], 2 ** 31 - 1, 0, q.data_ptr(), blocks.data_ptr(), out.data_ptr(), 0, 0, q.stride(0),
-        top, d ** -0.5 if scale is None else scale)))
+        plan[3].data_ptr(), rows, plan[2].shape[0] - 1, n_req, q.shape[1], 2 ** 31 - 1, 0, q.data_ptr(), blocks.data_ptr(), out.data_ptr(),
+        ws.data_ptr() if room else 0, room, q.stride(0), top, d ** -0.5 if scale is None else scale)))
     return out

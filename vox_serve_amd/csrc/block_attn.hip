@@ -270,65 +270,407 @@ __global__ __launch_bounds__(256) void k_block_select(SelectArgs a) {
 // ================================================================================================
 // attend
 // ================================================================================================
+// Sixteen columns - the query heads of one kv head (up to 16 of them), of one row or of as many neighbouring rows of a request as fit - meet the blocks that
+// any of their rows lists, 32 tokens at a time: two tiles of 16, of one block or of two.
+//   S^T = K Q^T     A: a token a lane, 8 channels; lane (c, g) then holds the scores of column c = lane % 16 for tokens 4 g .. 4 g + 3 (g = lane / 16) of each tile,
+//   O^T = V^T P^T   B: these same scores' weights, where they are - the order of the 32 tokens inside a product is free, so V's lanes take tokens 4 g ..
+//                   4 g + 3 of each tile too.  A lane loads 8 neighbouring channels (D = 128) of its 8 tokens, whole rows a sixteen lanes, and a tile t of
+//                   the product takes channel 8 m + t of each: halves of registers by v_perm, no LDS.
+// Maximum and sum of a column stay with its lanes (online softmax, exponents of two, fp32).  A weight enters as the sum of two 16-bit terms: one alone would
+// cost as much precision as the output's own rounding.
+// What a column must not see is kept from it by its score alone (weight 0), which holds as long as V is finite; where a result is not, the rows are gone through
+// again one by one in the same order with V's masked tokens as zero, and a value that is not finite multiplied by the weight as one term (an infinity times the
+// two terms would be inf - inf).  Rows that see no such value come out bit for bit as if it were not there.
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef half_t f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+template <int F16>
+__device__ __forceinline__ f32x4 mma32(uint4 a, uint4 b, f32x4 c) {
+    if constexpr (F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+template <int F16>
+__device__ __forceinline__ u32 pack2(float lo, float hi) {
+    if constexpr (F16) return (u32)f_elem<1>(lo) | ((u32)f_elem<1>(hi) << 16);
+    else return pack_bf2(lo, hi);
+}
+template <int OFF>                       // 16 or 32
+__device__ __forceinline__ float xor_max(float s) {
+    vox_u2 r;
+    if constexpr (OFF == 32) r = __builtin_amdgcn_permlane32_swap(__float_as_uint(s), __float_as_uint(s), false, false);
+    else r = __builtin_amdgcn_permlane16_swap(__float_as_uint(s), __float_as_uint(s), false, false);
+    return fmaxf(__uint_as_float(r.x), __uint_as_float(r.y));
+}
+template <int F16>
+__device__ __forceinline__ u32 halves_not_finite(u32 w) {          // 0xffff where a half is an infinity or NaN
+    const u32 e = F16 ? 0x7c00u : 0x7f80u;
+    return ((w & e) == e ? 0xffffu : 0u) | ((w >> 16 & e) == e ? 0xffff0000u : 0u);
+}
+
 struct BlockAttnArgs {
     const bf16_t *q, *kv;
     const int *q_req, *q_kvlen, *indptr, *indices, *blocks;
     bf16_t* out;
+    float *part_o, *part_ml;             // splits > 1: [row][head][split][D], [row][head][split][2]
     long q_stride;
-    float scale;
+    float scale2;                        // scale log2 e
     int n_rows, n_req, Hq, Hkv, max_kvlen, n_pages, page_size, block, top;
+    int per_tile, splits, head_tiles, cols, q_al, out_al;      // cols: columns of a wave in the merge's LDS
 };
-// one wave a row and query head: 64 tokens at a time, a token a lane for the scores, D / 64 channels a lane for the values
-template <int F16, int D>
-__global__ __launch_bounds__(64) void k_block_attention(BlockAttnArgs a) {
-    __shared__ float q[D];
-    const int i = blockIdx.x, hq = blockIdx.y, lane = threadIdx.x, h = hq / (a.Hq / a.Hkv);
-    int n = a.q_kvlen[i];
-    const int r = a.q_req[i];
-    if (n <= 0 || r < 0 || r >= a.n_req) return;
-    n = min(n, a.max_kvlen);
-    const float inf = __uint_as_float(0x7f800000u);
-    for (int d = lane; d < D; d += 64) q[d] = elem_f<F16>(a.q[(size_t)i * a.q_stride + (size_t)hq * D + d]);
-    __syncthreads();
-    const int* const list = a.blocks + ((size_t)i * a.Hkv + h) * a.top;
-    const int per = a.page_size / a.block, p0 = a.indptr[r], np = a.indptr[r + 1] - p0, have = (n + a.block - 1) / a.block;
-    float m = -inf, l = 0.0f, o[D / 64] = {};
-    int seen = -1;
-    for (int e = 0; e < a.top; ++e) {
-        const int j = list[e];
-        if (j <= seen) continue;
-        seen = j;
-        if (j >= have || j / per >= np) continue;
-        const int pg = a.indices[p0 + j / per];
-        if (pg < 0 || pg >= a.n_pages) continue;
-        const size_t base = ((size_t)pg * 2 * a.page_size + (size_t)(j % per) * a.block) * a.Hkv * D + (size_t)h * D;
-        const int len = min(a.block, n - j * a.block);
-        for (int t0 = 0; t0 < len; t0 += 64) {
-            const int t = t0 + lane;
-            float s = -inf;
-            if (t < len) {
-                const bf16_t* const k = a.kv + base + (size_t)t * a.Hkv * D;
-                float z = 0.0f;
-                for (int d = 0; d < D; ++d) z = __fmaf_rn(q[d], elem_f<F16>(k[d]), z);
-                s = z * a.scale;
+#define ATTN_CUS 256                     // of an MI355X
+#define ATTN_WINDOW 4096                 // blocks whose rows' bits lie in LDS at a time (rows of several: 8 KB)
+
+// The entries of a row's list that count, 64 at a time, by one wave: f(j, counts) for every lane.
+template <class F>
+__device__ __forceinline__ void row_entries(const int* list, int top, int have, int lane, F f) {
+    int carry = -1;
+    for (int e0 = 0; e0 < top; e0 += 64) {
+        const int j = e0 + lane < top ? list[e0 + lane] : -1;
+        int most = j;                                                // the largest entry up to this one
+        const int prev = __shfl_up(j, 1, 64);
+        if (__ballot(lane && j >= 0 && j <= prev) || __ballot(lane && j >= 0 && prev < 0))      // (not simply ascending)
+            for (int o = 1; o < 64; o <<= 1) {
+                const int x = __shfl_up(most, o, 64);
+                if (lane >= o) most = max(most, x);
             }
-            float top = s;
-            for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x, 64));
-            const float now = fmaxf(m, top);
-            const float keep = m == -inf ? 0.0f : expf(m - now), p = t < len ? expf(s - now) : 0.0f;
-            float all = p;
-            for (int x = 1; x < 64; x <<= 1) all += __shfl_xor(all, x, 64);
-            l = l * keep + all;
-            m = now;
-            for (int x = 0; x < D / 64; ++x) o[x] *= keep;
-            const bf16_t* const v = a.kv + base + (size_t)a.page_size * a.Hkv * D;
-            for (int t1 = 0; t1 < min(64, len - t0); ++t1) {
-                const float w = __shfl(p, t1, 64);
-                for (int x = 0; x < D / 64; ++x) o[x] = __fmaf_rn(w, elem_f<F16>(v[(size_t)(t0 + t1) * a.Hkv * D + lane + 64 * x]), o[x]);
-            }
+        int before = __shfl_up(most, 1, 64);
+        before = lane ? max(before, carry) : carry;
+        f(j, j >= 0 && j > before && j < have);
+        if (e0 + 64 < top) {                                         // the carry of the next 64
+            int last = j;
+            for (int o = 1; o < 64; o <<= 1) last = max(last, __shfl_xor(last, o, 64));
+            carry = max(carry, last);
         }
     }
-    for (int x = 0; x < D / 64; ++x) a.out[((size_t)i * a.Hq + hq) * D + lane + 64 * x] = f_elem<F16>(seen >= 0 && l != 0.0f ? o[x] / l : 0.0f);
+}
+
+template <int F16, int D, int W, bool ONE>
+__global__ __launch_bounds__(64 * W, W == 4 ? 2 : 1) void k_block_attn(BlockAttnArgs a) {
+    constexpr int CPL = D / 16, KS = D / 32, OS = D + 4;             // channels a lane, steps of a K row, floats a column of the merge
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    __shared__ int s_len[16], s_req[16], s_count[W + 1], s_next, s_seen;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
+    const float inf = __uint_as_float(0x7f800000u);
+    // block -> (kv head, tile of heads, split, tile of rows): neighbours are kv heads, so that a die's L2 keeps its heads' tokens
+    int id = blockIdx.x;
+    const int h = id % a.Hkv; id /= a.Hkv;
+    const int ht = id % a.head_tiles; id /= a.head_tiles;
+    const int split = id % a.splits, tile = id / a.splits;
+    const int G = a.Hq / a.Hkv, h0 = ht * 16, gh = min(G - h0, 16);  // this tile's heads
+    const int i0 = tile * a.per_tile, R = min(a.per_tile, a.n_rows - i0);
+    if (tid < 16) {
+        int len = 0, req = -1;
+        if (tid < R) {
+            len = a.q_kvlen[i0 + tid];
+            req = a.q_req[i0 + tid];
+            if (len <= 0 || req < 0 || req >= a.n_req) { len = 0; req = -1; }
+            len = min(len, a.max_kvlen);
+        }
+        s_len[tid] = len; s_req[tid] = req;
+    }
+    __syncthreads();
+    const int rc = ONE ? 0 : c / gh, hc = ONE ? c : c % gh;          // the column's row and head
+    const bool col = ONE ? c < gh : rc < R;
+    uint4 q[KS];
+    {
+        const bf16_t* const src = a.q + (size_t)(i0 + (col ? rc : 0)) * a.q_stride + (size_t)(h * G + h0 + (col ? hc : 0)) * D + 8 * g;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            if (a.q_al) q[s] = *reinterpret_cast<const uint4*>(src + 32 * s);
+            else {
+                u32 w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = (u32)src[32 * s + 2 * i] | ((u32)src[32 * s + 2 * i + 1] << 16);
+                q[s] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+            if (!col) q[s] = make_uint4(0, 0, 0, 0);
+        }
+    }
+    const int sub_shift = a.block == 16 ? 0 : a.block == 32 ? 1 : a.block == 64 ? 2 : 3, per = a.page_size / a.block;
+    const size_t row_el = (size_t)a.Hkv * D;                         // elements between tokens
+    int2* const s_list = reinterpret_cast<int2*>(lds);               // {block (from the window's first) << 16 | rows, or the block (ONE); page}
+    u32* const s_bits = reinterpret_cast<u32*>(lds);                 // rows of several: two blocks' rows a word, in front of the list
+    int2* const list = ONE ? s_list : s_list + ATTN_WINDOW / 4;
+    float* const s_o = reinterpret_cast<float*>(lds);                // after the loop: [wave][column][OS]
+    float* const s_ml = s_o + W * a.cols * OS;                           // [wave][column] maximum, sum
+
+    for (int ra = 0; ra < R;) {
+        if (s_req[ra] < 0) { ++ra; continue; }                       // (all of the block's threads read the same LDS words)
+        int rb = ra + 1;
+        while (rb < R && s_req[rb] == s_req[ra]) ++rb;
+        const int req = s_req[ra], p0 = a.indptr[req], np = a.indptr[req + 1] - p0;
+        int n_most = 0, n_least = 0x7fffffff;
+        for (int r = ra; r < rb; ++r) { n_most = max(n_most, s_len[r]); n_least = min(n_least, s_len[r]); }
+        const u32 all_rows = (rb == 32 ? 0u : 1u << rb) - (1u << ra);
+        const int own = ONE ? s_len[ra] : col && rc >= ra && rc < rb ? s_len[rc] : 0;
+
+        for (int careful = -1;;) {                                   // -1, then, if need be, the run's rows one by one
+            float m = -inf, l = 0.0f;
+            f32x4 o[CPL];
+#pragma unroll
+            for (int t = 0; t < CPL; ++t) o[t] = f32x4{0, 0, 0, 0};
+            const int v_len = careful >= 0 ? s_len[careful] : n_most;     // V of tokens from here on is taken as zero
+            if (tid == 0) s_seen = 0;
+            __syncthreads();
+
+            for (int w0 = 0; w0 >= 0;) {                             // windows of blocks (ONE: one, of everything)
+                int count;
+                if constexpr (ONE) {
+                    if (wave == 0) {
+                        int at = 0;
+                        row_entries(a.blocks + ((size_t)i0 * a.Hkv + h) * a.top, a.top, (n_most + a.block - 1) / a.block, lane, [&](int j, bool ok) {
+                            int pg = -1;
+                            if (ok && j / per < np) pg = a.indices[p0 + j / per];
+                            ok = pg >= 0 && pg < a.n_pages;
+                            const unsigned long long b = __ballot(ok);
+                            if (ok) list[at + __popcll(b & ((1ull << lane) - 1))] = make_int2(j, pg);
+                            at += __popcll(b);
+                        });
+                        if (lane == 0) s_count[0] = at;
+                    }
+                    __syncthreads();
+                    count = s_count[0];
+                    if (tid == 0 && count) s_seen = 1;
+                    w0 = -1;
+                } else {
+                    for (int i = tid; i < ATTN_WINDOW / 2; i += 64 * W) s_bits[i] = 0;
+                    if (tid == 0) s_next = 0x7fffffff;
+                    __syncthreads();
+                    for (int r = ra + wave; r < rb; r += W)
+                        row_entries(a.blocks + ((size_t)(i0 + r) * a.Hkv + h) * a.top, a.top, (s_len[r] + a.block - 1) / a.block, lane, [&](int j, bool ok) {
+                            if (!ok || j < w0) return;
+                            if (j - w0 < ATTN_WINDOW) atomicOr(&s_bits[(j - w0) >> 1], 1u << (r + 16 * ((j - w0) & 1)));
+                            else atomicMin(&s_next, j);
+                        });
+                    __syncthreads();
+                    // the window's blocks in order: a thread counts its neighbours' share
+                    constexpr int WPT = ATTN_WINDOW / 2 / (64 * W);
+                    u32 bits[WPT];
+                    int mine = 0;
+#pragma unroll
+                    for (int i = 0; i < WPT; ++i) {
+                        bits[i] = s_bits[tid * WPT + i];
+                        mine += (bits[i] & 0xffffu ? 1 : 0) + (bits[i] >> 16 ? 1 : 0);
+                    }
+                    int upto = mine;
+                    for (int x = 1; x < 64; x <<= 1) {
+                        const int y = __shfl_up(upto, x, 64);
+                        if (lane >= x) upto += y;
+                    }
+                    if (lane == 63) s_count[wave] = upto;
+                    __syncthreads();
+                    int at = upto - mine;
+                    count = 0;
+                    for (int x = 0; x < W; ++x) { if (x < wave) at += s_count[x]; count += s_count[x]; }
+                    u32 seen = 0;
+#pragma unroll
+                    for (int i = 0; i < WPT; ++i)
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            u32 rows = half ? bits[i] >> 16 : bits[i] & 0xffffu;
+                            if (!rows) continue;
+                            const int off = (tid * WPT + i) * 2 + half, j = w0 + off;
+                            int pg = j / per < np ? a.indices[p0 + j / per] : -1;
+                            if (pg < 0 || pg >= a.n_pages) { pg = 0; rows = 0; }      // (nobody's: page 0 is read and masked)
+                            list[at++] = make_int2((int)((u32)off << 16 | rows), pg);
+                            seen |= rows;
+                        }
+                    if (seen) atomicOr(&s_seen, (int)seen);
+                    __syncthreads();
+                }
+                const int units = ((count << sub_shift) + 1) / 2;
+                const int u0 = ONE ? (int)((long)units * split / a.splits) : 0, u1 = ONE ? (int)((long)units * (split + 1) / a.splits) : units;
+                for (int u = u0 + wave; u < u1; u += W) {
+                    // two tiles of 16 tokens
+                    uint4 k[2][KS];
+                    u32 v[2][4][CPL / 2];
+                    int tok[2];
+                    u32 rows[2];
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const int sub = 2 * u + x, e = min(sub >> sub_shift, count - 1), part = sub & ((1 << sub_shift) - 1);
+                        const int2 ent = list[e];
+                        const int j = ONE ? ent.x : w0 + (int)((u32)ent.x >> 16);
+                        rows[x] = (sub >> sub_shift) < count ? (ONE ? 1u : (u32)ent.x & 0xffffu) : 0u;      // (the odd last tile of blocks of 16: nobody's)
+                        tok[x] = j * a.block + 16 * part;
+                        const bf16_t* const kb = a.kv + ((size_t)ent.y * 2 * a.page_size + (size_t)(j % per) * a.block + 16 * part) * row_el + (size_t)h * D;
+                        const bf16_t* const vb = kb + (size_t)a.page_size * row_el;
+#pragma unroll
+                        for (int s = 0; s < KS; ++s) k[x][s] = *reinterpret_cast<const uint4*>(kb + (size_t)c * row_el + 32 * s + 8 * g);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const bf16_t* const src = vb + (size_t)(4 * g + i) * row_el + CPL * c;
+                            if constexpr (CPL == 8) {
+                                const uint4 t = *reinterpret_cast<const uint4*>(src);
+                                v[x][i][0] = t.x; v[x][i][1] = t.y; v[x][i][2] = t.z; v[x][i][3] = t.w;
+                            } else {
+                                const uint2 t = *reinterpret_cast<const uint2*>(src);
+                                v[x][i][0] = t.x; v[x][i][1] = t.y;
+                            }
+                        }
+                    }
+                    float p[8];
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        f32x4 s4 = {0, 0, 0, 0};
+#pragma unroll
+                        for (int s = 0; s < KS; ++s) s4 = mma32<F16>(k[x][s], q[s], s4);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) p[4 * x + i] = s4[i] * a.scale2;
+                        const bool whole = (ONE ? rows[x] != 0 : rows[x] == all_rows) && tok[x] + 16 <= n_least;
+                        if (!whole) {
+                            const bool mine = ONE ? rows[x] != 0 : (rows[x] >> rc & 1) != 0;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) p[4 * x + i] = mine && tok[x] + 4 * g + i < own ? p[4 * x + i] : -inf;
+                        }
+                        // (wave-uniform) V that nobody, or not the careful row, may see
+                        const bool none = rows[x] == 0 || (careful >= 0 && !ONE && !(rows[x] >> careful & 1));
+                        if (none || tok[x] + 16 > v_len) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const bool drop = none || tok[x] + 4 * g + i >= v_len;
+#pragma unroll
+                                for (int w = 0; w < CPL / 2; ++w) v[x][i][w] = drop ? 0u : v[x][i][w];
+                            }
+                        }
+                    }
+                    float top = fmaxf(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])), fmaxf(fmaxf(p[4], p[5]), fmaxf(p[6], p[7])));
+                    top = xor_max<32>(xor_max<16>(top));
+                    if (__ballot(top > m)) {
+                        const float now = fmaxf(m, top), keep = __builtin_amdgcn_exp2f(m - (now == -inf ? 0.0f : now));
+                        m = now;
+                        l *= keep;
+#pragma unroll
+                        for (int t = 0; t < CPL; ++t) o[t] *= keep;
+                    }
+                    const float base = m == -inf ? 0.0f : m;
+                    float part = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) { p[i] = __builtin_amdgcn_exp2f(p[i] - base); part += p[i]; }
+                    l += part;
+                    float hi[8];
+                    u32 ph[4], pl[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        ph[i] = pack2<F16>(p[2 * i], p[2 * i + 1]);
+                        hi[2 * i] = elem_f<F16>((bf16_t)ph[i]); hi[2 * i + 1] = elem_f<F16>((bf16_t)(ph[i] >> 16));
+                        pl[i] = pack2<F16>(p[2 * i] - hi[2 * i], p[2 * i + 1] - hi[2 * i + 1]);
+                    }
+                    const uint4 bh = make_uint4(ph[0], ph[1], ph[2], ph[3]), bl = make_uint4(pl[0], pl[1], pl[2], pl[3]);
+#pragma unroll
+                    for (int t = 0; t < CPL; ++t) {
+                        constexpr u32 LO = 0x05040100u, HI = 0x07060302u;
+                        u32 w[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_perm(v[i >> 1][2 * (i & 1) + 1][t >> 1], v[i >> 1][2 * (i & 1)][t >> 1], t & 1 ? HI : LO);
+                        if (careful < 0) {
+                            const uint4 av = make_uint4(w[0], w[1], w[2], w[3]);
+                            o[t] = mma32<F16>(av, bh, o[t]);
+                            o[t] = mma32<F16>(av, bl, o[t]);
+                        } else {
+                            u32 odd[4], ps[4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const u32 nf = halves_not_finite<F16>(w[i]);
+                                odd[i] = w[i] & nf;
+                                w[i] &= ~nf;
+                                // the weight as one term that is not zero where the weight is not
+                                const u32 tiny = (p[2 * i] > 0.0f && !(ph[i] & 0xffffu) ? 1u : 0u) | (p[2 * i + 1] > 0.0f && !(ph[i] >> 16) ? 0x10000u : 0u);
+                                ps[i] = ph[i] | tiny;
+                            }
+                            const uint4 av = make_uint4(w[0], w[1], w[2], w[3]);
+                            o[t] = mma32<F16>(av, bh, o[t]);
+                            o[t] = mma32<F16>(av, bl, o[t]);
+                            o[t] = mma32<F16>(make_uint4(odd[0], odd[1], odd[2], odd[3]), make_uint4(ps[0], ps[1], ps[2], ps[3]), o[t]);
+                        }
+                    }
+                }
+                if constexpr (!ONE) {
+                    __syncthreads();                                 // (the list has been read)
+                    w0 = s_next == 0x7fffffff ? -1 : s_next;
+                    __syncthreads();
+                }
+            }
+            // the waves' shares of each column meet
+            __syncthreads();
+            l = xor_add<32>(xor_add<16>(l));
+            if (c < a.cols) {
+                float* const dst = s_o + (wave * a.cols + c) * OS + 4 * g * CPL;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int t = 0; t < CPL; t += 4) *reinterpret_cast<float4*>(dst + i * CPL + t) = make_float4(o[t][i], o[t + 1][i], o[t + 2][i], o[t + 3][i]);
+                if (g == 0) { s_ml[(wave * a.cols + c) * 2] = m; s_ml[(wave * a.cols + c) * 2 + 1] = l; }
+            }
+            __syncthreads();
+            bool bad = false;
+            for (int it = tid; it < a.cols * (D / 8); it += 64 * W) {
+                const int cc = it / (D / 8), d = it % (D / 8) * 8, r = ONE ? 0 : cc / gh, hh = ONE ? cc : cc % gh;
+                if (ONE ? cc >= gh : r < ra || r >= rb) continue;
+                if (careful >= 0 && r != careful) continue;
+                float mm = -inf, sum = 0.0f, acc[8] = {};
+                for (int w = 0; w < W; ++w) mm = fmaxf(mm, s_ml[(w * a.cols + cc) * 2]);
+                const float base = mm == -inf ? 0.0f : mm;
+                for (int w = 0; w < W; ++w) {
+                    const float f = __builtin_amdgcn_exp2f(s_ml[(w * a.cols + cc) * 2] - base);
+                    sum = __fmaf_rn(f, s_ml[(w * a.cols + cc) * 2 + 1], sum);
+#pragma unroll
+                    for (int x = 0; x < 8; ++x) acc[x] = __fmaf_rn(f, s_o[(w * a.cols + cc) * OS + d + x], acc[x]);
+                }
+                bad |= !(fabsf(sum) < inf);
+#pragma unroll
+                for (int x = 0; x < 8; ++x) bad |= !(fabsf(acc[x]) < inf);
+                const size_t row = (size_t)(i0 + r) * a.Hq + h * G + h0 + hh;
+                if (ONE && a.splits > 1) {
+                    float* const dst = a.part_o + (row * a.splits + split) * D + d;
+                    *reinterpret_cast<float4*>(dst) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+                    *reinterpret_cast<float4*>(dst + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
+                    if (d == 0) *reinterpret_cast<float2*>(a.part_ml + (row * a.splits + split) * 2) = make_float2(mm, s_seen ? sum : -1.0f);      // (-1: the row lists nothing)
+                    continue;
+                }
+                const bool seen = (s_seen >> r & 1) != 0;            // a row that lists nothing is zero
+                u32 w[4];
+#pragma unroll
+                for (int x = 0; x < 4; ++x) w[x] = seen ? pack2<F16>(acc[2 * x] / sum, acc[2 * x + 1] / sum) : 0u;
+                bf16_t* const dst = a.out + row * D + d;
+                if (a.out_al) *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+                else
+#pragma unroll
+                    for (int x = 0; x < 8; ++x) dst[x] = (bf16_t)(w[x / 2] >> (16 * (x & 1)));
+            }
+            const int again = __syncthreads_or(bad);
+            if (careful < 0 ? !again : careful + 1 >= rb) break;
+            careful = careful < 0 ? ra : careful + 1;
+        }
+        ra = rb;
+    }
+}
+
+// the splits of a row and head: a wave each
+template <int F16, int D>
+__global__ __launch_bounds__(256) void k_block_attn_merge(BlockAttnArgs a) {
+    const int at = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (at >= a.n_rows * a.Hq) return;
+    const int i = at / a.Hq, len = a.q_kvlen[i], req = a.q_req[i];
+    if (len <= 0 || req < 0 || req >= a.n_req) return;
+    const float inf = __uint_as_float(0x7f800000u);
+    const float* const ml = a.part_ml + (size_t)at * a.splits * 2;
+    float m = lane < a.splits ? ml[2 * lane] : -inf, s = lane < a.splits ? ml[2 * lane + 1] : 0.0f;
+    const bool none = __shfl(s, 0, 64) == -1.0f;
+    float top = m;
+    for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+    const float f = __builtin_amdgcn_exp2f(m - (top == -inf ? 0.0f : top));
+    const float sum = butterfly<64>(lane < a.splits ? f * s : 0.0f);
+    float acc[D / 64] = {};
+    for (int z = 0; z < a.splits; ++z) {
+        const float fz = __shfl(f, z, 64);
+#pragma unroll
+        for (int x = 0; x < D / 64; ++x) acc[x] = __fmaf_rn(fz, a.part_o[((size_t)at * a.splits + z) * D + lane + 64 * x], acc[x]);
+    }
+#pragma unroll
+    for (int x = 0; x < D / 64; ++x) a.out[(size_t)at * D + lane + 64 * x] = none ? 0 : f_elem<F16>(acc[x] / sum);
 }
 
 // ================================================================================================
@@ -422,9 +764,26 @@ static int check_attention(const vox_block_attention_args* a) {
     if (a->q_stride < 0) return vox_fail(VOX_ERR_INVALID, "block_attention: a stride is negative");
     return VOX_OK;
 }
+// How a call's rows are laid out: rows a tile, and the parts that a row's list is split into.
+struct AttnShape { int per_tile, splits, head_tiles; };
+static AttnShape attn_shape(const vox_block_attention_args* a, int cus) {
+    const vox_block_rows& r = a->rows;
+    const int G = r.heads / a->cache.kv_heads;
+    AttnShape s{1, 1, (G + 15) / 16};
+    if (r.n_own > 0 && r.n_rows >= 2 * r.n_own && G <= 8) { s.per_tile = 16 / G; return s; }
+    const long tokens = (long)a->top * a->cache.block, blocks = (long)r.n_rows * a->cache.kv_heads * s.head_tiles;
+    if (tokens > 1024) {
+        long z = (2L * cus + blocks - 1) / blocks;
+        const long most = (tokens + 255) / 256;
+        if (z > most) z = most;
+        s.splits = (int)(z < 1 ? 1 : z > 64 ? 64 : z);
+    }
+    return s;
+}
 int64_t vox_block_attention_workspace_bytes(const vox_block_attention_args* a) {
     if (check_attention(a) != VOX_OK) return -1;
-    return 0;
+    const AttnShape s = attn_shape(a, ATTN_CUS);
+    return s.splits > 1 ? (int64_t)a->rows.n_rows * a->rows.heads * s.splits * (a->cache.head_dim + 2) * 4 : 0;
 }
 int vox_block_attention(vox_ctx* ctx, void* stream, const vox_block_attention_args* a) {
     (void)ctx;
@@ -433,9 +792,27 @@ int vox_block_attention(vox_ctx* ctx, void* stream, const vox_block_attention_ar
     const vox_block_rows& r = a->rows;
     if (r.n_rows == 0) return VOX_OK;
     if (!a->q || (!a->blocks && a->top) || !a->out || ((size_t)a->q | (size_t)a->out) & 1) return vox_fail(VOX_ERR_INVALID, "block_attention: an operand is NULL, or does not lie on its type");
-    BlockAttnArgs s{(const bf16_t*)a->q, (const bf16_t*)c.kv, r.q_req, r.q_kvlen, r.kv_indptr, r.kv_indices, a->blocks, (bf16_t*)a->out, (long)a->q_stride, a->scale,
-                    r.n_rows, r.n_req, r.heads, c.kv_heads, r.max_kvlen, c.n_pages, c.page_size, c.block, a->top};
-    return launch(BY_TYPE_AND_DIM(k_block_attention, c), dim3(r.n_rows, r.heads), 64, 0, (hipStream_t)stream, s);
+    const AttnShape z = attn_shape(a, ATTN_CUS);
+    const size_t rows = (size_t)r.n_rows * r.heads * z.splits;
+    if (z.splits > 1 && (!a->workspace || (size_t)a->workspace & 15 || a->workspace_bytes < (int64_t)(rows * (c.head_dim + 2) * 4)))
+        return vox_fail(VOX_ERR_INVALID, "block_attention: a workspace of %lld bytes on 16, %lld are wanted", (long long)(a->workspace ? a->workspace_bytes : 0), (long long)(rows * (c.head_dim + 2) * 4));
+    const int64_t grid = (int64_t)((r.n_rows + z.per_tile - 1) / z.per_tile) * z.splits * z.head_tiles * c.kv_heads;
+    if (grid > 0x7fffffff) return vox_fail(VOX_ERR_INVALID, "block_attention: %d rows of %d heads are more than a launch holds", r.n_rows, r.heads);
+    const bool one = z.per_tile == 1;
+    const int W = one ? 8 : 4, G = r.heads / c.kv_heads, cols = one && G < 16 ? G : 16;
+    BlockAttnArgs s{(const bf16_t*)a->q, (const bf16_t*)c.kv, r.q_req, r.q_kvlen, r.kv_indptr, r.kv_indices, a->blocks, (bf16_t*)a->out, (float*)a->workspace,
+                    (float*)a->workspace + rows * c.head_dim, (long)a->q_stride, a->scale * 1.44269504088896340736f, r.n_rows, r.n_req, r.heads, c.kv_heads, r.max_kvlen, c.n_pages,
+                    c.page_size, c.block, a->top, z.per_tile, z.splits, z.head_tiles, cols, ((size_t)a->q & 15) == 0 && a->q_stride % 8 == 0, ((size_t)a->out & 15) == 0};
+    const size_t merge = (size_t)W * cols * (c.head_dim + 4 + 2) * 4;
+    const size_t entries = (size_t)a->top * z.per_tile, lists = one ? entries * 8 : ATTN_WINDOW * 2 + (entries < ATTN_WINDOW ? entries : ATTN_WINDOW) * 8;
+    const size_t lds = merge > lists ? merge : lists;
+    const void* kern = one ? (c.dtype == VOX_DTYPE_F16 ? (c.head_dim == 128 ? (const void*)k_block_attn<1, 128, 8, true> : (const void*)k_block_attn<1, 64, 8, true>)
+                                                       : (c.head_dim == 128 ? (const void*)k_block_attn<0, 128, 8, true> : (const void*)k_block_attn<0, 64, 8, true>))
+                           : (c.dtype == VOX_DTYPE_F16 ? (c.head_dim == 128 ? (const void*)k_block_attn<1, 128, 4, false> : (const void*)k_block_attn<1, 64, 4, false>)
+                                                       : (c.head_dim == 128 ? (const void*)k_block_attn<0, 128, 4, false> : (const void*)k_block_attn<0, 64, 4, false>));
+    VOX_TRY(launch(kern, dim3((unsigned)grid), 64 * W, lds, (hipStream_t)stream, s));
+    if (z.splits == 1) return VOX_OK;
+    return launch(BY_TYPE_AND_DIM(k_block_attn_merge, c), dim3((unsigned)(((int64_t)r.n_rows * r.heads + 3) / 4)), 256, 0, (hipStream_t)stream, s);
 }
 
 }  // extern "C"

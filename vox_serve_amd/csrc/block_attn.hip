@@ -69,33 +69,182 @@ struct RopeAppendArgs {
     bf16_t *q_out, *kv;
     const int *pos, *page, *slot;
     const float* cs;
+    int8_t* bounds;                      // blocks of threads from `append_blocks` on: the bounds of the blocks that the rows complete
+    float* steps;
     long q_stride, k_stride, v_stride;
-    int n_rows, Hq, Hkv, D, rot, interleave, max_pos, page_size, n_pages;
+    int n_rows, Hq, Hkv, D, rot, interleave, max_pos, page_size, n_pages, block, slots, append_blocks;
 };
-// one thread a pair of channels that turn together (or two that do not)
+__device__ __forceinline__ bool row_place(const int* page, const int* slot, int n, int n_pages, int page_size, int& pg, int& sl) {
+    pg = page[n]; sl = slot[n];
+    return pg >= 0 && pg < n_pages && sl >= 0 && sl < page_size;
+}
+__device__ __forceinline__ int table_row(const RopeAppendArgs& a, int n) {
+    const int p = a.rot ? a.pos[n] : 0;
+    return p < 0 ? 0 : (p >= a.max_pos ? a.max_pos - 1 : p);
+}
 template <int F16>
-__global__ __launch_bounds__(256) void k_rope_append(RopeAppendArgs a) {
-    const int n = blockIdx.y, half_d = a.D >> 1, half = a.rot >> 1, heads = a.Hq + 2 * a.Hkv;
-    const int pg = a.page[n], slot = a.slot[n];
-    if (pg < 0 || pg >= a.n_pages || slot < 0 || slot >= a.page_size) return;
-    int p = a.rot ? a.pos[n] : 0;
-    p = p < 0 ? 0 : (p >= a.max_pos ? a.max_pos - 1 : p);
-    for (int i = blockIdx.x * 256 + threadIdx.x; i < heads * half_d; i += gridDim.x * 256) {
-        const int head = i / half_d, c = i % half_d;
-        const int kind = head < a.Hq ? 0 : head < a.Hq + a.Hkv ? 1 : 2, h = kind == 0 ? head : kind == 1 ? head - a.Hq : head - a.Hq - a.Hkv;
-        const bf16_t* const src = (kind == 0 ? a.q + n * a.q_stride : kind == 1 ? a.k + n * a.k_stride : a.v + n * a.v_stride) + (size_t)h * a.D;
-        bf16_t* const dst = kind == 0 ? a.q_out + ((size_t)n * a.Hq + h) * a.D
-                                      : a.kv + (((size_t)pg * 2 + (kind == 2)) * a.page_size + slot) * a.Hkv * a.D + (size_t)h * a.D;
-        const bool turns = kind < 2 && c < half;
-        const int i0 = turns && !a.interleave ? c : turns || kind == 2 ? 2 * c : a.rot + 2 * (c - half), i1 = turns && !a.interleave ? c + half : i0 + 1;
-        bf16_t x = src[i0], y = src[i1];
-        if (turns) {
-            const float fx = elem_f<F16>(x), fy = elem_f<F16>(y), cc = a.cs[((size_t)p * half + c) * 2], ss = a.cs[((size_t)p * half + c) * 2 + 1];
-            x = f_elem<F16>(__fmaf_rn(-fy, ss, fx * cc));
-            y = f_elem<F16>(__fmaf_rn(fx, ss, fy * cc));
+__device__ __forceinline__ void turn(float x, float y, float c, float s, bf16_t& u, bf16_t& v) {
+    u = f_elem<F16>(__fmaf_rn(-y, s, x * c));
+    v = f_elem<F16>(__fmaf_rn(x, s, y * c));
+}
+
+// Any dims, strides and alignment: one thread a pair of channels that turn together (or two that do not).
+template <int F16>
+__global__ __launch_bounds__(256) void k_rope_append_any(RopeAppendArgs a) {
+    const int half_d = a.D >> 1, half = a.rot >> 1, pairs = (a.Hq + 2 * a.Hkv) * half_d;
+    const long item = (long)blockIdx.x * 256 + threadIdx.x;
+    const int n = (int)(item / pairs), i = (int)(item % pairs);
+    int pg, slot;
+    if (n >= a.n_rows || !row_place(a.page, a.slot, n, a.n_pages, a.page_size, pg, slot)) return;
+    const int p = table_row(a, n), head = i / half_d, c = i % half_d;
+    const int kind = head < a.Hq ? 0 : head < a.Hq + a.Hkv ? 1 : 2, h = kind == 0 ? head : kind == 1 ? head - a.Hq : head - a.Hq - a.Hkv;
+    const bf16_t* const src = (kind == 0 ? a.q + n * a.q_stride : kind == 1 ? a.k + n * a.k_stride : a.v + n * a.v_stride) + (size_t)h * a.D;
+    bf16_t* const dst = kind == 0 ? a.q_out + ((size_t)n * a.Hq + h) * a.D
+                                  : a.kv + (((size_t)pg * 2 + (kind == 2)) * a.page_size + slot) * a.Hkv * a.D + (size_t)h * a.D;
+    const bool turns = kind < 2 && c < half;
+    const int i0 = turns && !a.interleave ? c : turns || kind == 2 ? 2 * c : a.rot + 2 * (c - half), i1 = turns && !a.interleave ? c + half : i0 + 1;
+    bf16_t x = src[i0], y = src[i1];
+    if (turns) turn<F16>(elem_f<F16>(x), elem_f<F16>(y), a.cs[((size_t)p * half + c) * 2], a.cs[((size_t)p * half + c) * 2 + 1], x, y);
+    dst[i0] = x;
+    dst[i1] = y;
+}
+
+// The bounds of one block, by one wave: D / 8 lanes hold a key, 512 / D keys at once.  key(l, t): channels 8 l .. 8 l + 7 of token t.
+template <int F16, int D, class K>
+__device__ __forceinline__ void block_bounds(int lane, int block, int8_t* bounds, float* step_out, K key) {
+    constexpr int LPT = D / 8, TPI = 64 / LPT;
+    const float inf = __uint_as_float(0x7f800000u);
+    const int l = lane % LPT;
+    float hi[8], lo[8], amax = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) { hi[i] = -inf; lo[i] = inf; }
+#pragma unroll 4
+    for (int t = lane / LPT; t < block; t += TPI) {
+        const uint4 v = key(l, t);
+        const u32 w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float x = elem_f<F16>((bf16_t)(w[i / 2] >> (16 * (i % 2))));
+            hi[i] = x > hi[i] ? x : hi[i];                          // (false for NaN)
+            lo[i] = x < lo[i] ? x : lo[i];
+            amax = fmaxf(amax, finite_abs(x));                      // (of all keys: infinities would stand in front of it in the bounds)
         }
-        dst[i0] = x;
-        dst[i1] = y;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int o = LPT; o < 64; o <<= 1) {
+            hi[i] = fmaxf(hi[i], __shfl_xor(hi[i], o, 64));
+            lo[i] = fminf(lo[i], __shfl_xor(lo[i], o, 64));
+        }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) amax = fmaxf(amax, __shfl_xor(amax, o, 64));
+    const float step = step_of(amax), inv = 1.0f / step;
+    if (lane < LPT) {
+        u32 wh[2] = {0, 0}, wl[2] = {0, 0};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const bool any = hi[i] >= lo[i];                        // (a channel of NaN: no)
+            const int H = any ? (int)fminf(fmaxf(ceilf(hi[i] * inv), -127.0f), 127.0f) : 0, L = any ? (int)fminf(fmaxf(floorf(lo[i] * inv), -127.0f), 127.0f) : 0;
+            wh[i / 4] |= (u32)(H & 255) << (8 * (i % 4));
+            wl[i / 4] |= (u32)(L & 255) << (8 * (i % 4));
+        }
+        *reinterpret_cast<uint2*>(bounds + 8 * l) = make_uint2(wh[0], wh[1]);
+        *reinterpret_cast<uint2*>(bounds + D + 8 * l) = make_uint2(wl[0], wl[1]);
+        if (lane == 0) *step_out = step;
+    }
+}
+
+// Vectors: a thread has 16 channels of a head that turn (two runs of eight whose pairs they are: halves, or 16 in a row: neighbours) or do not, and goes through the
+// row's heads slot, slot + slots, ..: the angles are loaded once.  Calls of few rows take a slot a head (everything in flight at once), calls of many rows eight
+// slots a row (the angles, 64 bytes a thread, would be as much to load as the channels).
+// With rows of different requests the launch has more blocks of threads behind these: a wave a row and kv head, which leaves at once unless the row
+// completes a block; the other keys of the block are in the cache from earlier calls, the row's own is turned here once more.
+template <int F16, int IL, int D>        // D: 64 or 128 with bounds, else 0 (any)
+__global__ __launch_bounds__(256) void k_rope_append(RopeAppendArgs a) {
+    if constexpr (D > 0) if ((int)blockIdx.x >= a.append_blocks) {
+        const int at = ((int)blockIdx.x - a.append_blocks) * 4 + (threadIdx.x >> 6), n = at / a.Hkv, h = at % a.Hkv, half = a.rot >> 1;
+        int pg, slot;
+        if (n >= a.n_rows || !row_place(a.page, a.slot, n, a.n_pages, a.page_size, pg, slot) || (slot + 1) % a.block) return;
+        const int p = table_row(a, n), per = a.page_size / a.block;
+        const bf16_t* const base = a.kv + ((size_t)pg * 2 * a.page_size + slot + 1 - a.block) * a.Hkv * D + (size_t)h * D;
+        const bf16_t* const own = a.k + n * a.k_stride + (size_t)h * D;
+        const size_t to = ((size_t)pg * a.Hkv + h) * per + slot / a.block;
+        block_bounds<F16, D>(threadIdx.x & 63, a.block, a.bounds + to * 2 * D, a.steps + to, [&](int l, int t) {
+            if (t + 1 < a.block) return *reinterpret_cast<const uint4*>(base + (size_t)t * a.Hkv * D + 8 * l);
+            bf16_t e[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int ch = 8 * l + i;
+                e[i] = own[ch];
+                if (ch < a.rot) {
+                    const int pair = IL ? ch >> 1 : ch % half;
+                    const bool second = IL ? ch & 1 : ch >= half;
+                    const float other = elem_f<F16>(own[IL ? ch ^ 1 : second ? ch - half : ch + half]), me = elem_f<F16>(e[i]);
+                    bf16_t u, v;
+                    turn<F16>(second ? other : me, second ? me : other, a.cs[((size_t)p * half + pair) * 2], a.cs[((size_t)p * half + pair) * 2 + 1], u, v);
+                    e[i] = second ? v : u;
+                }
+            }
+            return make_uint4((u32)e[0] | ((u32)e[1] << 16), (u32)e[2] | ((u32)e[3] << 16), (u32)e[4] | ((u32)e[5] << 16), (u32)e[6] | ((u32)e[7] << 16));
+        });
+        return;
+    }
+    const int units = a.D >> 4, per_row = units * a.slots, heads = a.Hq + 2 * a.Hkv;
+    const long item = (long)blockIdx.x * 256 + threadIdx.x;
+    const int n = (int)(item / per_row), j = (int)(item - (long)n * per_row), u = j % units, slot0 = j / units;
+    int pg, slot;
+    if (n >= a.n_rows || !row_place(a.page, a.slot, n, a.n_pages, a.page_size, pg, slot)) return;
+    const int half = a.rot >> 1;
+    const bool turns = 16 * u < a.rot;
+    const int c0 = turns && !IL ? 8 * u : 16 * u, c1 = turns && !IL ? half + 8 * u : c0 + 8;
+    float cs[16];
+    if (turns) {
+        const float4* const t = reinterpret_cast<const float4*>(a.cs + ((size_t)table_row(a, n) * half + 8 * u) * 2);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float4 x = t[i];
+            cs[4 * i] = x.x; cs[4 * i + 1] = x.y; cs[4 * i + 2] = x.z; cs[4 * i + 3] = x.w;
+        }
+    }
+    bf16_t* const kd = a.kv + ((size_t)pg * 2 * a.page_size + slot) * a.Hkv * a.D;
+    auto from = [&](int head) { return head < a.Hq ? a.q + n * a.q_stride + (size_t)head * a.D
+                                     : head < a.Hq + a.Hkv ? a.k + n * a.k_stride + (size_t)(head - a.Hq) * a.D : a.v + n * a.v_stride + (size_t)(head - a.Hq - a.Hkv) * a.D; };
+    constexpr int B = 3;                                             // heads in flight
+    for (int h0 = slot0; h0 < heads; h0 += B * a.slots) {
+        uint4 x[B], y[B];
+#pragma unroll
+        for (int b = 0; b < B; ++b)
+            if (h0 + b * a.slots < heads) {
+                const bf16_t* const src = from(h0 + b * a.slots);
+                x[b] = *reinterpret_cast<const uint4*>(src + c0);
+                y[b] = *reinterpret_cast<const uint4*>(src + c1);
+            }
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+            const int head = h0 + b * a.slots;
+            if (head >= heads) break;
+            bf16_t* const dst = head < a.Hq ? a.q_out + ((size_t)n * a.Hq + head) * a.D
+                              : head < a.Hq + a.Hkv ? kd + (size_t)(head - a.Hq) * a.D : kd + ((size_t)a.page_size * a.Hkv + head - a.Hq - a.Hkv) * a.D;
+            if (turns && head < a.Hq + a.Hkv) {
+                u32 w[8] = {x[b].x, x[b].y, x[b].z, x[b].w, y[b].x, y[b].y, y[b].z, y[b].w};
+                bf16_t e[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) e[i] = (bf16_t)(w[i / 2] >> (16 * (i % 2)));
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    bf16_t& s = e[IL ? 2 * i : i];
+                    bf16_t& t = e[IL ? 2 * i + 1 : 8 + i];
+                    turn<F16>(elem_f<F16>(s), elem_f<F16>(t), cs[2 * i], cs[2 * i + 1], s, t);
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) w[i] = (u32)e[2 * i] | ((u32)e[2 * i + 1] << 16);
+                x[b] = make_uint4(w[0], w[1], w[2], w[3]);
+                y[b] = make_uint4(w[4], w[5], w[6], w[7]);
+            }
+            *reinterpret_cast<uint4*>(dst + c0) = x[b];
+            *reinterpret_cast<uint4*>(dst + c1) = y[b];
+        }
     }
 }
 
@@ -106,60 +255,19 @@ struct BoundsArgs {
     const int *page, *slot;
     int n_rows, n_pages, page_size, block, Hkv;
 };
-// one wave a row that completes its block, and kv head: D / 8 lanes hold a key, 512 / D keys at once
+// 64 rows and a kv head a block of threads; its waves share the rows that complete a block
 template <int F16, int D>
 __global__ __launch_bounds__(256) void k_block_bounds(BoundsArgs a) {
-    constexpr int LPT = D / 8, TPI = 64 / LPT;
-    const int n = blockIdx.x * 4 + (threadIdx.x >> 6), h = blockIdx.y, lane = threadIdx.x & 63, l = lane % LPT;
-    if (n >= a.n_rows) return;
-    const int pg = a.page[n], slot = a.slot[n];
-    if (pg < 0 || pg >= a.n_pages || slot < 0 || slot >= a.page_size || (slot + 1) % a.block) return;
-    const bf16_t* const k = a.kv + ((size_t)pg * 2 * a.page_size + slot + 1 - a.block) * a.Hkv * D + (size_t)h * D;
-    const float inf = __uint_as_float(0x7f800000u);
-    float hi[8], lo[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) { hi[i] = -inf; lo[i] = inf; }
-    for (int t = lane / LPT; t < a.block; t += TPI) {
-        const uint4 v = reinterpret_cast<const uint4*>(k + (size_t)t * a.Hkv * D)[l];
-        const u32 w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float x = elem_f<F16>((bf16_t)(w[i / 2] >> (16 * (i % 2))));
-            hi[i] = x > hi[i] ? x : hi[i];                          // (false for NaN)
-            lo[i] = x < lo[i] ? x : lo[i];
-        }
-    }
-    float amax = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        for (int o = LPT; o < 64; o <<= 1) {
-            hi[i] = fmaxf(hi[i], __shfl_xor(hi[i], o, 64));
-            lo[i] = fminf(lo[i], __shfl_xor(lo[i], o, 64));
-        }
-    }
-    // the largest finite magnitude: of all keys, not of the bounds, where infinities stand in front of it
-    for (int t = lane / LPT; t < a.block; t += TPI) {
-        const uint4 v = reinterpret_cast<const uint4*>(k + (size_t)t * a.Hkv * D)[l];
-        const u32 w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int i = 0; i < 8; ++i) amax = fmaxf(amax, finite_abs(elem_f<F16>((bf16_t)(w[i / 2] >> (16 * (i % 2))))));
-    }
-    for (int o = 1; o < 64; o <<= 1) amax = fmaxf(amax, __shfl_xor(amax, o, 64));
-    const float step = step_of(amax), inv = 1.0f / step;
-    if (lane < LPT) {
-        const int per = a.page_size / a.block;
-        const size_t at = ((size_t)pg * a.Hkv + h) * per + slot / a.block;
-        u32 wh[2] = {0, 0}, wl[2] = {0, 0};
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const bool any = hi[i] >= lo[i];                        // (a channel of NaN: no)
-            const int H = any ? (int)fminf(fmaxf(ceilf(hi[i] * inv), -127.0f), 127.0f) : 0, L = any ? (int)fminf(fmaxf(floorf(lo[i] * inv), -127.0f), 127.0f) : 0;
-            wh[i / 4] |= (u32)(H & 255) << (8 * (i % 4));
-            wl[i / 4] |= (u32)(L & 255) << (8 * (i % 4));
-        }
-        *reinterpret_cast<uint2*>(a.bounds + at * 2 * D + 8 * l) = make_uint2(wh[0], wh[1]);
-        *reinterpret_cast<uint2*>(a.bounds + at * 2 * D + D + 8 * l) = make_uint2(wl[0], wl[1]);
-        if (lane == 0) a.steps[at] = step;
+    const int n0 = blockIdx.x * 64, h = blockIdx.y, lane = threadIdx.x & 63;
+    int pg = -1, slot = 0;
+    const bool done = n0 + lane < a.n_rows && row_place(a.page, a.slot, n0 + lane, a.n_pages, a.page_size, pg, slot) && (slot + 1) % a.block == 0;
+    unsigned long long left = __ballot(done);
+    for (int i = 0; left; ++i, left &= left - 1) {
+        if ((i & 3) != (int)(threadIdx.x >> 6)) continue;
+        const int from = __builtin_ctzll(left), p = __shfl(pg, from, 64), s = __shfl(slot, from, 64);
+        const bf16_t* const k = a.kv + ((size_t)p * 2 * a.page_size + s + 1 - a.block) * a.Hkv * D + (size_t)h * D;
+        const size_t to = ((size_t)p * a.Hkv + h) * (a.page_size / a.block) + s / a.block;
+        block_bounds<F16, D>(lane, a.block, a.bounds + to * 2 * D, a.steps + to, [&](int l, int t) { return *reinterpret_cast<const uint4*>(k + (size_t)t * a.Hkv * D + 8 * l); });
     }
 }
 
@@ -676,6 +784,7 @@ __global__ __launch_bounds__(256) void k_block_attn_merge(BlockAttnArgs a) {
 // ================================================================================================
 // entry points
 // ================================================================================================
+#define APPEND_MANY (1 << 18)             // 16-channel pieces of a call from which on threads go through several heads
 #define BY_TYPE_AND_DIM(KERN, c) \
     ((c).dtype == VOX_DTYPE_F16 ? ((c).head_dim == 128 ? (const void*)KERN<1, 128> : (const void*)KERN<1, 64>) \
                                 : ((c).head_dim == 128 ? (const void*)KERN<0, 128> : (const void*)KERN<0, 64>))
@@ -683,7 +792,7 @@ __global__ __launch_bounds__(256) void k_block_attn_merge(BlockAttnArgs a) {
 static int launch_bounds(hipStream_t st, const vox_block_cache& c, const int* page, const int* slot, int n_rows) {
     if (n_rows == 0) return VOX_OK;
     BoundsArgs b{(const bf16_t*)c.kv, c.bounds, c.steps, page, slot, n_rows, c.n_pages, c.page_size, c.block, c.kv_heads};
-    return launch(BY_TYPE_AND_DIM(k_block_bounds, c), dim3((n_rows + 3) / 4, c.kv_heads), 256, 0, st, b);
+    return launch(BY_TYPE_AND_DIM(k_block_bounds, c), dim3((n_rows + 63) / 64, c.kv_heads), 256, 0, st, b);
 }
 
 extern "C" {
@@ -712,17 +821,32 @@ int vox_rope_append(vox_ctx* ctx, void* stream, const vox_rope_append_args* a) {
     if (a->rot && (!a->pos || !a->table || a->table_max_pos <= 0)) return vox_fail(VOX_ERR_INVALID, "rope_append: no positions or no table");
     if (((size_t)a->q | (size_t)a->k | (size_t)a->v | (size_t)a->q_out) & 1 || (a->rot && (size_t)a->table & 3)) return vox_fail(VOX_ERR_INVALID, "rope_append: an operand does not lie on its type");
     if (a->q_stride < 0 || a->k_stride < 0 || a->v_stride < 0) return vox_fail(VOX_ERR_INVALID, "rope_append: a stride is negative");
-    RopeAppendArgs r{(const bf16_t*)a->q, (const bf16_t*)a->k, (const bf16_t*)a->v, (bf16_t*)a->q_out, (bf16_t*)c.kv, a->pos, a->page, a->slot, a->table,
-                     (long)a->q_stride, (long)a->k_stride, (long)a->v_stride, a->n_rows, a->heads, c.kv_heads, D, a->rot, a->interleave, a->table_max_pos, c.page_size, c.n_pages};
-    const int pairs = (a->heads + 2 * c.kv_heads) * (D / 2);
-    for (int at = 0; at < a->n_rows; at += 65535) {                 // (grid.y)
-        RopeAppendArgs p = r;
-        p.n_rows = a->n_rows - at < 65535 ? a->n_rows - at : 65535;
-        p.q += (size_t)at * r.q_stride; p.k += (size_t)at * r.k_stride; p.v += (size_t)at * r.v_stride; p.q_out += (size_t)at * r.Hq * D;
-        p.pos = p.pos ? p.pos + at : nullptr; p.page += at; p.slot += at;
-        VOX_TRY(launch(c.dtype == VOX_DTYPE_F16 ? (const void*)k_rope_append<1> : (const void*)k_rope_append<0>, dim3((pairs + 255) / 256, p.n_rows), 256, 0, (hipStream_t)stream, p));
-    }
-    return c.bounds ? launch_bounds((hipStream_t)stream, c, a->page, a->slot, a->n_rows) : VOX_OK;
+    const int heads = a->heads + 2 * c.kv_heads;
+    RopeAppendArgs r{(const bf16_t*)a->q, (const bf16_t*)a->k, (const bf16_t*)a->v, (bf16_t*)a->q_out, (bf16_t*)c.kv, a->pos, a->page, a->slot, a->table, c.bounds, c.steps,
+                     (long)a->q_stride, (long)a->k_stride, (long)a->v_stride, a->n_rows, a->heads, c.kv_heads, D, a->rot, a->interleave, a->table_max_pos, c.page_size, c.n_pages, c.block, heads, 0};
+    const bool f16 = c.dtype == VOX_DTYPE_F16;
+    // 16 channels a thread: everything on 16 bytes, and no pair of eight across the border of what turns
+    const bool vec = D % 16 == 0 && a->rot % 16 == 0 && (((size_t)a->q | (size_t)a->k | (size_t)a->v | (size_t)a->q_out | (a->rot ? (size_t)a->table : 0)) & 15) == 0 &&
+                     a->q_stride % 8 == 0 && a->k_stride % 8 == 0 && a->v_stride % 8 == 0;
+    const bool with = vec && c.bounds && a->n_own == a->n_rows;      // the bounds in the same launch
+    int64_t blocks;
+    if (vec) {
+        if ((int64_t)a->n_rows * heads * (D / 16) >= APPEND_MANY && heads > 8) r.slots = 8;
+        blocks = ((int64_t)a->n_rows * r.slots * (D / 16) + 255) / 256;
+    } else blocks = ((int64_t)a->n_rows * heads * (D / 2) + 255) / 256;
+    const int64_t more = with ? ((int64_t)a->n_rows * c.kv_heads + 3) / 4 : 0;
+    if (blocks + more > 0x7fffffff) return vox_fail(VOX_ERR_INVALID, "rope_append: %d rows of %d heads are more than a launch holds", a->n_rows, a->heads);
+    r.append_blocks = (int)blocks;
+    const void* kern;
+    if (!vec) kern = f16 ? (const void*)k_rope_append_any<1> : (const void*)k_rope_append_any<0>;
+#define APPEND_OF(IL) \
+    (!with ? (f16 ? (const void*)k_rope_append<1, IL, 0> : (const void*)k_rope_append<0, IL, 0>) \
+     : D == 128 ? (f16 ? (const void*)k_rope_append<1, IL, 128> : (const void*)k_rope_append<0, IL, 128>) \
+                : (f16 ? (const void*)k_rope_append<1, IL, 64> : (const void*)k_rope_append<0, IL, 64>))
+    else kern = a->interleave ? APPEND_OF(1) : APPEND_OF(0);
+#undef APPEND_OF
+    VOX_TRY(launch(kern, dim3((unsigned)(blocks + more)), 256, 0, (hipStream_t)stream, r));
+    return c.bounds && !with ? launch_bounds((hipStream_t)stream, c, a->page, a->slot, a->n_rows) : VOX_OK;
 }
 
 static int check_select(const vox_block_select_args* a) {

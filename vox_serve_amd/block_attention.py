@@ -30,9 +30,8 @@ _ATTEND = struct.Struct(_CACHE + _ROWS + "PPPP2qif0q")
 
 
 def _on(device):
-    """Context and stream of the device that is current; tensors elsewhere are refused by the callers."""
-    h = N._ctxs.get(device.index)
-    return (h or N.ctx()), torch.cuda.current_stream().cuda_stream
+    """Context and stream of the device that is current.  (The raw stream costs 0.1 us, a torch.cuda.Stream object of it 2.7: as much as the launch.)"""
+    return N._ctxs.get(device.index) or N.ctx(), torch._C._cuda_getCurrentRawStream(device.index)
 
 
 _kept = []                               # workspaces that captured graphs go back to
@@ -76,12 +75,13 @@ def _ints(t, shape, device, name):
 
 def _heads(t, rows, dim, like, name):
     """[rows, heads, dim] whose heads lie together; rows may lie apart."""
-    if t.dim() != 3 or t.shape[0] != rows or t.shape[2] != dim:
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, [{rows}, heads, {dim}] is wanted")
+    shape = t.shape
+    if len(shape) != 3 or shape[0] != rows or shape[2] != dim:
+        raise ValueError(f"{name} has shape {tuple(shape)}, [{rows}, heads, {dim}] is wanted")
     if t.dtype is not like.dtype or t.device != like.device:
-        raise ValueError(f"{name} is {t.dtype} on {t.device}, the cache {like.dtype} on {like.device}")
-    s = t.stride()
-    return t if s[2] == 1 and (s[1] == dim or t.shape[1] == 1) and s[0] >= 0 else t.contiguous()
+        raise ValueError(f"{name} is {t.dtype} on {t.device}, {like.dtype} on {like.device} is wanted")
+    _, apart, unit = t.stride()
+    return t if unit == 1 and (apart == dim or shape[1] == 1) else t.contiguous()
 
 
 def _cache(kv):
@@ -93,27 +93,29 @@ def _cache(kv):
 
 
 def _bounds(bounds, steps, device):
-    if bounds.dim() != 5 or bounds.shape[3] != 2 or bounds.dtype is not torch.int8 or not bounds.is_contiguous():
-        raise ValueError(f"bounds is {bounds.dtype} {tuple(bounds.shape)}: a contiguous int8 [pages, kv heads, blocks, 2, dim] is wanted")
-    if steps.shape != bounds.shape[:3] or steps.dtype is not torch.float32 or not steps.is_contiguous():
-        raise ValueError(f"steps is {steps.dtype} {tuple(steps.shape)}: a contiguous float32 {tuple(bounds.shape[:3])} is wanted")
+    """The shape (pages, kv heads, blocks, 2, dim)."""
+    shape = bounds.shape
+    if len(shape) != 5 or shape[3] != 2 or bounds.dtype is not torch.int8 or not bounds.is_contiguous():
+        raise ValueError(f"bounds is {bounds.dtype} {tuple(shape)}: a contiguous int8 [pages, kv heads, blocks, 2, dim] is wanted")
+    if steps.shape != shape[:3] or steps.dtype is not torch.float32 or not steps.is_contiguous():
+        raise ValueError(f"steps is {steps.dtype} {tuple(steps.shape)}: a contiguous float32 {tuple(shape[:3])} is wanted")
     if bounds.device != device or steps.device != device:
         raise ValueError(f"bounds and steps are on {bounds.device} and {steps.device}, {device} is wanted")
+    return shape
 
 
 def _bounds_of(kv, bounds, steps):
     """(bounds, steps, block) of a cache layer, as pointers."""
-    _bounds(bounds, steps, kv.device)
+    pages, heads, per, _, dim = _bounds(bounds, steps, kv.device)
     p, _, page, h, d = kv.shape
-    per = bounds.shape[2]
-    if bounds.shape[0] != p or bounds.shape[1] != h or bounds.shape[4] != d or per == 0 or page % per:
+    if pages != p or heads != h or dim != d or per == 0 or page % per:
         raise ValueError(f"bounds {tuple(bounds.shape)} are not those of a cache {tuple(kv.shape)}")
     return bounds.data_ptr(), steps.data_ptr(), page // per
 
 
 def _out(out, shape, like, device, name="out"):
     if out is None:
-        return torch.empty(shape, dtype=like, device=device)
+        return torch.empty(shape, dtype=like, device=device)      # (rows that are passed over hold what the allocator left)
     if out.shape != shape or out.dtype is not like or out.device != device or not out.is_contiguous():
         raise ValueError(f"{name} is {out.dtype} {tuple(out.shape)} on {out.device}: a contiguous {like} {tuple(shape)} on {device} is wanted")
     return out
@@ -195,8 +197,7 @@ def select_blocks(q, bounds, steps, q_req, q_kvlen, kv_indptr, kv_indices, *, bl
     if device.index != torch.cuda.current_device():
         with torch.cuda.device(device):
             return select_blocks(q, bounds, steps, q_req, q_kvlen, kv_indptr, kv_indices, block=block, top=top, max_kvlen=max_kvlen, first=first, last=last, n_req=n_req, out=out)
-    _bounds(bounds, steps, device)
-    n_pages, h, per, _, d = bounds.shape
+    n_pages, h, per, _, d = _bounds(bounds, steps, device)
     rows = q.shape[0]
     if q.dtype not in _DTYPES:
         raise TypeError(f"q is {q.dtype}: bfloat16 or float16 is wanted")

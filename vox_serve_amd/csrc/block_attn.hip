@@ -281,7 +281,7 @@ struct SelectArgs {
     const int *q_req, *q_kvlen, *indptr, *indices;
     int* blocks;
     long q_stride;
-    int n_rows, n_req, Hq, Hkv, max_kvlen, n_pages, page_size, block, top, first, last;
+    int n_rows, n_req, Hq, Hkv, max_kvlen, n_pages, page_size, block, top, first, last, stride;
 };
 // order of the scores as unsigned numbers; 0 is below all of them
 __device__ __forceinline__ u32 score_key(float s) {
@@ -292,87 +292,231 @@ __device__ __forceinline__ int q_steps(float x, float inv) {
     const float t = fminf(fmaxf(__builtin_rintf(x * inv), -127.0f), 127.0f);
     return x == x ? (int)t : 0;
 }
-// one block of threads a row and kv head
-template <int F16, int D>
-__global__ __launch_bounds__(256) void k_block_select(SelectArgs a) {
-    extern __shared__ u32 key[];                                    // of every candidate
-    __shared__ int sum_pos[D], sum_neg[D], red[4];
-    __shared__ float redf[4];
-    const int i = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, G = a.Hq / a.Hkv;
-    int n = a.q_kvlen[i];
-    const int r = a.q_req[i];
-    if (n <= 0 || r < 0 || r >= a.n_req) return;
-    n = min(n, a.max_kvlen);
-    int* const out = a.blocks + ((size_t)i * a.Hkv + h) * a.top;
-    const int have = (n + a.block - 1) / a.block;
-    if (have <= a.top) {
-        for (int j = tid; j < a.top; j += 256) out[j] = j < have ? j : -1;
-        return;
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+// The scores of QT rows of one request (or of one row) and a kv head, then their choice.
+//   sum over heads and channels of max(a hi, a lo) = sum over channels of P hi + N lo, P = sum over heads of max(a, 0), N of min(a, 0): one product of 2 dim
+// whole numbers however many heads there are.  P and N have up to 13 bits; 64 times their high part and their low six bits are two rows of an 8-bit matrix
+// product, so 16 rows of it are 8 query rows, and 16 blocks its columns: C's lanes have both rows of a query beside each other.
+// A tile of 16 (or 8) query rows reads the bounds of a request's blocks once; what a choice costs is its rounds over the keys, in a wave's registers.
+// The keys of all candidates lie in LDS: [row][SEL_STRIDE(blocks)].
+#define SEL_PAD 8
+// keys of one row, a wave's or W waves' (W > 1: all threads call): the need largest, older first where equal, written in order of their index
+template <int KPL, int W>
+__device__ __forceinline__ void choose(const u32* key, int lo, int cand, int need, int first, int last, int have, int top, int* out, int lane, int wave, int (*red)[16]) {
+    u32 k[KPL];
+    const int c0 = W > 1 ? wave * KPL * 64 : 0;
+    u32 least = 0xffffffffu, most = 0;
+#pragma unroll
+    for (int i = 0; i < KPL; ++i) {
+        const int c = c0 + i * 64 + lane;
+        const bool in = c < cand;
+        k[i] = in ? key[lo + c] : 0;                                 // (0: below every key but that of a block without a page, and counted with care)
+        least = min(least, in ? k[i] : 0xffffffffu);
+        most = max(most, k[i]);
     }
-    const bf16_t* const q = a.q + (size_t)i * a.q_stride + (size_t)h * G * D;
-    float amax = 0.0f;
-    for (int e = tid; e < G * D; e += 256) amax = fmaxf(amax, finite_abs(elem_f<F16>(q[e])));
-    for (int o = 1; o < 64; o <<= 1) amax = fmaxf(amax, __shfl_xor(amax, o, 64));
-    if (lane == 0) redf[wave] = amax;
-    __syncthreads();
-    const float inv = 1.0f / step_of(fmaxf(fmaxf(redf[0], redf[1]), fmaxf(redf[2], redf[3])));
-    for (int d = tid; d < D; d += 256) {
-        int p = 0, m = 0;
-        for (int g = 0; g < G; ++g) {
-            const int s = q_steps(elem_f<F16>(q[g * D + d]), inv);
-            p += max(s, 0); m += min(s, 0);
+    int turn_ = 0;
+    auto total = [&](int x) {                                        // over the row's waves
+        if constexpr (W > 1) {
+            int* const r = red[turn_ & 1];
+            ++turn_;
+            if (lane == 0) r[wave] = x;
+            __syncthreads();
+            x = 0;
+#pragma unroll
+            for (int w = 0; w < W; ++w) x += r[w];
         }
-        sum_pos[d] = p; sum_neg[d] = m;
+        return x;
+    };
+    // the need-th largest key t lies in [a, b): at least need keys reach a, fewer reach b
+    for (int o = 1; o < 64; o <<= 1) {
+        least = min(least, (u32)__shfl_xor((int)least, o, 64));
+        most = max(most, (u32)__shfl_xor((int)most, o, 64));
     }
-    __syncthreads();
-    const int per = a.page_size / a.block, lo = a.first, cand = have - a.last - a.first, need = a.top - a.first - a.last;
-    const int p0 = a.indptr[r], np = a.indptr[r + 1] - p0;
-    for (int c = tid; c < cand; c += 256) {
-        const int j = lo + c, pj = j / per;
-        const int pg = pj < np ? a.indices[p0 + pj] : -1;
-        u32 k = 0;                                                  // a block without a page: behind all others
-        if (pg >= 0 && pg < a.n_pages) {
-            const size_t at = ((size_t)pg * a.Hkv + h) * per + j % per;
-            const int8_t* const b = a.bounds + at * 2 * D;
-            int s = 0;
-            for (int d = 0; d < D; ++d) s += sum_pos[d] * b[d] + sum_neg[d] * b[D + d];
-            k = score_key((float)s * a.steps[at]);
+    if constexpr (W > 1) {
+        u32* const r = reinterpret_cast<u32*>(red[2]);
+        u32* const s = reinterpret_cast<u32*>(red[3]);
+        if (lane == 0) { r[wave] = least; s[wave] = most; }
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < W; ++w) { least = min(least, r[w]); most = max(most, s[w]); }
+    }
+    least = __builtin_amdgcn_readfirstlane(least);
+    most = __builtin_amdgcn_readfirstlane(most);
+    u32 a = least, t = least, above = 0;
+    unsigned long long b = (unsigned long long)most + 1;
+    bool exact = false;                                              // exactly `need` keys reach t: no ties to break
+    if (need == 0) { t = 0xffffffffu; exact = true; }
+    while (!exact && b - a > 1) {
+        const u32 mid = a + (u32)((b - a) >> 1);
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < KPL; ++i) n += (int)__popcll(__ballot(k[i] >= mid));      // (mid > least >= 0: lanes outside, 0, never reach it)
+        n = total(n);
+        if (n >= need) a = mid; else b = mid;
+        if (n == need) { exact = true; }
+        t = a;
+    }
+    (void)above;
+    // keys above t, and the oldest equal ones
+    int gt = 0, eq = 0;
+    if (need && !exact) {
+#pragma unroll
+        for (int i = 0; i < KPL; ++i) {
+            const bool in = c0 + i * 64 + lane < cand;
+            gt += (int)__popcll(__ballot(in && k[i] > t));
+            eq += (int)__popcll(__ballot(in && k[i] == t));
         }
-        key[c] = k;
+    } else if (need) {
+#pragma unroll
+        for (int i = 0; i < KPL; ++i) gt += (int)__popcll(__ballot(c0 + i * 64 + lane < cand && k[i] >= t));
     }
-    __syncthreads();
-    // the need-th largest key, bit by bit: the largest t that at least `need` keys reach
-    u32 t = 0;
-    for (int bit = 31; bit >= 0; --bit) {
-        const u32 at = t | (1u << bit);
-        int count = 0;
-        for (int c = tid; c < cand; c += 256) count += key[c] >= at;
-        for (int o = 1; o < 64; o <<= 1) count += __shfl_xor(count, o, 64);
-        if (lane == 0) red[wave] = count;
+    int gt_before = 0, eq_before = 0, gt_all = gt;
+    if constexpr (W > 1) {
         __syncthreads();
-        if (red[0] + red[1] + red[2] + red[3] >= need) t = at;
+        if (lane == 0) { red[0][wave] = gt; red[1][wave] = eq; }
         __syncthreads();
+        gt_all = 0;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            if (w < wave) { gt_before += red[0][w]; eq_before += red[1][w]; }
+            gt_all += red[0][w];
+        }
     }
-    if (wave) return;
-    // in order of their index: larger keys, and as many equal ones as are left
-    int above = 0;
-    for (int c = lane; c < cand; c += 64) above += key[c] > t;
-    for (int o = 1; o < 64; o <<= 1) above += __shfl_xor(above, o, 64);
-    int ties = need - above, at = a.first;
-    for (int j = lane; j < a.first; j += 64) out[j] = j;
+    int ties = exact ? 0 : need - gt_all;                            // equal ones to take, from the oldest
     const unsigned long long below = lane ? ~0ull >> (64 - lane) : 0ull;
-    for (int c0 = 0; c0 < cand; c0 += 64) {
-        const int c = c0 + lane;
-        const u32 k = c < cand ? key[c] : 0;
-        const bool eq = c < cand && k == t, gt = c < cand && k > t;
-        const unsigned long long be = __ballot(eq);
-        const bool take = gt || (eq && __popcll(be & below) < ties);
+    int at = first + gt_before + min(eq_before, ties);
+    ties = max(ties - eq_before, 0);
+#pragma unroll
+    for (int i = 0; i < KPL; ++i) {
+        if (c0 + i * 64 >= cand || need == 0) break;
+        const bool in = c0 + i * 64 + lane < cand, e = in && !exact && k[i] == t, g = in && (exact ? k[i] >= t : k[i] > t);
+        const unsigned long long be = __ballot(e);
+        const bool take = g || (e && (int)__popcll(be & below) < ties);
         const unsigned long long bt = __ballot(take);
-        if (take) out[at + __popcll(bt & below)] = lo + c;
-        at += __popcll(bt);
+        if (take) out[at + (int)__popcll(bt & below)] = lo + c0 + i * 64 + lane;
+        at += (int)__popcll(bt);
         ties -= min(ties, (int)__popcll(be));
     }
-    for (int j = lane; j < a.last; j += 64) out[at + j] = have - a.last + j;
+    if (W == 1 || wave == 0) {
+        for (int j = lane; j < first; j += 64) out[j] = j;
+        for (int j = lane; j < last; j += 64) out[top - last + j] = have - last + j;
+    }
+}
+
+// QT > 1: tiles of QT rows, a wave a row in the choice; QT == 1: a row, all waves together
+template <int F16, int D, int QT, int W>
+__global__ __launch_bounds__(64 * W) void k_block_select(SelectArgs a) {
+    constexpr int MT = (2 * QT + 15) / 16, KS = 2 * D / 64;          // tiles of 16 product rows, steps of 64 numbers
+    extern __shared__ __attribute__((aligned(16))) u32 keys[];       // [QT][a.stride]
+    __shared__ __attribute__((aligned(16))) int8_t s_a[MT * 16][2 * D];
+    __shared__ int s_len[QT], s_req[QT], red[4][16];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
+    const int h = blockIdx.x % a.Hkv, i0 = blockIdx.x / a.Hkv * QT, R = min(QT, a.n_rows - i0), G = a.Hq / a.Hkv, per = a.page_size / a.block;
+    if (tid < QT) {
+        int n = 0, r = -1;
+        if (tid < R) {
+            n = a.q_kvlen[i0 + tid];
+            r = a.q_req[i0 + tid];
+            if (n <= 0 || r < 0 || r >= a.n_req) { n = 0; r = -1; }
+            n = min(n, a.max_kvlen);
+            if (n == 0) r = -1;
+        }
+        s_len[tid] = n; s_req[tid] = r;
+    }
+    if constexpr (QT < 8) for (int x = tid; x < (MT * 16 - 2 * QT) * 2 * D / 4; x += 64 * W) reinterpret_cast<int*>(s_a[2 * QT])[x] = 0;
+    // P and N of the rows, a wave a row
+    for (int r = wave; r < R; r += W) {
+        const bf16_t* const q = a.q + (size_t)(i0 + r) * a.q_stride + (size_t)h * G * D;
+        float amax = 0.0f;
+        for (int e = lane; e < G * D; e += 64) amax = fmaxf(amax, finite_abs(elem_f<F16>(q[e])));
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) amax = fmaxf(amax, __shfl_xor(amax, o, 64));
+        const float inv = 1.0f / step_of(amax);
+#pragma unroll
+        for (int x = 0; x < D / 64; ++x) {
+            const int d = lane + 64 * x;
+            int p = 0, m = 0;
+            for (int e = 0; e < G; ++e) {
+                const int s = q_steps(elem_f<F16>(q[e * D + d]), inv);
+                p += max(s, 0); m += min(s, 0);
+            }
+            s_a[2 * r][d] = (int8_t)(p & 63); s_a[2 * r + 1][d] = (int8_t)(p >> 6);
+            s_a[2 * r][D + d] = (int8_t)(m & 63); s_a[2 * r + 1][D + d] = (int8_t)(m >> 6);
+        }
+    }
+    __syncthreads();
+    i32x4 av[MT][KS];
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int s = 0; s < KS; ++s) av[t][s] = *reinterpret_cast<const i32x4*>(&s_a[16 * t + c][64 * s + 16 * g]);
+
+    for (int ra = 0; ra < R;) {
+        if (s_req[ra] < 0) { ++ra; continue; }
+        int rb = ra + 1;
+        while (rb < R && s_req[rb] == s_req[ra]) ++rb;
+        const int req = s_req[ra], p0 = a.indptr[req], np = a.indptr[req + 1] - p0;
+        int n_most = 0;
+        for (int r = ra; r < rb; ++r) n_most = max(n_most, s_len[r]);
+        const int have = (n_most + a.block - 1) / a.block, j1 = have > a.top ? have - a.last : 0;      // blocks to score: [first, j1)
+        constexpr int U = 4;                                         // tiles of 16 blocks in flight
+        for (int j0 = a.first + wave * 16 * U; j0 < j1; j0 += W * 16 * U) {
+            int pg[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int j = j0 + 16 * u + c, pj = j / per;
+                pg[u] = j < j1 && pj < np ? a.indices[p0 + pj] : -1;
+            }
+            i32x4 b[U][KS];
+            float st[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int j = j0 + 16 * u + c;
+                const bool ok = pg[u] >= 0 && pg[u] < a.n_pages;
+                const size_t at = ok ? ((size_t)pg[u] * a.Hkv + h) * per + j % per : 0;
+                const i32x4* const src = reinterpret_cast<const i32x4*>(a.bounds + at * 2 * D) + g;
+#pragma unroll
+                for (int s = 0; s < KS; ++s) b[u][s] = src[4 * s];
+                st[u] = a.steps[at];
+                pg[u] = ok;
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int j = j0 + 16 * u + c;
+#pragma unroll
+                for (int t = 0; t < MT; ++t) {
+                    i32x4 s4 = {0, 0, 0, 0};
+#pragma unroll
+                    for (int s = 0; s < KS; ++s) s4 = __builtin_amdgcn_mfma_i32_16x16x64_i8(av[t][s], b[u][s], s4, 0, 0, 0);
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {                    // product rows 4 g + 2 x, + 1: query row 8 t + 2 g + x
+                        const int r = 8 * t + 2 * g + x;
+                        if (j < j1 && r < QT) keys[(size_t)r * a.stride + j] = pg[u] ? score_key((float)(s4[2 * x] + 64 * s4[2 * x + 1]) * st[u]) : 0;
+                    }
+                }
+            }
+        }
+        __syncthreads();
+        for (int r = ra + (QT > 1 ? wave : 0); r < rb; r += QT > 1 ? W : 1) {
+            const int mine = (s_len[r] + a.block - 1) / a.block, cand = mine - a.first - a.last, need = a.top - a.first - a.last;
+            int* const out = a.blocks + ((size_t)(i0 + r) * a.Hkv + h) * a.top;
+            if (mine <= a.top) {
+                for (int j = QT > 1 ? lane : tid; j < a.top; j += QT > 1 ? 64 : 64 * W) out[j] = j < mine ? j : -1;
+                continue;
+            }
+            const u32* const key = keys + (size_t)r * a.stride;
+            constexpr int GW = QT > 1 ? 1 : W;
+#define CHOOSE(KPL) choose<KPL, GW>(key, a.first, cand, need, a.first, a.last, mine, a.top, out, lane, wave, red)
+            if (cand <= 4 * 64 * GW) CHOOSE(4);
+            else if (cand <= 8 * 64 * GW) CHOOSE(8);
+            else if (cand <= 16 * 64 * GW) CHOOSE(16);
+            else if constexpr (QT == 1 || QT == 8) { if (cand <= 32 * 64 * GW) CHOOSE(32); else CHOOSE(64); }
+#undef CHOOSE
+        }
+        __syncthreads();
+        ra = rb;
+    }
 }
 
 // ================================================================================================
@@ -874,10 +1018,20 @@ int vox_block_select(vox_ctx* ctx, void* stream, const vox_block_select_args* a)
     const vox_block_rows& r = a->rows;
     if (r.n_rows == 0) return VOX_OK;
     if (!a->q || !a->blocks || (size_t)a->q & 1) return vox_fail(VOX_ERR_INVALID, "block_select: an operand is NULL, or does not lie on its type");
-    SelectArgs s{(const bf16_t*)a->q, c.bounds, c.steps, r.q_req, r.q_kvlen, r.kv_indptr, r.kv_indices, a->blocks, (long)a->q_stride,
-                 r.n_rows, r.n_req, r.heads, c.kv_heads, r.max_kvlen, c.n_pages, c.page_size, c.block, a->top, a->first, a->last};
     const int most = (r.max_kvlen + c.block - 1) / c.block;
-    return launch(BY_TYPE_AND_DIM(k_block_select, c), dim3(r.n_rows, c.kv_heads), 256, (size_t)most * 4, (hipStream_t)stream, s);
+    // rows a tile: 16 while their keys take half a CU's LDS, 8 while they take most of it (4096 blocks), else (and for rows of different requests) one
+    const bool many = r.n_own > 0 && r.n_rows >= 2 * r.n_own;
+    const int qt = many && most <= 1024 ? 16 : many && most <= 4096 ? 8 : 1;
+    const int W = qt > 1 ? 8 : most <= 512 ? 4 : 16;
+    SelectArgs s{(const bf16_t*)a->q, c.bounds, c.steps, r.q_req, r.q_kvlen, r.kv_indptr, r.kv_indices, a->blocks, (long)a->q_stride,
+                 r.n_rows, r.n_req, r.heads, c.kv_heads, r.max_kvlen, c.n_pages, c.page_size, c.block, a->top, a->first, a->last, most + (qt > 1 ? SEL_PAD : 0)};
+    const int64_t grid = (int64_t)((r.n_rows + qt - 1) / qt) * c.kv_heads;
+    if (grid > 0x7fffffff) return vox_fail(VOX_ERR_INVALID, "block_select: %d rows of %d kv heads are more than a launch holds", r.n_rows, c.kv_heads);
+#define SELECT_OF(QT, W) (c.dtype == VOX_DTYPE_F16 ? (c.head_dim == 128 ? (const void*)k_block_select<1, 128, QT, W> : (const void*)k_block_select<1, 64, QT, W>) \
+                                                  : (c.head_dim == 128 ? (const void*)k_block_select<0, 128, QT, W> : (const void*)k_block_select<0, 64, QT, W>))
+    const void* kern = qt == 16 ? SELECT_OF(16, 8) : qt == 8 ? SELECT_OF(8, 8) : W == 4 ? SELECT_OF(1, 4) : SELECT_OF(1, 16);
+#undef SELECT_OF
+    return launch(kern, dim3((unsigned)grid), 64 * W, (size_t)qt * s.stride * 4, (hipStream_t)stream, s);
 }
 
 static int check_attention(const vox_block_attention_args* a) {

@@ -1,5 +1,7 @@
 // Long contexts: rows rotated into a paged cache, the bounds of its blocks, the blocks that a row reads, and attention over them
 // (voxhip.h: vox_rope_append, vox_block_bounds, vox_block_select, vox_block_attention).
+#include <type_traits>
+
 #include "vox_internal.h"
 
 typedef _Float16 half_t;
@@ -37,6 +39,7 @@ static int check_cache(const char* who, const vox_block_cache& c, bool bounds) {
     if (c.dtype != VOX_DTYPE_BF16 && c.dtype != VOX_DTYPE_F16) return vox_fail(VOX_ERR_INVALID, "%s: dtype %d", who, c.dtype);
     if ((size_t)c.kv & 15) return vox_fail(VOX_ERR_INVALID, "%s: the cache does not lie on 16 bytes", who);
     if (!bounds) return VOX_OK;
+    if ((int64_t)c.n_pages * c.page_size > 0x7fffffff) return vox_fail(VOX_ERR_INVALID, "%s: %d pages of %d tokens are 2^31 or more", who, c.n_pages, c.page_size);
     if (c.block != 16 && c.block != 32 && c.block != 64 && c.block != 128) return vox_fail(VOX_ERR_INVALID, "%s: blocks of %d tokens (16, 32, 64 or 128)", who, c.block);
     if (c.page_size % c.block) return vox_fail(VOX_ERR_INVALID, "%s: pages of %d tokens are not whole blocks of %d", who, c.page_size, c.block);
     if (c.head_dim != 64 && c.head_dim != 128) return vox_fail(VOX_ERR_INVALID, "%s: head_dim %d (64 or 128)", who, c.head_dim);
@@ -411,7 +414,7 @@ __global__ __launch_bounds__(64 * W) void k_block_select(SelectArgs a) {
     extern __shared__ __attribute__((aligned(16))) u32 keys[];       // [QT][a.stride]
     __shared__ __attribute__((aligned(16))) int8_t s_a[MT * 16][2 * D];
     __shared__ int s_len[QT], s_req[QT], red[4][16];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
     const int h = blockIdx.x % a.Hkv, i0 = blockIdx.x / a.Hkv * QT, R = min(QT, a.n_rows - i0), G = a.Hq / a.Hkv, per = a.page_size / a.block;
     if (tid < QT) {
         int n = 0, r = -1;
@@ -453,12 +456,14 @@ __global__ __launch_bounds__(64 * W) void k_block_select(SelectArgs a) {
         for (int s = 0; s < KS; ++s) av[t][s] = *reinterpret_cast<const i32x4*>(&s_a[16 * t + c][64 * s + 16 * g]);
 
     for (int ra = 0; ra < R;) {
-        if (s_req[ra] < 0) { ++ra; continue; }
+        const int req = __builtin_amdgcn_readfirstlane(s_req[ra]);
+        if (req < 0) { ++ra; continue; }
         int rb = ra + 1;
-        while (rb < R && s_req[rb] == s_req[ra]) ++rb;
-        const int req = s_req[ra], p0 = a.indptr[req], np = a.indptr[req + 1] - p0;
+        while (rb < R && __builtin_amdgcn_readfirstlane(s_req[rb]) == req) ++rb;
+        const int p0 = a.indptr[req], np = a.indptr[req + 1] - p0;
         int n_most = 0;
         for (int r = ra; r < rb; ++r) n_most = max(n_most, s_len[r]);
+        n_most = __builtin_amdgcn_readfirstlane(n_most);
         const int have = (n_most + a.block - 1) / a.block, j1 = have > a.top ? have - a.last : 0;      // blocks to score: [first, j1)
         constexpr int U = 4;                                         // tiles of 16 blocks in flight
         for (int j0 = a.first + wave * 16 * U; j0 < j1; j0 += W * 16 * U) {
@@ -569,20 +574,20 @@ struct BlockAttnArgs {
     long q_stride;
     float scale2;                        // scale log2 e
     int n_rows, n_req, Hq, Hkv, max_kvlen, n_pages, page_size, block, top;
-    int per_tile, splits, head_tiles, cols, q_al, out_al;      // cols: columns of a wave in the merge's LDS
+    int splits, head_tiles, cols, q_al, out_al;      // cols: columns of a wave in the merge's LDS
 };
 #define ATTN_CUS 256                     // of an MI355X
 #define ATTN_WINDOW 4096                 // blocks whose rows' bits lie in LDS at a time (rows of several: 8 KB)
 
-// The entries of a row's list that count, 64 at a time, by one wave: f(j, counts) for every lane.
+// The entries of a row's list that count, 64 at a time, by one wave: f(j, counts) for every lane.  first: the lane's entry of the first 64.
 template <class F>
-__device__ __forceinline__ void row_entries(const int* list, int top, int have, int lane, F f) {
+__device__ __forceinline__ void row_entries(const int* list, int first, int top, int have, int lane, F f) {
     int carry = -1;
     for (int e0 = 0; e0 < top; e0 += 64) {
-        const int j = e0 + lane < top ? list[e0 + lane] : -1;
+        const int j = e0 == 0 ? first : e0 + lane < top ? list[e0 + lane] : -1;
         int most = j;                                                // the largest entry up to this one
         const int prev = __shfl_up(j, 1, 64);
-        if (__ballot(lane && j >= 0 && j <= prev) || __ballot(lane && j >= 0 && prev < 0))      // (not simply ascending)
+        if (__ballot(lane && j >= 0 && (j <= prev || prev < 0)))     // (not simply ascending)
             for (int o = 1; o < 64; o <<= 1) {
                 const int x = __shfl_up(most, o, 64);
                 if (lane >= o) most = max(most, x);
@@ -597,302 +602,486 @@ __device__ __forceinline__ void row_entries(const int* list, int top, int have, 
         }
     }
 }
+__device__ __forceinline__ int first_entry(const int* list, int top, int lane) { return lane < top ? list[lane] : -1; }
 
-template <int F16, int D, int W, bool ONE>
-__global__ __launch_bounds__(64 * W, W == 4 ? 2 : 1) void k_block_attn(BlockAttnArgs a) {
-    constexpr int CPL = D / 16, KS = D / 32, OS = D + 4;             // channels a lane, steps of a K row, floats a column of the merge
-    extern __shared__ __attribute__((aligned(16))) char lds[];
-    __shared__ int s_len[16], s_req[16], s_count[W + 1], s_next, s_seen;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
+// T tiles of 16 tokens as a wave's registers: K's rows, V's rows.  (Loads of one tile; at: its first token's place in the cache, [page][2][page_size] flat)
+template <int D, int T>
+struct AttnTiles {
+    static constexpr int CPL = D / 16, KS = D / 32;
+    uint4 k[T][KS];
+    u32 v[T][4][CPL / 2];
+    __device__ __forceinline__ void load(int x, const bf16_t* kv, u32 at, size_t row_el, size_t v_el, int c, int g) {
+        const bf16_t* const kb = kv + (size_t)at * row_el;
+        const bf16_t* const vb = kb + v_el;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) k[x][s] = *reinterpret_cast<const uint4*>(kb + (size_t)c * row_el + 32 * s + 8 * g);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const bf16_t* const src = vb + (size_t)(4 * g + i) * row_el + CPL * c;
+            if constexpr (CPL == 8) {
+                const uint4 t = *reinterpret_cast<const uint4*>(src);
+                v[x][i][0] = t.x; v[x][i][1] = t.y; v[x][i][2] = t.z; v[x][i][3] = t.w;
+            } else {
+                const uint2 t = *reinterpret_cast<const uint2*>(src);
+                v[x][i][0] = t.x; v[x][i][1] = t.y;
+            }
+        }
+    }
+    // V of the tile's tokens from `from` on is zero (the others may hold anything: weight 0 times it would not be 0)
+    __device__ __forceinline__ void drop_v(int x, int from, int g) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int w = 0; w < CPL / 2; ++w) v[x][i][w] = 4 * g + i >= from ? 0u : v[x][i][w];
+    }
+    // V^T's rows of the product over tiles 2 y and 2 y + 1: channel CPL c + t of the lane's eight tokens
+    __device__ __forceinline__ uint4 vt(int y, int t) const {
+        const u32 sel = t & 1 ? 0x07060302u : 0x05040100u;
+        u32 w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_perm(v[2 * y + (i >> 1)][2 * (i & 1) + 1][t >> 1], v[2 * y + (i >> 1)][2 * (i & 1)][t >> 1], sel);
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+};
+// A tile of columns against T tiles of tokens.  sees[x]: how many of the lane's tokens 4 g, 4 g + 1, .. of tile x its column sees (any number: 4 and more are all).
+// CAREFUL: V that is not finite meets the weight as one term.
+template <int F16, int D, int T, bool CAREFUL>
+__device__ __forceinline__ void attend_tiles(const AttnTiles<D, T>& f, const uint4 (&vt)[T / 2][D / 16], const uint4 (&q)[D / 32], const int (&sees)[T], float scale2, float& m, float& l, f32x4 (&o)[D / 16]) {
+    constexpr int CPL = D / 16, KS = D / 32;
     const float inf = __uint_as_float(0x7f800000u);
-    // block -> (kv head, tile of heads, split, tile of rows): neighbours are kv heads, so that a die's L2 keeps its heads' tokens
+    float p[4 * T];
+#pragma unroll
+    for (int x = 0; x < T; ++x) {
+        f32x4 s4 = {0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < KS; ++s) s4 = mma32<F16>(f.k[x][s], q[s], s4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[4 * x + i] = i < sees[x] ? s4[i] * scale2 : -inf;
+    }
+    float top = p[0];
+#pragma unroll
+    for (int i = 1; i < 4 * T; ++i) top = fmaxf(top, p[i]);
+    top = xor_max<32>(xor_max<16>(top));
+    if (__ballot(top > m)) {
+        const float now = fmaxf(m, top), keep = __builtin_amdgcn_exp2f(m - (now == -inf ? 0.0f : now));
+        m = now;
+        l *= keep;
+#pragma unroll
+        for (int t = 0; t < CPL; ++t) o[t] *= keep;
+    }
+    const float base = m == -inf ? 0.0f : m;
+    float part[T];
+#pragma unroll
+    for (int x = 0; x < T; ++x) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[4 * x + i] = __builtin_amdgcn_exp2f(p[4 * x + i] - base);
+        part[x] = (p[4 * x] + p[4 * x + 1]) + (p[4 * x + 2] + p[4 * x + 3]);
+    }
+#pragma unroll
+    for (int x = 0; x < T; ++x) l += part[x];
+#pragma unroll
+    for (int y = 0; y < T / 2; ++y) {
+        const float* const w = p + 8 * y;
+        u32 ph[4], pl[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            ph[i] = pack2<F16>(w[2 * i], w[2 * i + 1]);
+            pl[i] = pack2<F16>(w[2 * i] - elem_f<F16>((bf16_t)ph[i]), w[2 * i + 1] - elem_f<F16>((bf16_t)(ph[i] >> 16)));
+        }
+        const uint4 bh = make_uint4(ph[0], ph[1], ph[2], ph[3]), bl = make_uint4(pl[0], pl[1], pl[2], pl[3]);
+        if constexpr (CAREFUL) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)                              // (one term, not zero where the weight is not)
+                ph[i] |= (w[2 * i] > 0.0f && !(ph[i] & 0xffffu) ? 1u : 0u) | (w[2 * i + 1] > 0.0f && !(ph[i] >> 16) ? 0x10000u : 0u);
+            const uint4 one = make_uint4(ph[0], ph[1], ph[2], ph[3]);
+#pragma unroll
+            for (int t = 0; t < CPL; ++t) {
+                const uint4 a = vt[y][t], odd = make_uint4(a.x & halves_not_finite<F16>(a.x), a.y & halves_not_finite<F16>(a.y), a.z & halves_not_finite<F16>(a.z), a.w & halves_not_finite<F16>(a.w));
+                const uint4 fine = make_uint4(a.x ^ odd.x, a.y ^ odd.y, a.z ^ odd.z, a.w ^ odd.w);
+                o[t] = mma32<F16>(odd, one, o[t]);
+                o[t] = mma32<F16>(fine, bh, o[t]);
+                o[t] = mma32<F16>(fine, bl, o[t]);
+            }
+        } else {
+#pragma unroll
+            for (int t = 0; t < CPL; ++t) {
+                o[t] = mma32<F16>(vt[y][t], bh, o[t]);
+                o[t] = mma32<F16>(vt[y][t], bl, o[t]);
+            }
+        }
+    }
+}
+// a tile of columns of one wave, into the merge's LDS: s_o [wave][column][D + 4], s_ml [wave][column]
+template <int D>
+__device__ __forceinline__ void put_columns(float* s_o, float2* s_ml, int wave, int cols, int c, int g, float m, float l, const f32x4 (&o)[D / 16]) {
+    constexpr int CPL = D / 16;
+    l = xor_add<32>(xor_add<16>(l));
+    if (c >= cols) return;
+    float* const dst = s_o + (wave * cols + c) * (D + 4) + 4 * g * CPL;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int t = 0; t < CPL; t += 4) *reinterpret_cast<float4*>(dst + i * CPL + t) = make_float4(o[t][i], o[t + 1][i], o[t + 2][i], o[t + 3][i]);
+    if (g == 0) s_ml[wave * cols + c] = make_float2(m, l);
+}
+// four channels of a column of all waves; false: not finite
+template <int D, int W>
+__device__ __forceinline__ bool merge_columns(const float* s_o, const float2* s_ml, int cols, int cc, int d, float& m, float& sum, float (&acc)[4]) {
+    const float inf = __uint_as_float(0x7f800000u);
+    float2 ml[W];
+    float4 o[W];
+#pragma unroll
+    for (int w = 0; w < W; ++w) { ml[w] = s_ml[w * cols + cc]; o[w] = *reinterpret_cast<const float4*>(s_o + (w * cols + cc) * (D + 4) + d); }
+    m = -inf; sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) m = fmaxf(m, ml[w].x);
+    const float base = m == -inf ? 0.0f : m;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) acc[x] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+        const float f = __builtin_amdgcn_exp2f(ml[w].x - base);
+        sum = __fmaf_rn(f, ml[w].y, sum);
+        acc[0] = __fmaf_rn(f, o[w].x, acc[0]); acc[1] = __fmaf_rn(f, o[w].y, acc[1]); acc[2] = __fmaf_rn(f, o[w].z, acc[2]); acc[3] = __fmaf_rn(f, o[w].w, acc[3]);
+    }
+    return fabsf(sum) < inf && fabsf(acc[0]) < inf && fabsf(acc[1]) < inf && fabsf(acc[2]) < inf && fabsf(acc[3]) < inf;
+}
+// acc / sum (by one reciprocal: 2^-23 more beside the output's 2^-9), or zero where a row lists nothing
+template <int F16>
+__device__ __forceinline__ void store_columns(bf16_t* dst, int aligned, bool seen, float sum, const float (&acc)[4]) {
+    const float r = 1.0f / sum;
+    u32 w[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) w[x] = seen ? pack2<F16>(acc[2 * x] * r, acc[2 * x + 1] * r) : 0u;
+    if (aligned) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+    else
+#pragma unroll
+        for (int x = 0; x < 4; ++x) dst[x] = (bf16_t)(w[x / 2] >> (16 * (x & 1)));
+}
+// the lane's part of a column's q
+template <int D>
+__device__ __forceinline__ void load_q(uint4 (&q)[D / 32], const bf16_t* src, int aligned, bool col) {
+    if (aligned) {
+#pragma unroll
+        for (int s = 0; s < D / 32; ++s) q[s] = *reinterpret_cast<const uint4*>(src + 32 * s);
+    } else {
+#pragma unroll
+        for (int s = 0; s < D / 32; ++s) {
+            u32 w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = (u32)src[32 * s + 2 * i] | ((u32)src[32 * s + 2 * i + 1] << 16);
+            q[s] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+#pragma unroll
+    for (int s = 0; s < D / 32; ++s) q[s] = col ? q[s] : make_uint4(0, 0, 0, 0);
+}
+
+// A row (and up to 16 of its heads of a kv head); its list split over `splits` blocks of threads.  A wave takes 64 tokens at a time, all of their K and V asked for at
+// once.  A list of up to 64 entries lies in each wave's lanes (LONG: in LDS).
+template <int F16, int D, int W, bool LONG>
+__global__ __launch_bounds__(64 * W, 1) void k_block_attn_row(BlockAttnArgs a) {
+    constexpr int CPL = D / 16, T = 4;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    __shared__ int s_count;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
+    const float inf = __uint_as_float(0x7f800000u);
+    // block -> (kv head, tile of heads, split, row): neighbours are kv heads, so that a die's L2 keeps its heads' tokens
     int id = blockIdx.x;
     const int h = id % a.Hkv; id /= a.Hkv;
     const int ht = id % a.head_tiles; id /= a.head_tiles;
-    const int split = id % a.splits, tile = id / a.splits;
-    const int G = a.Hq / a.Hkv, h0 = ht * 16, gh = min(G - h0, 16);  // this tile's heads
-    const int i0 = tile * a.per_tile, R = min(a.per_tile, a.n_rows - i0);
+    const int split = id % a.splits, i = id / a.splits;
+    const int* const from = a.blocks + ((size_t)i * a.Hkv + h) * a.top;
+    const int first = first_entry(from, a.top, lane);
+    int n = a.q_kvlen[i];
+    const int req = a.q_req[i], G = a.Hq / a.Hkv, h0 = ht * 16, gh = min(G - h0, 16);
+    uint4 q[D / 32];
+    load_q<D>(q, a.q + (size_t)i * a.q_stride + (size_t)(h * G + h0 + (c < gh ? c : 0)) * D + 8 * g, a.q_al, c < gh);
+    if (n <= 0 || req < 0 || req >= a.n_req || a.max_kvlen <= 0) return;
+    n = min(n, a.max_kvlen);
+    const int p0 = a.indptr[req], np = a.indptr[req + 1] - p0, per = a.page_size / a.block, have = (n - 1) / a.block + 1;
+    const int sub_shift = a.block == 16 ? 0 : a.block == 32 ? 1 : a.block == 64 ? 2 : 3;
+    const size_t row_el = (size_t)a.Hkv * D, v_el = (size_t)a.page_size * row_el;
+    const bf16_t* const kv = a.kv + (size_t)h * D;
+    // the entries that count: their block, and its first token's place
+    uint2* const list = reinterpret_cast<uint2*>(lds);
+    int count = 0;
+    u32 e_block = 0, e_at = 0;
+    auto entry = [&](int j, bool ok, u32& at) {
+        const int pj = j / per;
+        int pg = -1;
+        if (ok && pj < np) pg = a.indices[p0 + pj];
+        at = (u32)pg * 2 * a.page_size + (u32)(j - pj * per) * a.block;
+        return pg >= 0 && pg < a.n_pages;
+    };
+    if constexpr (LONG) {
+        if (wave == 0) {
+            row_entries(from, first, a.top, have, lane, [&](int j, bool ok) {
+                u32 at;
+                ok = entry(j, ok, at);
+                const unsigned long long b = __ballot(ok);
+                if (ok) list[count + __popcll(b & ((1ull << lane) - 1))] = make_uint2((u32)j, at);
+                count += __popcll(b);
+            });
+            if (lane == 0) s_count = count;
+        }
+        __syncthreads();
+        count = __builtin_amdgcn_readfirstlane(s_count);
+    } else {
+        row_entries(from, first, a.top, have, lane, [&](int j, bool ok) {
+            ok = entry(j, ok, e_at);
+            e_block = (u32)j;
+            const unsigned long long b = __ballot(ok);
+            count = (int)__popcll(b);
+            if (b & (b + 1)) {                                       // (not all in front: they move there)
+                const int rank = (int)__popcll(b & ((1ull << lane) - 1)), to = 4 * (ok ? rank : 63 - (lane - rank));
+                e_block = __builtin_amdgcn_ds_permute(to, e_block);
+                e_at = __builtin_amdgcn_ds_permute(to, e_at);
+            }
+        });
+        count = __builtin_amdgcn_readfirstlane(count);
+    }
+    float* const s_o = reinterpret_cast<float*>(lds + (LONG ? (size_t)a.top * 8 + 15 & ~(size_t)15 : 0));
+    float2* const s_ml = reinterpret_cast<float2*>(s_o + W * a.cols * (D + 4));
+    const int units = ((count << sub_shift) + T - 1) / T, u0 = (int)((long)units * split / a.splits), u1 = (int)((long)units * (split + 1) / a.splits);
+
+    for (int careful = 0;; ++careful) {
+        float m = -inf, l = 0.0f;
+        f32x4 o[CPL];
+#pragma unroll
+        for (int t = 0; t < CPL; ++t) o[t] = f32x4{0, 0, 0, 0};
+        auto go = [&](auto is_careful) {
+            for (int u = u0 + wave; u < u1; u += W) {
+                AttnTiles<D, T> f;
+                int sees[T], tok[T];
+#pragma unroll
+                for (int x = 0; x < T; ++x) {
+                    const int sub = T * u + x, e = sub >> sub_shift, part = 16 * (sub & ((1 << sub_shift) - 1)), at = min(e, count - 1);
+                    // (scalars: what a wave's branches go by, for a matrix instruction runs whatever the lanes' mask says)
+                    u32 block, place;
+                    if constexpr (LONG) { const uint2 ent = list[at]; block = __builtin_amdgcn_readfirstlane(ent.x); place = __builtin_amdgcn_readfirstlane(ent.y); }
+                    else { block = __builtin_amdgcn_readlane(e_block, at); place = __builtin_amdgcn_readlane(e_at, at); }
+                    tok[x] = e < count ? (int)block * a.block + part : n;             // (behind the list's end: nothing)
+                    f.load(x, kv, place + part, row_el, v_el, c, g);
+                }
+#pragma unroll
+                for (int x = 0; x < T; ++x) {
+                    sees[x] = n - tok[x] - 4 * g;
+                    if (tok[x] + 16 > n) f.drop_v(x, n - tok[x], g);
+                }
+                uint4 vt[T / 2][CPL];
+#pragma unroll
+                for (int y = 0; y < T / 2; ++y)
+#pragma unroll
+                    for (int t = 0; t < CPL; ++t) vt[y][t] = f.vt(y, t);
+                attend_tiles<F16, D, T, decltype(is_careful)::value>(f, vt, q, sees, a.scale2, m, l, o);
+            }
+        };
+        if (careful) go(std::true_type{});
+        else go(std::false_type{});
+        put_columns<D>(s_o, s_ml, wave, a.cols, c, g, m, l, o);
+        __syncthreads();
+        bool bad = false;
+        for (int it = tid; it < gh * (D / 4); it += 64 * W) {
+            const int cc = it / (D / 4), d = it % (D / 4) * 4;
+            float top, sum, acc[4];
+            bad |= !merge_columns<D, W>(s_o, s_ml, a.cols, cc, d, top, sum, acc);
+            const size_t row = (size_t)i * a.Hq + h * G + h0 + cc;
+            if (a.splits > 1) {
+                *reinterpret_cast<float4*>(a.part_o + (row * a.splits + split) * D + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+                if (d == 0) *reinterpret_cast<float2*>(a.part_ml + (row * a.splits + split) * 2) = make_float2(top, count ? sum : -1.0f);      // (-1: the row lists nothing)
+            } else store_columns<F16>(a.out + row * D + d, a.out_al, count != 0, sum, acc);
+        }
+        if (careful || !__builtin_amdgcn_readfirstlane(__syncthreads_or(bad))) break;
+    }
+}
+
+// NC tiles of 16 columns whose rows share a request's blocks.  The waves of a block share the list's tokens, 32 in turn, each keeps all columns, and they meet in LDS
+// at the end; the next 32 tokens are on their way while a wave works.
+template <int D>
+struct AttnUnit {
+    AttnTiles<D, 2> f;
+    int tok[2];
+    u32 rows[2];
+};
+template <int F16, int D, int W, int NC>
+__global__ __launch_bounds__(64 * W, 1) void k_block_attn_rows(BlockAttnArgs a) {
+    constexpr int CPL = D / 16;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    __shared__ int s_len[16], s_req[16], s_count[W], s_next, s_seen;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
+    const float inf = __uint_as_float(0x7f800000u);
+    // block -> (kv head, tile of rows), kv heads neighbours as above
+    const int h = blockIdx.x % a.Hkv, tile = blockIdx.x / a.Hkv, G = a.Hq / a.Hkv, rpt = 16 / G;      // rpt: rows of a tile of columns
+    const int i0 = tile * NC * rpt, R = min(NC * rpt, a.n_rows - i0);
+    const int* const lists = a.blocks + ((size_t)i0 * a.Hkv + h) * a.top;
     if (tid < 16) {
         int len = 0, req = -1;
         if (tid < R) {
             len = a.q_kvlen[i0 + tid];
             req = a.q_req[i0 + tid];
-            if (len <= 0 || req < 0 || req >= a.n_req) { len = 0; req = -1; }
+            if (len <= 0 || req < 0 || req >= a.n_req || a.max_kvlen <= 0) { len = 0; req = -1; }
             len = min(len, a.max_kvlen);
         }
         s_len[tid] = len; s_req[tid] = req;
     }
     __syncthreads();
-    const int rc = ONE ? 0 : c / gh, hc = ONE ? c : c % gh;          // the column's row and head
-    const bool col = ONE ? c < gh : rc < R;
-    uint4 q[KS];
-    {
-        const bf16_t* const src = a.q + (size_t)(i0 + (col ? rc : 0)) * a.q_stride + (size_t)(h * G + h0 + (col ? hc : 0)) * D + 8 * g;
+    const int rc = c / G, hc = c % G;                                // the column's row (of its tile) and head
+    uint4 q[NC][D / 32];
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            if (a.q_al) q[s] = *reinterpret_cast<const uint4*>(src + 32 * s);
-            else {
-                u32 w[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] = (u32)src[32 * s + 2 * i] | ((u32)src[32 * s + 2 * i + 1] << 16);
-                q[s] = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-            if (!col) q[s] = make_uint4(0, 0, 0, 0);
-        }
+    for (int n = 0; n < NC; ++n) {
+        const bool col = rc < rpt && n * rpt + rc < R;
+        load_q<D>(q[n], a.q + (size_t)(i0 + (col ? n * rpt + rc : 0)) * a.q_stride + (size_t)(h * G + (col ? hc : 0)) * D + 8 * g, a.q_al, col);
     }
     const int sub_shift = a.block == 16 ? 0 : a.block == 32 ? 1 : a.block == 64 ? 2 : 3, per = a.page_size / a.block;
-    const size_t row_el = (size_t)a.Hkv * D;                         // elements between tokens
-    int2* const s_list = reinterpret_cast<int2*>(lds);               // {block (from the window's first) << 16 | rows, or the block (ONE); page}
-    u32* const s_bits = reinterpret_cast<u32*>(lds);                 // rows of several: two blocks' rows a word, in front of the list
-    int2* const list = ONE ? s_list : s_list + ATTN_WINDOW / 4;
-    float* const s_o = reinterpret_cast<float*>(lds);                // after the loop: [wave][column][OS]
-    float* const s_ml = s_o + W * a.cols * OS;                           // [wave][column] maximum, sum
+    const size_t row_el = (size_t)a.Hkv * D, v_el = (size_t)a.page_size * row_el;      // elements between tokens, from K to V
+    const bf16_t* const kv = a.kv + (size_t)h * D;
+    u32* const s_bits = reinterpret_cast<u32*>(lds);                 // two blocks' rows a word
+    uint2* const list = reinterpret_cast<uint2*>(lds) + ATTN_WINDOW / 4;     // {block from the window's first << 16 | rows; its first token's place}
+    float* const s_o = reinterpret_cast<float*>(lds);                // after the loop
+    float2* const s_ml = reinterpret_cast<float2*>(s_o + W * 16 * (D + 4));
 
     for (int ra = 0; ra < R;) {
-        if (s_req[ra] < 0) { ++ra; continue; }                       // (all of the block's threads read the same LDS words)
+        const int req = __builtin_amdgcn_readfirstlane(s_req[ra]);
+        if (req < 0) { ++ra; continue; }
         int rb = ra + 1;
-        while (rb < R && s_req[rb] == s_req[ra]) ++rb;
-        const int req = s_req[ra], p0 = a.indptr[req], np = a.indptr[req + 1] - p0;
-        int n_most = 0, n_least = 0x7fffffff;
-        for (int r = ra; r < rb; ++r) { n_most = max(n_most, s_len[r]); n_least = min(n_least, s_len[r]); }
-        const u32 all_rows = (rb == 32 ? 0u : 1u << rb) - (1u << ra);
-        const int own = ONE ? s_len[ra] : col && rc >= ra && rc < rb ? s_len[rc] : 0;
-
+        while (rb < R && __builtin_amdgcn_readfirstlane(s_req[rb]) == req) ++rb;
+        int n_most = 0;
+        for (int r = ra; r < rb; ++r) n_most = max(n_most, s_len[r]);
+        n_most = __builtin_amdgcn_readfirstlane(n_most);
+        const int p0 = a.indptr[req], np = a.indptr[req + 1] - p0;
+        int own[NC];                                                 // tokens that the column's row sees
+#pragma unroll
+        for (int n = 0; n < NC; ++n) {
+            const int r = n * rpt + rc;
+            own[n] = rc < rpt && r >= ra && r < rb ? s_len[r] : 0;
+        }
         for (int careful = -1;;) {                                   // -1, then, if need be, the run's rows one by one
-            float m = -inf, l = 0.0f;
-            f32x4 o[CPL];
+            float m[NC], l[NC];
+            f32x4 o[NC][CPL];
 #pragma unroll
-            for (int t = 0; t < CPL; ++t) o[t] = f32x4{0, 0, 0, 0};
-            const int v_len = careful >= 0 ? s_len[careful] : n_most;     // V of tokens from here on is taken as zero
+            for (int n = 0; n < NC; ++n) {
+                m[n] = -inf; l[n] = 0.0f;
+#pragma unroll
+                for (int t = 0; t < CPL; ++t) o[n][t] = f32x4{0, 0, 0, 0};
+            }
+            const int v_len = careful >= 0 ? __builtin_amdgcn_readfirstlane(s_len[careful]) : n_most;     // V of tokens from here on is taken as zero
             if (tid == 0) s_seen = 0;
-            __syncthreads();
-
-            for (int w0 = 0; w0 >= 0;) {                             // windows of blocks (ONE: one, of everything)
-                int count;
-                if constexpr (ONE) {
-                    if (wave == 0) {
-                        int at = 0;
-                        row_entries(a.blocks + ((size_t)i0 * a.Hkv + h) * a.top, a.top, (n_most + a.block - 1) / a.block, lane, [&](int j, bool ok) {
-                            int pg = -1;
-                            if (ok && j / per < np) pg = a.indices[p0 + j / per];
-                            ok = pg >= 0 && pg < a.n_pages;
-                            const unsigned long long b = __ballot(ok);
-                            if (ok) list[at + __popcll(b & ((1ull << lane) - 1))] = make_int2(j, pg);
-                            at += __popcll(b);
-                        });
-                        if (lane == 0) s_count[0] = at;
-                    }
-                    __syncthreads();
-                    count = s_count[0];
-                    if (tid == 0 && count) s_seen = 1;
-                    w0 = -1;
-                } else {
-                    for (int i = tid; i < ATTN_WINDOW / 2; i += 64 * W) s_bits[i] = 0;
-                    if (tid == 0) s_next = 0x7fffffff;
-                    __syncthreads();
-                    for (int r = ra + wave; r < rb; r += W)
-                        row_entries(a.blocks + ((size_t)(i0 + r) * a.Hkv + h) * a.top, a.top, (s_len[r] + a.block - 1) / a.block, lane, [&](int j, bool ok) {
-                            if (!ok || j < w0) return;
-                            if (j - w0 < ATTN_WINDOW) atomicOr(&s_bits[(j - w0) >> 1], 1u << (r + 16 * ((j - w0) & 1)));
-                            else atomicMin(&s_next, j);
-                        });
-                    __syncthreads();
-                    // the window's blocks in order: a thread counts its neighbours' share
-                    constexpr int WPT = ATTN_WINDOW / 2 / (64 * W);
-                    u32 bits[WPT];
-                    int mine = 0;
-#pragma unroll
-                    for (int i = 0; i < WPT; ++i) {
-                        bits[i] = s_bits[tid * WPT + i];
-                        mine += (bits[i] & 0xffffu ? 1 : 0) + (bits[i] >> 16 ? 1 : 0);
-                    }
-                    int upto = mine;
-                    for (int x = 1; x < 64; x <<= 1) {
-                        const int y = __shfl_up(upto, x, 64);
-                        if (lane >= x) upto += y;
-                    }
-                    if (lane == 63) s_count[wave] = upto;
-                    __syncthreads();
-                    int at = upto - mine;
-                    count = 0;
-                    for (int x = 0; x < W; ++x) { if (x < wave) at += s_count[x]; count += s_count[x]; }
-                    u32 seen = 0;
-#pragma unroll
-                    for (int i = 0; i < WPT; ++i)
-#pragma unroll
-                        for (int half = 0; half < 2; ++half) {
-                            u32 rows = half ? bits[i] >> 16 : bits[i] & 0xffffu;
-                            if (!rows) continue;
-                            const int off = (tid * WPT + i) * 2 + half, j = w0 + off;
-                            int pg = j / per < np ? a.indices[p0 + j / per] : -1;
-                            if (pg < 0 || pg >= a.n_pages) { pg = 0; rows = 0; }      // (nobody's: page 0 is read and masked)
-                            list[at++] = make_int2((int)((u32)off << 16 | rows), pg);
-                            seen |= rows;
-                        }
-                    if (seen) atomicOr(&s_seen, (int)seen);
-                    __syncthreads();
+            for (int w0 = 0; w0 >= 0;) {                             // windows of blocks
+                for (int i = tid; i < ATTN_WINDOW / 2; i += 64 * W) s_bits[i] = 0;
+                if (tid == 0) s_next = 0x7fffffff;
+                __syncthreads();
+                for (int r = ra + wave; r < rb; r += W) {
+                    const int* const from = lists + (size_t)r * a.Hkv * a.top;
+                    row_entries(from, first_entry(from, a.top, lane), a.top, (s_len[r] - 1) / a.block + 1, lane, [&](int j, bool ok) {
+                        if (!ok || j < w0) return;
+                        if (j - w0 < ATTN_WINDOW) atomicOr(&s_bits[(j - w0) >> 1], 1u << (r + 16 * ((j - w0) & 1)));
+                        else atomicMin(&s_next, j);
+                    });
                 }
+                __syncthreads();
+                // the window's blocks in order: a thread counts its neighbours' share
+                constexpr int WPT = ATTN_WINDOW / 2 / (64 * W);
+                u32 bits[WPT];
+                int mine = 0;
+#pragma unroll
+                for (int i = 0; i < WPT; ++i) {
+                    bits[i] = s_bits[tid * WPT + i];
+                    mine += (bits[i] & 0xffffu ? 1 : 0) + (bits[i] >> 16 ? 1 : 0);
+                }
+                int upto = mine;
+                for (int x = 1; x < 64; x <<= 1) {
+                    const int y = __shfl_up(upto, x, 64);
+                    if (lane >= x) upto += y;
+                }
+                if (lane == 63) s_count[wave] = upto;
+                __syncthreads();
+                int at = upto - mine, count = 0;
+                for (int x = 0; x < W; ++x) { if (x < wave) at += s_count[x]; count += s_count[x]; }
+                count = __builtin_amdgcn_readfirstlane(count);
+                u32 seen = 0;
+                for (int i = 0; i < 2 * WPT; ++i) {
+                    u32 rows = bits[0];
+#pragma unroll
+                    for (int x = 1; x < WPT; ++x) rows = i >> 1 == x ? bits[x] : rows;
+                    rows = i & 1 ? rows >> 16 : rows & 0xffffu;
+                    if (!rows) continue;
+                    const int off = tid * WPT * 2 + i, j = w0 + off, pj = j / per;
+                    int pg = pj < np ? a.indices[p0 + pj] : -1;
+                    if (pg < 0 || pg >= a.n_pages) { pg = 0; rows = 0; }      // (nobody's: page 0 is read and masked)
+                    list[at++] = make_uint2((u32)off << 16 | rows, (u32)pg * 2 * a.page_size + (u32)(j - pj * per) * a.block);
+                    seen |= rows;
+                }
+                if (seen) atomicOr(&s_seen, (int)seen);
+                __syncthreads();
                 const int units = ((count << sub_shift) + 1) / 2;
-                const int u0 = ONE ? (int)((long)units * split / a.splits) : 0, u1 = ONE ? (int)((long)units * (split + 1) / a.splits) : units;
-                for (int u = u0 + wave; u < u1; u += W) {
-                    // two tiles of 16 tokens
-                    uint4 k[2][KS];
-                    u32 v[2][4][CPL / 2];
-                    int tok[2];
-                    u32 rows[2];
+                auto load = [&](AttnUnit<D>& u, int at_unit) {
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
-                        const int sub = 2 * u + x, e = min(sub >> sub_shift, count - 1), part = sub & ((1 << sub_shift) - 1);
-                        const int2 ent = list[e];
-                        const int j = ONE ? ent.x : w0 + (int)((u32)ent.x >> 16);
-                        rows[x] = (sub >> sub_shift) < count ? (ONE ? 1u : (u32)ent.x & 0xffffu) : 0u;      // (the odd last tile of blocks of 16: nobody's)
-                        tok[x] = j * a.block + 16 * part;
-                        const bf16_t* const kb = a.kv + ((size_t)ent.y * 2 * a.page_size + (size_t)(j % per) * a.block + 16 * part) * row_el + (size_t)h * D;
-                        const bf16_t* const vb = kb + (size_t)a.page_size * row_el;
-#pragma unroll
-                        for (int s = 0; s < KS; ++s) k[x][s] = *reinterpret_cast<const uint4*>(kb + (size_t)c * row_el + 32 * s + 8 * g);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const bf16_t* const src = vb + (size_t)(4 * g + i) * row_el + CPL * c;
-                            if constexpr (CPL == 8) {
-                                const uint4 t = *reinterpret_cast<const uint4*>(src);
-                                v[x][i][0] = t.x; v[x][i][1] = t.y; v[x][i][2] = t.z; v[x][i][3] = t.w;
-                            } else {
-                                const uint2 t = *reinterpret_cast<const uint2*>(src);
-                                v[x][i][0] = t.x; v[x][i][1] = t.y;
-                            }
-                        }
+                        const int sub = 2 * at_unit + x, e = sub >> sub_shift, part = 16 * (sub & ((1 << sub_shift) - 1));
+                        const uint2 ent = list[min(e, count - 1)];
+                        const u32 word = __builtin_amdgcn_readfirstlane(ent.x), place = __builtin_amdgcn_readfirstlane(ent.y);      // (scalars, as above)
+                        u.rows[x] = e < count ? word & 0xffffu : 0u; // (the odd last tile of blocks of 16: nobody's)
+                        u.tok[x] = (w0 + (int)(word >> 16)) * a.block + part;
+                        u.f.load(x, kv, place + part, row_el, v_el, c, g);
                     }
-                    float p[8];
+                };
+                auto work = [&](AttnUnit<D>& u, auto is_careful) {
+                    constexpr bool CAREFUL = decltype(is_careful)::value;
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        f32x4 s4 = {0, 0, 0, 0};
-#pragma unroll
-                        for (int s = 0; s < KS; ++s) s4 = mma32<F16>(k[x][s], q[s], s4);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) p[4 * x + i] = s4[i] * a.scale2;
-                        const bool whole = (ONE ? rows[x] != 0 : rows[x] == all_rows) && tok[x] + 16 <= n_least;
-                        if (!whole) {
-                            const bool mine = ONE ? rows[x] != 0 : (rows[x] >> rc & 1) != 0;
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) p[4 * x + i] = mine && tok[x] + 4 * g + i < own ? p[4 * x + i] : -inf;
-                        }
-                        // (wave-uniform) V that nobody, or not the careful row, may see
-                        const bool none = rows[x] == 0 || (careful >= 0 && !ONE && !(rows[x] >> careful & 1));
-                        if (none || tok[x] + 16 > v_len) {
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const bool drop = none || tok[x] + 4 * g + i >= v_len;
-#pragma unroll
-                                for (int w = 0; w < CPL / 2; ++w) v[x][i][w] = drop ? 0u : v[x][i][w];
-                            }
-                        }
+                    for (int x = 0; x < 2; ++x) {                    // V that nobody, or not the careful row, may see
+                        const bool none = u.rows[x] == 0 || (CAREFUL && !(u.rows[x] >> careful & 1));
+                        if (none || u.tok[x] + 16 > v_len) u.f.drop_v(x, none ? 0 : v_len - u.tok[x], g);
                     }
-                    float top = fmaxf(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])), fmaxf(fmaxf(p[4], p[5]), fmaxf(p[6], p[7])));
-                    top = xor_max<32>(xor_max<16>(top));
-                    if (__ballot(top > m)) {
-                        const float now = fmaxf(m, top), keep = __builtin_amdgcn_exp2f(m - (now == -inf ? 0.0f : now));
-                        m = now;
-                        l *= keep;
+                    uint4 vt[1][CPL];
 #pragma unroll
-                        for (int t = 0; t < CPL; ++t) o[t] *= keep;
+                    for (int t = 0; t < CPL; ++t) vt[0][t] = u.f.vt(0, t);
+#pragma unroll
+                    for (int n = 0; n < NC; ++n) {
+                        if (NC > 1 && !((u.rows[0] | u.rows[1]) >> (n * rpt) & ((1u << rpt) - 1))) continue;      // no row of this tile lists these tokens
+                        int sees[2];
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) sees[x] = u.rows[x] >> (n * rpt + rc) & 1 ? own[n] - u.tok[x] - 4 * g : 0;
+                        attend_tiles<F16, D, 2, CAREFUL>(u.f, vt, q[n], sees, a.scale2, m[n], l[n], o[n]);
                     }
-                    const float base = m == -inf ? 0.0f : m;
-                    float part = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) { p[i] = __builtin_amdgcn_exp2f(p[i] - base); part += p[i]; }
-                    l += part;
-                    float hi[8];
-                    u32 ph[4], pl[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        ph[i] = pack2<F16>(p[2 * i], p[2 * i + 1]);
-                        hi[2 * i] = elem_f<F16>((bf16_t)ph[i]); hi[2 * i + 1] = elem_f<F16>((bf16_t)(ph[i] >> 16));
-                        pl[i] = pack2<F16>(p[2 * i] - hi[2 * i], p[2 * i + 1] - hi[2 * i + 1]);
+                };
+                auto go = [&](auto is_careful) {
+                    AttnUnit<D> f[2];
+                    load(f[0], wave);
+                    for (int u = wave; u < units; u += 2 * W) {      // (behind the last: asked for once more and not used)
+                        load(f[1], min(u + W, units - 1));
+                        work(f[0], is_careful);
+                        if (u + W >= units) break;
+                        load(f[0], min(u + 2 * W, units - 1));
+                        work(f[1], is_careful);
                     }
-                    const uint4 bh = make_uint4(ph[0], ph[1], ph[2], ph[3]), bl = make_uint4(pl[0], pl[1], pl[2], pl[3]);
-#pragma unroll
-                    for (int t = 0; t < CPL; ++t) {
-                        constexpr u32 LO = 0x05040100u, HI = 0x07060302u;
-                        u32 w[4];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_perm(v[i >> 1][2 * (i & 1) + 1][t >> 1], v[i >> 1][2 * (i & 1)][t >> 1], t & 1 ? HI : LO);
-                        if (careful < 0) {
-                            const uint4 av = make_uint4(w[0], w[1], w[2], w[3]);
-                            o[t] = mma32<F16>(av, bh, o[t]);
-                            o[t] = mma32<F16>(av, bl, o[t]);
-                        } else {
-                            u32 odd[4], ps[4];
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const u32 nf = halves_not_finite<F16>(w[i]);
-                                odd[i] = w[i] & nf;
-                                w[i] &= ~nf;
-                                // the weight as one term that is not zero where the weight is not
-                                const u32 tiny = (p[2 * i] > 0.0f && !(ph[i] & 0xffffu) ? 1u : 0u) | (p[2 * i + 1] > 0.0f && !(ph[i] >> 16) ? 0x10000u : 0u);
-                                ps[i] = ph[i] | tiny;
-                            }
-                            const uint4 av = make_uint4(w[0], w[1], w[2], w[3]);
-                            o[t] = mma32<F16>(av, bh, o[t]);
-                            o[t] = mma32<F16>(av, bl, o[t]);
-                            o[t] = mma32<F16>(make_uint4(odd[0], odd[1], odd[2], odd[3]), make_uint4(ps[0], ps[1], ps[2], ps[3]), o[t]);
-                        }
-                    }
+                };
+                if (wave < units) {
+                    if (careful < 0) go(std::false_type{});
+                    else go(std::true_type{});
                 }
-                if constexpr (!ONE) {
-                    __syncthreads();                                 // (the list has been read)
-                    w0 = s_next == 0x7fffffff ? -1 : s_next;
-                    __syncthreads();
-                }
+                __syncthreads();                                     // (the list has been read)
+                w0 = __builtin_amdgcn_readfirstlane(s_next);
+                if (w0 == 0x7fffffff) w0 = -1;
+                __syncthreads();
             }
-            // the waves' shares of each column meet
-            __syncthreads();
-            l = xor_add<32>(xor_add<16>(l));
-            if (c < a.cols) {
-                float* const dst = s_o + (wave * a.cols + c) * OS + 4 * g * CPL;
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int t = 0; t < CPL; t += 4) *reinterpret_cast<float4*>(dst + i * CPL + t) = make_float4(o[t][i], o[t + 1][i], o[t + 2][i], o[t + 3][i]);
-                if (g == 0) { s_ml[(wave * a.cols + c) * 2] = m; s_ml[(wave * a.cols + c) * 2 + 1] = l; }
-            }
-            __syncthreads();
+            // the waves' shares of each column meet, a tile of columns at a time
             bool bad = false;
-            for (int it = tid; it < a.cols * (D / 8); it += 64 * W) {
-                const int cc = it / (D / 8), d = it % (D / 8) * 8, r = ONE ? 0 : cc / gh, hh = ONE ? cc : cc % gh;
-                if (ONE ? cc >= gh : r < ra || r >= rb) continue;
-                if (careful >= 0 && r != careful) continue;
-                float mm = -inf, sum = 0.0f, acc[8] = {};
-                for (int w = 0; w < W; ++w) mm = fmaxf(mm, s_ml[(w * a.cols + cc) * 2]);
-                const float base = mm == -inf ? 0.0f : mm;
-                for (int w = 0; w < W; ++w) {
-                    const float f = __builtin_amdgcn_exp2f(s_ml[(w * a.cols + cc) * 2] - base);
-                    sum = __fmaf_rn(f, s_ml[(w * a.cols + cc) * 2 + 1], sum);
+            const int seen_rows = s_seen;
 #pragma unroll
-                    for (int x = 0; x < 8; ++x) acc[x] = __fmaf_rn(f, s_o[(w * a.cols + cc) * OS + d + x], acc[x]);
+            for (int n = 0; n < NC; ++n) {
+                if (n) __syncthreads();
+                put_columns<D>(s_o, s_ml, wave, 16, c, g, m[n], l[n], o[n]);
+                __syncthreads();
+                for (int it = tid; it < rpt * G * (D / 4); it += 64 * W) {
+                    const int cc = it / (D / 4), d = it % (D / 4) * 4, r = n * rpt + cc / G;
+                    if (r < ra || r >= rb || (careful >= 0 && r != careful)) continue;
+                    float top, sum, acc[4];
+                    bad |= !merge_columns<D, W>(s_o, s_ml, 16, cc, d, top, sum, acc);
+                    store_columns<F16>(a.out + ((size_t)(i0 + r) * a.Hq + h * G + cc % G) * D + d, a.out_al, (seen_rows >> r & 1) != 0, sum, acc);
                 }
-                bad |= !(fabsf(sum) < inf);
-#pragma unroll
-                for (int x = 0; x < 8; ++x) bad |= !(fabsf(acc[x]) < inf);
-                const size_t row = (size_t)(i0 + r) * a.Hq + h * G + h0 + hh;
-                if (ONE && a.splits > 1) {
-                    float* const dst = a.part_o + (row * a.splits + split) * D + d;
-                    *reinterpret_cast<float4*>(dst) = make_float4(acc[0], acc[1], acc[2], acc[3]);
-                    *reinterpret_cast<float4*>(dst + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
-                    if (d == 0) *reinterpret_cast<float2*>(a.part_ml + (row * a.splits + split) * 2) = make_float2(mm, s_seen ? sum : -1.0f);      // (-1: the row lists nothing)
-                    continue;
-                }
-                const bool seen = (s_seen >> r & 1) != 0;            // a row that lists nothing is zero
-                u32 w[4];
-#pragma unroll
-                for (int x = 0; x < 4; ++x) w[x] = seen ? pack2<F16>(acc[2 * x] / sum, acc[2 * x + 1] / sum) : 0u;
-                bf16_t* const dst = a.out + row * D + d;
-                if (a.out_al) *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
-                else
-#pragma unroll
-                    for (int x = 0; x < 8; ++x) dst[x] = (bf16_t)(w[x / 2] >> (16 * (x & 1)));
             }
-            const int again = __syncthreads_or(bad);
+            const int again = __builtin_amdgcn_readfirstlane(__syncthreads_or(bad));
             if (careful < 0 ? !again : careful + 1 >= rb) break;
             careful = careful < 0 ? ra : careful + 1;
         }
@@ -900,29 +1089,43 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 2 : 1) void k_block_attn(BlockAttn
     }
 }
 
-// the splits of a row and head: a wave each
+// the splits of a row and head, a block of threads each: four channels a thread, the splits over the groups of D / 4 threads
 template <int F16, int D>
 __global__ __launch_bounds__(256) void k_block_attn_merge(BlockAttnArgs a) {
-    const int at = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (at >= a.n_rows * a.Hq) return;
-    const int i = at / a.Hq, len = a.q_kvlen[i], req = a.q_req[i];
-    if (len <= 0 || req < 0 || req >= a.n_req) return;
+    constexpr int LPD = D / 4, GROUPS = 256 / LPD, MOST = 64 / GROUPS;
+    __shared__ float s_o[GROUPS][D + 4];
+    const int at = blockIdx.x, lane = threadIdx.x & 63, d = threadIdx.x % LPD * 4, grp = threadIdx.x / LPD;
     const float inf = __uint_as_float(0x7f800000u);
-    const float* const ml = a.part_ml + (size_t)at * a.splits * 2;
-    float m = lane < a.splits ? ml[2 * lane] : -inf, s = lane < a.splits ? ml[2 * lane + 1] : 0.0f;
-    const bool none = __shfl(s, 0, 64) == -1.0f;
-    float top = m;
-    for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-    const float f = __builtin_amdgcn_exp2f(m - (top == -inf ? 0.0f : top));
-    const float sum = butterfly<64>(lane < a.splits ? f * s : 0.0f);
-    float acc[D / 64] = {};
-    for (int z = 0; z < a.splits; ++z) {
-        const float fz = __shfl(f, z, 64);
+    const float2* const ml = reinterpret_cast<const float2*>(a.part_ml) + (size_t)at * a.splits;
+    float4 o[MOST];
 #pragma unroll
-        for (int x = 0; x < D / 64; ++x) acc[x] = __fmaf_rn(fz, a.part_o[((size_t)at * a.splits + z) * D + lane + 64 * x], acc[x]);
+    for (int i = 0; i < MOST; ++i) {
+        const int z = grp + i * GROUPS;
+        if (z < a.splits) o[i] = *reinterpret_cast<const float4*>(a.part_o + ((size_t)at * a.splits + z) * D + d);
     }
+    const float2 mine = lane < a.splits ? ml[lane] : make_float2(-inf, 0.0f);
+    const int i = at / a.Hq, len = min(a.q_kvlen[i], a.max_kvlen), req = a.q_req[i];
+    if (len <= 0 || req < 0 || req >= a.n_req) return;               // (the whole block: its parts were not written either)
+    float top = mine.x;
+    for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x, 64));
+    const float f = __builtin_amdgcn_exp2f(mine.x - (top == -inf ? 0.0f : top));
+    const float sum = butterfly<64>(lane < a.splits ? f * mine.y : 0.0f);
+    const bool none = __shfl(mine.y, 0, 64) == -1.0f;
+    float4 acc = make_float4(0, 0, 0, 0);
 #pragma unroll
-    for (int x = 0; x < D / 64; ++x) a.out[(size_t)at * D + lane + 64 * x] = none ? 0 : f_elem<F16>(acc[x] / sum);
+    for (int x = 0; x < MOST; ++x) {
+        const int z = grp + x * GROUPS;
+        const float w = __shfl(f, z & 63, 64);
+        if (z < a.splits) { acc.x = __fmaf_rn(w, o[x].x, acc.x); acc.y = __fmaf_rn(w, o[x].y, acc.y); acc.z = __fmaf_rn(w, o[x].z, acc.z); acc.w = __fmaf_rn(w, o[x].w, acc.w); }
+    }
+    *reinterpret_cast<float4*>(&s_o[grp][d]) = acc;
+    __syncthreads();
+    if (threadIdx.x < D) {
+        float all = 0.0f;
+#pragma unroll
+        for (int x = 0; x < GROUPS; ++x) all += s_o[x][threadIdx.x];
+        a.out[(size_t)at * D + threadIdx.x] = none ? 0 : f_elem<F16>(all / sum);
+    }
 }
 
 // ================================================================================================
@@ -1043,12 +1246,16 @@ static int check_attention(const vox_block_attention_args* a) {
     return VOX_OK;
 }
 // How a call's rows are laid out: rows a tile, and the parts that a row's list is split into.
-struct AttnShape { int per_tile, splits, head_tiles; };
+struct AttnShape { int tiles, per_tile, splits, head_tiles; };      // tiles of columns (0: a row a block of threads), rows a block, ..
 static AttnShape attn_shape(const vox_block_attention_args* a, int cus) {
     const vox_block_rows& r = a->rows;
     const int G = r.heads / a->cache.kv_heads;
-    AttnShape s{1, 1, (G + 15) / 16};
-    if (r.n_own > 0 && r.n_rows >= 2 * r.n_own && G <= 8) { s.per_tile = 16 / G; return s; }
+    AttnShape s{0, 1, 1, (G + 15) / 16};
+    if (r.n_own > 0 && r.n_rows >= 2 * r.n_own && G <= 16) {
+        s.tiles = G > 1 ? 2 : 1;
+        s.per_tile = s.tiles * (16 / G);
+        return s;
+    }
     const long tokens = (long)a->top * a->cache.block, blocks = (long)r.n_rows * a->cache.kv_heads * s.head_tiles;
     if (tokens > 1024) {
         long z = (2L * cus + blocks - 1) / blocks;
@@ -1076,21 +1283,22 @@ int vox_block_attention(vox_ctx* ctx, void* stream, const vox_block_attention_ar
         return vox_fail(VOX_ERR_INVALID, "block_attention: a workspace of %lld bytes on 16, %lld are wanted", (long long)(a->workspace ? a->workspace_bytes : 0), (long long)(rows * (c.head_dim + 2) * 4));
     const int64_t grid = (int64_t)((r.n_rows + z.per_tile - 1) / z.per_tile) * z.splits * z.head_tiles * c.kv_heads;
     if (grid > 0x7fffffff) return vox_fail(VOX_ERR_INVALID, "block_attention: %d rows of %d heads are more than a launch holds", r.n_rows, r.heads);
-    const bool one = z.per_tile == 1;
+    const bool one = z.tiles == 0;
     const int W = one ? 8 : 4, G = r.heads / c.kv_heads, cols = one && G < 16 ? G : 16;
     BlockAttnArgs s{(const bf16_t*)a->q, (const bf16_t*)c.kv, r.q_req, r.q_kvlen, r.kv_indptr, r.kv_indices, a->blocks, (bf16_t*)a->out, (float*)a->workspace,
                     (float*)a->workspace + rows * c.head_dim, (long)a->q_stride, a->scale * 1.44269504088896340736f, r.n_rows, r.n_req, r.heads, c.kv_heads, r.max_kvlen, c.n_pages,
-                    c.page_size, c.block, a->top, z.per_tile, z.splits, z.head_tiles, cols, ((size_t)a->q & 15) == 0 && a->q_stride % 8 == 0, ((size_t)a->out & 15) == 0};
-    const size_t merge = (size_t)W * cols * (c.head_dim + 4 + 2) * 4;
-    const size_t entries = (size_t)a->top * z.per_tile, lists = one ? entries * 8 : ATTN_WINDOW * 2 + (entries < ATTN_WINDOW ? entries : ATTN_WINDOW) * 8;
-    const size_t lds = merge > lists ? merge : lists;
-    const void* kern = one ? (c.dtype == VOX_DTYPE_F16 ? (c.head_dim == 128 ? (const void*)k_block_attn<1, 128, 8, true> : (const void*)k_block_attn<1, 64, 8, true>)
-                                                       : (c.head_dim == 128 ? (const void*)k_block_attn<0, 128, 8, true> : (const void*)k_block_attn<0, 64, 8, true>))
-                           : (c.dtype == VOX_DTYPE_F16 ? (c.head_dim == 128 ? (const void*)k_block_attn<1, 128, 4, false> : (const void*)k_block_attn<1, 64, 4, false>)
-                                                       : (c.head_dim == 128 ? (const void*)k_block_attn<0, 128, 4, false> : (const void*)k_block_attn<0, 64, 4, false>));
+                    c.page_size, c.block, a->top, z.splits, z.head_tiles, cols, ((size_t)a->q & 15) == 0 && a->q_stride % 8 == 0, ((size_t)a->out & 7) == 0};
+    const size_t merge = (size_t)W * cols * (c.head_dim + 4 + 2) * 4, entries = (size_t)a->top * z.per_tile;
+    const size_t lists = ATTN_WINDOW * 2 + (entries < ATTN_WINDOW ? entries : ATTN_WINDOW) * 8;
+    const bool big = a->top > 64;
+    const size_t lds = one ? merge + (big ? ((size_t)a->top * 8 + 15 & ~(size_t)15) : 0) : merge > lists ? merge : lists;
+#define ATTN_OF(KERN, ...) (c.dtype == VOX_DTYPE_F16 ? (c.head_dim == 128 ? (const void*)KERN<1, 128, __VA_ARGS__> : (const void*)KERN<1, 64, __VA_ARGS__>) \
+                                                     : (c.head_dim == 128 ? (const void*)KERN<0, 128, __VA_ARGS__> : (const void*)KERN<0, 64, __VA_ARGS__>))
+    const void* kern = one ? (big ? ATTN_OF(k_block_attn_row, 8, true) : ATTN_OF(k_block_attn_row, 8, false)) : z.tiles == 2 ? ATTN_OF(k_block_attn_rows, 4, 2) : ATTN_OF(k_block_attn_rows, 4, 1);
+#undef ATTN_OF
     VOX_TRY(launch(kern, dim3((unsigned)grid), 64 * W, lds, (hipStream_t)stream, s));
     if (z.splits == 1) return VOX_OK;
-    return launch(BY_TYPE_AND_DIM(k_block_attn_merge, c), dim3((unsigned)(((int64_t)r.n_rows * r.heads + 3) / 4)), 256, 0, (hipStream_t)stream, s);
+    return launch(BY_TYPE_AND_DIM(k_block_attn_merge, c), dim3((unsigned)(r.n_rows * r.heads)), 256, 0, (hipStream_t)stream, s);
 }
 
 }  // extern "C"

@@ -46,7 +46,8 @@ def test_block_select_refuses(wrong):
     assert b"block_select" in N.lib().vox_last_error()
 
 
-@pytest.mark.parametrize("wrong", BAD_CACHE + BAD_ROWS + [dict(out=0), dict(out=AT + 1), dict(top=-1), dict(top=1025)], ids=str)
+@pytest.mark.parametrize("wrong", BAD_CACHE + BAD_ROWS + [dict(out=0), dict(out=AT + 1), dict(top=-1), dict(top=1025), dict(scale=float("inf")),
+                                                               dict(scale=float("nan"))], ids=str)
 def test_block_attention_refuses(wrong):
     assert call("vox_block_attention", B._ATTEND, ATTEND, **wrong) == 1
     assert b"block_attention" in N.lib().vox_last_error()

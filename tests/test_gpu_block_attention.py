@@ -430,6 +430,20 @@ def test_attention_entries_that_do_not_count(dev):
     assert B.block_attention(q[:0], s.kv, plain[:0, None], s.q_req[:0], s.q_kvlen[:0], s.indptr, s.indices, block=16).shape == (0, 4, 64)
 
 
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 3.0, 1e-12])
+@pytest.mark.parametrize("q_lens", [[1, 1], [21, 6]])
+def test_attention_scales(dev, scale, q_lens):
+    """Negative, no and large scales; scores in rising order, so that the largest one moves again and again."""
+    from vox_serve_amd import block_attention as B
+    s = Paged(dev, torch.bfloat16, 2, 64, 32, [400, 90], q_lens, seed=3)
+    for r, pages in enumerate(s.pages):
+        for j, p in enumerate(pages):
+            s.kv[p, 0] *= 0.2 * (j + 1)
+    q = s.rnd(s.n, 8, 64)
+    blocks = random_lists(s, 2, 16, 25, 4)
+    check_attend(s, q, B.block_attention(q, s.kv, blocks, *s.plan, block=16, scale=scale, n_req=2), blocks, 16, scale)
+
+
 def test_all_blocks_are_dense_attention(dev):
     from vox_serve_amd.flashinfer_utils import FlashInferPrefillWrapper
     hq, h, d, page, q_lens, kv_lens = 16, 8, 128, 32, [40, 1, 75], [140, 90, 75]

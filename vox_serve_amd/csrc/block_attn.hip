@@ -572,9 +572,9 @@ struct BlockAttnArgs {
     bf16_t* out;
     float *part_o, *part_ml;             // splits > 1: [row][head][split][D], [row][head][split][2]
     long q_stride;
-    float scale2;                        // scale log2 e
+    float scale2;                        // |scale| log2 e, a little above zero (a lower score is a larger one where the scale is negative: q changes its sign)
     int n_rows, n_req, Hq, Hkv, max_kvlen, n_pages, page_size, block, top;
-    int splits, head_tiles, cols, q_al, out_al;      // cols: columns of a wave in the merge's LDS
+    int splits, head_tiles, cols, q_al, out_al, negate;      // cols: columns of a wave in the merge's LDS
 };
 #define ATTN_CUS 256                     // of an MI355X
 #define ATTN_WINDOW 4096                 // blocks whose rows' bits lie in LDS at a time (rows of several: 8 KB)
@@ -610,14 +610,16 @@ struct AttnTiles {
     static constexpr int CPL = D / 16, KS = D / 32;
     uint4 k[T][KS];
     u32 v[T][4][CPL / 2];
+    // (a scalar base and 32 bits a lane: the lane's part of every address stays one register)
     __device__ __forceinline__ void load(int x, const bf16_t* kv, u32 at, size_t row_el, size_t v_el, int c, int g) {
-        const bf16_t* const kb = kv + (size_t)at * row_el;
-        const bf16_t* const vb = kb + v_el;
+        const char* const kb = reinterpret_cast<const char*>(kv + (size_t)at * row_el);
+        const char* const vb = kb + 2 * v_el;
+        const u32 ko = 2 * ((u32)c * (u32)row_el + 8 * g), vo = 2 * (4 * g * (u32)row_el + CPL * c);
 #pragma unroll
-        for (int s = 0; s < KS; ++s) k[x][s] = *reinterpret_cast<const uint4*>(kb + (size_t)c * row_el + 32 * s + 8 * g);
+        for (int s = 0; s < KS; ++s) k[x][s] = *reinterpret_cast<const uint4*>(kb + 64 * s + ko);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const bf16_t* const src = vb + (size_t)(4 * g + i) * row_el + CPL * c;
+            const char* const src = vb + 2 * i * row_el + vo;
             if constexpr (CPL == 8) {
                 const uint4 t = *reinterpret_cast<const uint4*>(src);
                 v[x][i][0] = t.x; v[x][i][1] = t.y; v[x][i][2] = t.z; v[x][i][3] = t.w;
@@ -644,41 +646,57 @@ struct AttnTiles {
     }
 };
 // A tile of columns against T tiles of tokens.  sees[x]: how many of the lane's tokens 4 g, 4 g + 1, .. of tile x its column sees (any number: 4 and more are all).
-// CAREFUL: V that is not finite meets the weight as one term.
+// m: the exponent's base, in powers of two.  It need not be the maximum, only near enough that no weight passes 2^8: a lane looks at its own scores alone, and the
+// column's lanes meet only when one of them is that far above (the first time, and a few times more).  A tile is masked as a whole, by the base, unless the
+// column's last token lies in it.  What was a third more vector instructions a tile is the same to fp32 rounding.  CAREFUL: every score is masked, and
+// V that is not finite meets the weight as one term.
+#define ATTN_AHEAD 8.0f
+__device__ __forceinline__ float vmax(float x, float y) {            // (fmaxf of values that are no signalling NaN: without the two instructions that would quiet them)
+    float r;
+    asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(x), "v"(y));
+    return r;
+}
 template <int F16, int D, int T, bool CAREFUL>
 __device__ __forceinline__ void attend_tiles(const AttnTiles<D, T>& f, const uint4 (&vt)[T / 2][D / 16], const uint4 (&q)[D / 32], const int (&sees)[T], float scale2, float& m, float& l, f32x4 (&o)[D / 16]) {
     constexpr int CPL = D / 16, KS = D / 32;
     const float inf = __uint_as_float(0x7f800000u);
-    float p[4 * T];
+    f32x4 s4[T];
+    bool part = CAREFUL;
 #pragma unroll
     for (int x = 0; x < T; ++x) {
-        f32x4 s4 = {0, 0, 0, 0};
+        s4[x] = f32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int s = 0; s < KS; ++s) s4 = mma32<F16>(f.k[x][s], q[s], s4);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) p[4 * x + i] = i < sees[x] ? s4[i] * scale2 : -inf;
+        for (int s = 0; s < KS; ++s) s4[x] = mma32<F16>(f.k[x][s], q[s], s4[x]);
+        part |= sees[x] > 0 && sees[x] < 4;
     }
-    float top = p[0];
+    if (__ballot(part)) {
 #pragma unroll
-    for (int i = 1; i < 4 * T; ++i) top = fmaxf(top, p[i]);
-    top = xor_max<32>(xor_max<16>(top));
-    if (__ballot(top > m)) {
-        const float now = fmaxf(m, top), keep = __builtin_amdgcn_exp2f(m - (now == -inf ? 0.0f : now));
+        for (int x = 0; x < T; ++x)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s4[x][i] = i < sees[x] ? s4[x][i] : -inf;
+    }
+    float top = -inf;
+#pragma unroll
+    for (int x = 0; x < T; ++x) top = vmax(top, sees[x] > 0 ? vmax(vmax(s4[x][0], s4[x][1]), vmax(s4[x][2], s4[x][3])) : -inf);
+    top *= scale2;
+    if (__ballot(top > m + ATTN_AHEAD)) {
+        const float now = vmax(m, xor_max<32>(xor_max<16>(top))), keep = __builtin_amdgcn_exp2f(m - (now == -inf ? 0.0f : now));
         m = now;
         l *= keep;
 #pragma unroll
         for (int t = 0; t < CPL; ++t) o[t] *= keep;
     }
-    const float base = m == -inf ? 0.0f : m;
-    float part[T];
+    const float base = m == -inf ? 0.0f : -m;
+    float p[4 * T], sum[T];
 #pragma unroll
     for (int x = 0; x < T; ++x) {
+        const float b = sees[x] > 0 ? base : -inf;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) p[4 * x + i] = __builtin_amdgcn_exp2f(p[4 * x + i] - base);
-        part[x] = (p[4 * x] + p[4 * x + 1]) + (p[4 * x + 2] + p[4 * x + 3]);
+        for (int i = 0; i < 4; ++i) p[4 * x + i] = __builtin_amdgcn_exp2f(__fmaf_rn(s4[x][i], scale2, b));
+        sum[x] = (p[4 * x] + p[4 * x + 1]) + (p[4 * x + 2] + p[4 * x + 3]);
     }
 #pragma unroll
-    for (int x = 0; x < T; ++x) l += part[x];
+    for (int x = 0; x < T; ++x) l += sum[x];
 #pragma unroll
     for (int y = 0; y < T / 2; ++y) {
         const float* const w = p + 8 * y;
@@ -760,7 +778,7 @@ __device__ __forceinline__ void store_columns(bf16_t* dst, int aligned, bool see
 }
 // the lane's part of a column's q
 template <int D>
-__device__ __forceinline__ void load_q(uint4 (&q)[D / 32], const bf16_t* src, int aligned, bool col) {
+__device__ __forceinline__ void load_q(uint4 (&q)[D / 32], const bf16_t* src, int aligned, bool col, int negate) {
     if (aligned) {
 #pragma unroll
         for (int s = 0; s < D / 32; ++s) q[s] = *reinterpret_cast<const uint4*>(src + 32 * s);
@@ -775,6 +793,10 @@ __device__ __forceinline__ void load_q(uint4 (&q)[D / 32], const bf16_t* src, in
     }
 #pragma unroll
     for (int s = 0; s < D / 32; ++s) q[s] = col ? q[s] : make_uint4(0, 0, 0, 0);
+    if (negate) {
+#pragma unroll
+        for (int s = 0; s < D / 32; ++s) q[s] = make_uint4(q[s].x ^ 0x80008000u, q[s].y ^ 0x80008000u, q[s].z ^ 0x80008000u, q[s].w ^ 0x80008000u);
+    }
 }
 
 // A row (and up to 16 of its heads of a kv head); its list split over `splits` blocks of threads.  A wave takes 64 tokens at a time, all of their K and V asked for at
@@ -796,7 +818,7 @@ __global__ __launch_bounds__(64 * W, 1) void k_block_attn_row(BlockAttnArgs a) {
     int n = a.q_kvlen[i];
     const int req = a.q_req[i], G = a.Hq / a.Hkv, h0 = ht * 16, gh = min(G - h0, 16);
     uint4 q[D / 32];
-    load_q<D>(q, a.q + (size_t)i * a.q_stride + (size_t)(h * G + h0 + (c < gh ? c : 0)) * D + 8 * g, a.q_al, c < gh);
+    load_q<D>(q, a.q + (size_t)i * a.q_stride + (size_t)(h * G + h0 + (c < gh ? c : 0)) * D + 8 * g, a.q_al, c < gh, a.negate);
     if (n <= 0 || req < 0 || req >= a.n_req || a.max_kvlen <= 0) return;
     n = min(n, a.max_kvlen);
     const int p0 = a.indptr[req], np = a.indptr[req + 1] - p0, per = a.page_size / a.block, have = (n - 1) / a.block + 1;
@@ -877,7 +899,7 @@ __global__ __launch_bounds__(64 * W, 1) void k_block_attn_row(BlockAttnArgs a) {
                 attend_tiles<F16, D, T, decltype(is_careful)::value>(f, vt, q, sees, a.scale2, m, l, o);
             }
         };
-        if (careful) go(std::true_type{});
+        if (__builtin_expect(careful, 0)) go(std::true_type{});
         else go(std::false_type{});
         put_columns<D>(s_o, s_ml, wave, a.cols, c, g, m, l, o);
         __syncthreads();
@@ -897,7 +919,7 @@ __global__ __launch_bounds__(64 * W, 1) void k_block_attn_row(BlockAttnArgs a) {
 }
 
 // NC tiles of 16 columns whose rows share a request's blocks.  The waves of a block share the list's tokens, 32 in turn, each keeps all columns, and they meet in LDS
-// at the end; the next 32 tokens are on their way while a wave works.
+// at the end.
 template <int D>
 struct AttnUnit {
     AttnTiles<D, 2> f;
@@ -905,7 +927,7 @@ struct AttnUnit {
     u32 rows[2];
 };
 template <int F16, int D, int W, int NC>
-__global__ __launch_bounds__(64 * W, 1) void k_block_attn_rows(BlockAttnArgs a) {
+__global__ __launch_bounds__(64 * W, 2) void k_block_attn_rows(BlockAttnArgs a) {
     constexpr int CPL = D / 16;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     __shared__ int s_len[16], s_req[16], s_count[W], s_next, s_seen;
@@ -931,7 +953,7 @@ __global__ __launch_bounds__(64 * W, 1) void k_block_attn_rows(BlockAttnArgs a) 
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
         const bool col = rc < rpt && n * rpt + rc < R;
-        load_q<D>(q[n], a.q + (size_t)(i0 + (col ? n * rpt + rc : 0)) * a.q_stride + (size_t)(h * G + (col ? hc : 0)) * D + 8 * g, a.q_al, col);
+        load_q<D>(q[n], a.q + (size_t)(i0 + (col ? n * rpt + rc : 0)) * a.q_stride + (size_t)(h * G + (col ? hc : 0)) * D + 8 * g, a.q_al, col, a.negate);
     }
     const int sub_shift = a.block == 16 ? 0 : a.block == 32 ? 1 : a.block == 64 ? 2 : 3, per = a.page_size / a.block;
     const size_t row_el = (size_t)a.Hkv * D, v_el = (size_t)a.page_size * row_el;      // elements between tokens, from K to V
@@ -999,18 +1021,24 @@ __global__ __launch_bounds__(64 * W, 1) void k_block_attn_rows(BlockAttnArgs a) 
                 int at = upto - mine, count = 0;
                 for (int x = 0; x < W; ++x) { if (x < wave) at += s_count[x]; count += s_count[x]; }
                 count = __builtin_amdgcn_readfirstlane(count);
-                u32 seen = 0;
-                for (int i = 0; i < 2 * WPT; ++i) {
+                for (int i = 0; mine && i < 2 * WPT; ++i) {
                     u32 rows = bits[0];
 #pragma unroll
                     for (int x = 1; x < WPT; ++x) rows = i >> 1 == x ? bits[x] : rows;
                     rows = i & 1 ? rows >> 16 : rows & 0xffffu;
                     if (!rows) continue;
-                    const int off = tid * WPT * 2 + i, j = w0 + off, pj = j / per;
+                    list[at++].x = (u32)(tid * WPT * 2 + i) << 16 | rows;
+                }
+                __syncthreads();
+                u32 seen = 0;
+                for (int e = tid; e < count; e += 64 * W) {          // their pages, a thread an entry
+                    const u32 word = list[e].x;
+                    const int j = w0 + (int)(word >> 16), pj = j / per;
                     int pg = pj < np ? a.indices[p0 + pj] : -1;
-                    if (pg < 0 || pg >= a.n_pages) { pg = 0; rows = 0; }      // (nobody's: page 0 is read and masked)
-                    list[at++] = make_uint2((u32)off << 16 | rows, (u32)pg * 2 * a.page_size + (u32)(j - pj * per) * a.block);
-                    seen |= rows;
+                    const bool ok = pg >= 0 && pg < a.n_pages;
+                    pg = ok ? pg : 0;                                // (nobody's: page 0 is read and masked)
+                    list[e] = make_uint2(ok ? word : word & 0xffff0000u, (u32)pg * 2 * a.page_size + (u32)(j - pj * per) * a.block);
+                    seen |= ok ? word & 0xffffu : 0u;
                 }
                 if (seen) atomicOr(&s_seen, (int)seen);
                 __syncthreads();
@@ -1046,18 +1074,14 @@ __global__ __launch_bounds__(64 * W, 1) void k_block_attn_rows(BlockAttnArgs a) 
                     }
                 };
                 auto go = [&](auto is_careful) {
-                    AttnUnit<D> f[2];
-                    load(f[0], wave);
-                    for (int u = wave; u < units; u += 2 * W) {      // (behind the last: asked for once more and not used)
-                        load(f[1], min(u + W, units - 1));
-                        work(f[0], is_careful);
-                        if (u + W >= units) break;
-                        load(f[0], min(u + 2 * W, units - 1));
-                        work(f[1], is_careful);
+                    for (int u = wave; u < units; u += W) {
+                        AttnUnit<D> f;
+                        load(f, u);
+                        work(f, is_careful);
                     }
                 };
                 if (wave < units) {
-                    if (careful < 0) go(std::false_type{});
+                    if (__builtin_expect(careful < 0, 1)) go(std::false_type{});
                     else go(std::true_type{});
                 }
                 __syncthreads();                                     // (the list has been read)
@@ -1283,11 +1307,13 @@ int vox_block_attention(vox_ctx* ctx, void* stream, const vox_block_attention_ar
         return vox_fail(VOX_ERR_INVALID, "block_attention: a workspace of %lld bytes on 16, %lld are wanted", (long long)(a->workspace ? a->workspace_bytes : 0), (long long)(rows * (c.head_dim + 2) * 4));
     const int64_t grid = (int64_t)((r.n_rows + z.per_tile - 1) / z.per_tile) * z.splits * z.head_tiles * c.kv_heads;
     if (grid > 0x7fffffff) return vox_fail(VOX_ERR_INVALID, "block_attention: %d rows of %d heads are more than a launch holds", r.n_rows, r.heads);
+    if (!(fabsf(a->scale) < 3e38f)) return vox_fail(VOX_ERR_INVALID, "block_attention: the scale is not finite");
     const bool one = z.tiles == 0;
+    const float scale2 = fabsf(a->scale) * 1.44269504088896340736f;
     const int W = one ? 8 : 4, G = r.heads / c.kv_heads, cols = one && G < 16 ? G : 16;
     BlockAttnArgs s{(const bf16_t*)a->q, (const bf16_t*)c.kv, r.q_req, r.q_kvlen, r.kv_indptr, r.kv_indices, a->blocks, (bf16_t*)a->out, (float*)a->workspace,
-                    (float*)a->workspace + rows * c.head_dim, (long)a->q_stride, a->scale * 1.44269504088896340736f, r.n_rows, r.n_req, r.heads, c.kv_heads, r.max_kvlen, c.n_pages,
-                    c.page_size, c.block, a->top, z.splits, z.head_tiles, cols, ((size_t)a->q & 15) == 0 && a->q_stride % 8 == 0, ((size_t)a->out & 7) == 0};
+                    (float*)a->workspace + rows * c.head_dim, (long)a->q_stride, scale2 > 1e-30f ? scale2 : 1e-30f, r.n_rows, r.n_req, r.heads, c.kv_heads, r.max_kvlen, c.n_pages,
+                    c.page_size, c.block, a->top, z.splits, z.head_tiles, cols, ((size_t)a->q & 15) == 0 && a->q_stride % 8 == 0, ((size_t)a->out & 7) == 0, a->scale < 0.0f};
     const size_t merge = (size_t)W * cols * (c.head_dim + 4 + 2) * 4, entries = (size_t)a->top * z.per_tile;
     const size_t lists = ATTN_WINDOW * 2 + (entries < ATTN_WINDOW ? entries : ATTN_WINDOW) * 8;
     const bool big = a->top > 64;

@@ -45,6 +45,13 @@ def _attend_room(*sizes):
     return max(n, 0)                    # (sizes that the call itself will refuse)
 
 
+@functools.lru_cache(maxsize=4096)
+def _select_room(*sizes):
+    rows, n_own, heads, kv_heads, dim, dtype, page, block, top, first, last, max_kvlen = sizes
+    n = N.lib().vox_block_select_workspace_bytes(_SELECT.pack(0, 16, 16, 1, page, block, kv_heads, dim, dtype, 16, 16, 16, 16, rows, 1, n_own, heads, max_kvlen, 0, 16, 16, 0, 0, 0, top, first, last))
+    return max(n, 0)
+
+
 def _workspace(n, device):
     """A buffer for one call.  Eagerly the allocator's stream order makes it safe to let go of behind the call; a call that a `graph_capture` records keeps
     its own for good, so that no two graphs, and no graph and eager call, ever share one (torch's own graphs keep theirs by their pool)."""
@@ -206,10 +213,13 @@ def select_blocks(q, bounds, steps, q_req, q_kvlen, kv_indptr, kv_indices, *, bl
     q = _heads(q, rows, d, q, "q")
     plan = _plan(q_req, q_kvlen, kv_indptr, kv_indices, rows, device)
     out = _out(out, (rows, h, top), torch.int32, device)
+    room = _select_room(rows, n_req, q.shape[1], h, d, _DTYPES[q.dtype], per * block, block, top, first, last, max_kvlen)
+    ws = _workspace(room, device) if room else None
     ctx, stream = _on(device)
     N.check(N.lib().vox_block_select(ctx, stream, _SELECT.pack(
         0, bounds.data_ptr(), steps.data_ptr(), n_pages, per * block, block, h, d, _DTYPES[q.dtype], plan[0].data_ptr(), plan[1].data_ptr(), plan[2].data_ptr(),
-        plan[3].data_ptr(), rows, plan[2].shape[0] - 1, n_req, q.shape[1], max_kvlen, 0, q.data_ptr(), out.data_ptr(), 0, 0, q.stride(0), top, first, last)))
+        plan[3].data_ptr(), rows, plan[2].shape[0] - 1, n_req, q.shape[1], max_kvlen, 0, q.data_ptr(), out.data_ptr(),
+        ws.data_ptr() if room else 0, room, q.stride(0), top, first, last)))
     return out
 
 

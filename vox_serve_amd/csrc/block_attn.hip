@@ -33,6 +33,8 @@ __device__ __forceinline__ float finite_abs(float x) {
     return a < __uint_as_float(0x7f800000u) ? a : 0.0f;             // NaN and infinities: 0
 }
 
+#define ATTN_CUS 256                     // of an MI355X
+
 static int check_cache(const char* who, const vox_block_cache& c, bool bounds) {
     if (!c.kv) return vox_fail(VOX_ERR_INVALID, "%s: no cache", who);
     if (c.n_pages <= 0 || c.page_size <= 0 || c.kv_heads <= 0 || c.kv_heads > 65535) return vox_fail(VOX_ERR_INVALID, "%s: %d pages of %d tokens, %d kv heads", who, c.n_pages, c.page_size, c.kv_heads);
@@ -284,7 +286,9 @@ struct SelectArgs {
     const int *q_req, *q_kvlen, *indptr, *indices;
     int* blocks;
     long q_stride;
-    int n_rows, n_req, Hq, Hkv, max_kvlen, n_pages, page_size, block, top, first, last, stride;
+    int n_rows, n_req, Hq, Hkv, max_kvlen, n_pages, page_size, block, top, first, last, stride, q_al, splits;
+    u32* keys;                           // splits > 1: [row][kv head][stride]
+    u32 per_magic;                       // j / per = umulhi(j, per_magic) for j < 2^16 (0: per is 1)
 };
 // order of the scores as unsigned numbers; 0 is below all of them
 __device__ __forceinline__ u32 score_key(float s) {
@@ -296,6 +300,21 @@ __device__ __forceinline__ int q_steps(float x, float inv) {
     return x == x ? (int)t : 0;
 }
 typedef int i32x4 __attribute__((ext_vector_type(4)));
+// f over all lanes of a wave, f commutative: partners by swaps and DPP moves (vox_device.h's xor_add), not by the LDS crossbar
+template <class F>
+__device__ __forceinline__ u32 wave_all(u32 x, F f) {
+    vox_u2 r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    x = f(r.x, r.y);
+    r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = f(r.x, r.y);
+    x = f(x, (u32)__builtin_amdgcn_update_dpp((int)x, (int)x, 0x128, 0xF, 0xF, false));      // lane ^ 8
+    int y = __builtin_amdgcn_update_dpp((int)x, (int)x, 0x104, 0xF, 0x5, false);             // lane ^ 4
+    y = __builtin_amdgcn_update_dpp(y, (int)x, 0x114, 0xF, 0xA, false);
+    x = f(x, (u32)y);
+    x = f(x, (u32)__builtin_amdgcn_update_dpp((int)x, (int)x, 0x4E, 0xF, 0xF, false));       // lane ^ 2
+    x = f(x, (u32)__builtin_amdgcn_update_dpp((int)x, (int)x, 0xB1, 0xF, 0xF, false));       // lane ^ 1
+    return __builtin_amdgcn_readfirstlane(x);
+}
 
 // The scores of QT rows of one request (or of one row) and a kv head, then their choice.
 //   sum over heads and channels of max(a hi, a lo) = sum over channels of P hi + N lo, P = sum over heads of max(a, 0), N of min(a, 0): one product of 2 dim
@@ -318,49 +337,57 @@ __device__ __forceinline__ void choose(const u32* key, int lo, int cand, int nee
         least = min(least, in ? k[i] : 0xffffffffu);
         most = max(most, k[i]);
     }
-    int turn_ = 0;
-    auto total = [&](int x) {                                        // over the row's waves
-        if constexpr (W > 1) {
-            int* const r = red[turn_ & 1];
-            ++turn_;
-            if (lane == 0) r[wave] = x;
-            __syncthreads();
-            x = 0;
+    int turn = 0;
+    auto total3 = [&](int (&n)[3]) {                                 // over the row's waves: three sums in turn, the next one cleared before this one's barrier
+        if (lane < 3) atomicAdd(&red[turn][lane], lane == 0 ? n[0] : lane == 1 ? n[1] : n[2]);
+        const int next = turn == 2 ? 0 : turn + 1;
+        if (wave == 0 && lane < 3) red[next][lane] = 0;
+        __syncthreads();
 #pragma unroll
-            for (int w = 0; w < W; ++w) x += r[w];
-        }
-        return x;
+        for (int x = 0; x < 3; ++x) n[x] = __builtin_amdgcn_readfirstlane(red[turn][x]);
+        turn = next;
     };
     // the need-th largest key t lies in [a, b): at least need keys reach a, fewer reach b
-    for (int o = 1; o < 64; o <<= 1) {
-        least = min(least, (u32)__shfl_xor((int)least, o, 64));
-        most = max(most, (u32)__shfl_xor((int)most, o, 64));
-    }
+    least = wave_all(least, [](u32 x, u32 y) { return min(x, y); });
+    most = wave_all(most, [](u32 x, u32 y) { return max(x, y); });
     if constexpr (W > 1) {
-        u32* const r = reinterpret_cast<u32*>(red[2]);
-        u32* const s = reinterpret_cast<u32*>(red[3]);
+        u32* const r = reinterpret_cast<u32*>(red[3]);
+        u32* const s = reinterpret_cast<u32*>(red[4]);
         if (lane == 0) { r[wave] = least; s[wave] = most; }
+        if (wave == 0 && lane < 3) red[0][lane] = 0;
         __syncthreads();
 #pragma unroll
         for (int w = 0; w < W; ++w) { least = min(least, r[w]); most = max(most, s[w]); }
+        least = __builtin_amdgcn_readfirstlane(least);
+        most = __builtin_amdgcn_readfirstlane(most);
     }
-    least = __builtin_amdgcn_readfirstlane(least);
-    most = __builtin_amdgcn_readfirstlane(most);
-    u32 a = least, t = least, above = 0;
+    u32 a = least, t = least;
     unsigned long long b = (unsigned long long)most + 1;
-    bool exact = false;                                              // exactly `need` keys reach t: no ties to break
-    if (need == 0) { t = 0xffffffffu; exact = true; }
+    bool exact = need == 0;                                          // exactly `need` keys reach t: no ties to break
     while (!exact && b - a > 1) {
-        const u32 mid = a + (u32)((b - a) >> 1);
-        int n = 0;
+        if constexpr (W > 1) {
+            // three cuts a round: a round is its barrier, not its compares
+            const u32 len = (u32)((b - a) >> 2), cut[3] = {a + max(len, 1u), a + max(2 * len, 1u), a + max(3 * len, 1u)};
+            int n[3] = {0, 0, 0};
 #pragma unroll
-        for (int i = 0; i < KPL; ++i) n += (int)__popcll(__ballot(k[i] >= mid));      // (mid > least >= 0: lanes outside, 0, never reach it)
-        n = total(n);
-        if (n >= need) a = mid; else b = mid;
-        if (n == need) { exact = true; }
+            for (int i = 0; i < KPL; ++i)
+#pragma unroll
+                for (int x = 0; x < 3; ++x) n[x] += (int)__popcll(__ballot(k[i] >= cut[x]));
+            total3(n);
+            if (n[0] < need) b = cut[0];
+            else if (n[1] < need) { a = cut[0]; b = cut[1]; exact = n[0] == need; }
+            else if (n[2] < need) { a = cut[1]; b = cut[2]; exact = n[1] == need; }
+            else { a = cut[2]; exact = n[2] == need; }
+        } else {
+            const u32 mid = a + (u32)((b - a) >> 1);
+            int n = 0;
+#pragma unroll
+            for (int i = 0; i < KPL; ++i) n += (int)__popcll(__ballot(k[i] >= mid));      // (mid > least >= 0: lanes outside, 0, never reach it)
+            if (n >= need) a = mid; else b = mid;
+            exact = n == need;
+        }
         t = a;
     }
-    (void)above;
     // keys above t, and the oldest equal ones
     int gt = 0, eq = 0;
     if (need && !exact) {
@@ -408,45 +435,64 @@ __device__ __forceinline__ void choose(const u32* key, int lo, int cand, int nee
 }
 
 // QT > 1: tiles of QT rows, a wave a row in the choice; QT == 1: a row, all waves together
-template <int F16, int D, int QT, int W>
-__global__ __launch_bounds__(64 * W) void k_block_select(SelectArgs a) {
+// SPLIT (QT == 1): the scores alone, of one part of the row's blocks, into the workspace
+template <int F16, int D, int QT, int W, bool SPLIT>
+__global__ __launch_bounds__(64 * W, QT == 16 ? 4 : 2) void k_block_select(SelectArgs a) {
     constexpr int MT = (2 * QT + 15) / 16, KS = 2 * D / 64;          // tiles of 16 product rows, steps of 64 numbers
-    extern __shared__ __attribute__((aligned(16))) u32 keys[];       // [QT][a.stride]
+    extern __shared__ __attribute__((aligned(16))) u32 keys[];       // [QT][a.stride]; before: [QT][D], N and P of a channel in the halves
     __shared__ __attribute__((aligned(16))) int8_t s_a[MT * 16][2 * D];
-    __shared__ int s_len[QT], s_req[QT], red[4][16];
+    __shared__ int s_len[QT], s_req[QT], red[5][16];
+    __shared__ u32 s_amax[QT];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
-    const int h = blockIdx.x % a.Hkv, i0 = blockIdx.x / a.Hkv * QT, R = min(QT, a.n_rows - i0), G = a.Hq / a.Hkv, per = a.page_size / a.block;
+    const int h = blockIdx.x % a.Hkv, tile = blockIdx.x / a.Hkv, i0 = (SPLIT ? tile / a.splits : tile) * QT, R = min(QT, a.n_rows - i0), G = a.Hq / a.Hkv, per = a.page_size / a.block;
+    const int split = SPLIT ? tile % a.splits : 0;
     if (tid < QT) {
         int n = 0, r = -1;
         if (tid < R) {
             n = a.q_kvlen[i0 + tid];
             r = a.q_req[i0 + tid];
-            if (n <= 0 || r < 0 || r >= a.n_req) { n = 0; r = -1; }
+            if (n <= 0 || r < 0 || r >= a.n_req || a.max_kvlen <= 0) { n = 0; r = -1; }
             n = min(n, a.max_kvlen);
-            if (n == 0) r = -1;
         }
         s_len[tid] = n; s_req[tid] = r;
+        s_amax[tid] = 0;
     }
+    for (int x = tid; x < QT * D; x += 64 * W) keys[x] = 0;
     if constexpr (QT < 8) for (int x = tid; x < (MT * 16 - 2 * QT) * 2 * D / 4; x += 64 * W) reinterpret_cast<int*>(s_a[2 * QT])[x] = 0;
-    // P and N of the rows, a wave a row
-    for (int r = wave; r < R; r += W) {
-        const bf16_t* const q = a.q + (size_t)(i0 + r) * a.q_stride + (size_t)h * G * D;
+    // P and N of the rows: eight channels of a head a thread
+    const int chunks = G * D / 8;
+    auto piece = [&](int it) {
+        const bf16_t* const q = a.q + (size_t)(i0 + it / chunks) * a.q_stride + (size_t)h * G * D + it % chunks * 8;
+        if (a.q_al) return *reinterpret_cast<const uint4*>(q);
+        return make_uint4((u32)q[0] | ((u32)q[1] << 16), (u32)q[2] | ((u32)q[3] << 16), (u32)q[4] | ((u32)q[5] << 16), (u32)q[6] | ((u32)q[7] << 16));
+    };
+    const uint4 mine = tid < R * chunks ? piece(tid) : make_uint4(0, 0, 0, 0);
+    __syncthreads();
+    for (int it = tid; it < R * chunks; it += 64 * W) {
+        const uint4 x = it == tid ? mine : piece(it);
+        const u32 w[4] = {x.x, x.y, x.z, x.w};
         float amax = 0.0f;
-        for (int e = lane; e < G * D; e += 64) amax = fmaxf(amax, finite_abs(elem_f<F16>(q[e])));
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) amax = fmaxf(amax, __shfl_xor(amax, o, 64));
-        const float inv = 1.0f / step_of(amax);
+        for (int e = 0; e < 8; ++e) amax = fmaxf(amax, finite_abs(elem_f<F16>((bf16_t)(w[e / 2] >> (16 * (e % 2))))));
+        atomicMax(&s_amax[it / chunks], __float_as_uint(amax));
+    }
+    __syncthreads();
+    for (int it = tid; it < R * chunks; it += 64 * W) {
+        const uint4 x = it == tid ? mine : piece(it);
+        const u32 w[4] = {x.x, x.y, x.z, x.w};
+        const int r = it / chunks, d = it % chunks % (D / 8) * 8;
+        const float inv = 1.0f / step_of(__uint_as_float(s_amax[r]));
 #pragma unroll
-        for (int x = 0; x < D / 64; ++x) {
-            const int d = lane + 64 * x;
-            int p = 0, m = 0;
-            for (int e = 0; e < G; ++e) {
-                const int s = q_steps(elem_f<F16>(q[e * D + d]), inv);
-                p += max(s, 0); m += min(s, 0);
-            }
-            s_a[2 * r][d] = (int8_t)(p & 63); s_a[2 * r + 1][d] = (int8_t)(p >> 6);
-            s_a[2 * r][D + d] = (int8_t)(m & 63); s_a[2 * r + 1][D + d] = (int8_t)(m >> 6);
+        for (int e = 0; e < 8; ++e) {
+            const int s = q_steps(elem_f<F16>((bf16_t)(w[e / 2] >> (16 * (e % 2)))), inv);
+            atomicAdd(&keys[r * D + d + e], s >= 0 ? (u32)s : (u32)-s << 16);
         }
+    }
+    __syncthreads();
+    for (int x = tid; x < R * D; x += 64 * W) {
+        const int r = x / D, d = x % D, p = (int)(keys[x] & 0xffffu), m = -(int)(keys[x] >> 16);
+        s_a[2 * r][d] = (int8_t)(p & 63); s_a[2 * r + 1][d] = (int8_t)(p >> 6);
+        s_a[2 * r][D + d] = (int8_t)(m & 63); s_a[2 * r + 1][D + d] = (int8_t)(m >> 6);
     }
     __syncthreads();
     i32x4 av[MT][KS];
@@ -465,43 +511,42 @@ __global__ __launch_bounds__(64 * W) void k_block_select(SelectArgs a) {
         for (int r = ra; r < rb; ++r) n_most = max(n_most, s_len[r]);
         n_most = __builtin_amdgcn_readfirstlane(n_most);
         const int have = (n_most + a.block - 1) / a.block, j1 = have > a.top ? have - a.last : 0;      // blocks to score: [first, j1)
-        constexpr int U = 4;                                         // tiles of 16 blocks in flight
-        for (int j0 = a.first + wave * 16 * U; j0 < j1; j0 += W * 16 * U) {
-            int pg[U];
+        // 64 blocks a step: a lane looks up one of them, four tiles of 16 go through the product
+        u32* const dst0 = SPLIT ? a.keys + ((size_t)i0 * a.Hkv + h) * a.stride : keys;
+        for (int j0 = a.first + (split * W + wave) * 64; j0 < j1; j0 += (SPLIT ? a.splits : 1) * W * 64) {
+            const int j = j0 + lane, pj = a.per_magic ? (int)__umulhi((u32)j, a.per_magic) : j;
+            int pg = -1;
+            if (j < j1 && pj < np) pg = a.indices[p0 + pj];
+            const bool ok = pg >= 0 && pg < a.n_pages;
+            const size_t at = ok ? ((size_t)pg * a.Hkv + h) * per + (j - pj * per) : 0;
+            const float step = ok ? a.steps[at] : __uint_as_float(0x7fc00000u);      // (NaN: a block without a page)
+            const u32 at_lo = (u32)at, at_hi = (u32)(at >> 32);
+            i32x4 b[4][KS];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int j = j0 + 16 * u + c, pj = j / per;
-                pg[u] = j < j1 && pj < np ? a.indices[p0 + pj] : -1;
-            }
-            i32x4 b[U][KS];
-            float st[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int j = j0 + 16 * u + c;
-                const bool ok = pg[u] >= 0 && pg[u] < a.n_pages;
-                const size_t at = ok ? ((size_t)pg[u] * a.Hkv + h) * per + j % per : 0;
-                const i32x4* const src = reinterpret_cast<const i32x4*>(a.bounds + at * 2 * D) + g;
+            for (int u = 0; u < 4; ++u) {
+                const size_t from = (size_t)(u32)__shfl((int)at_lo, 16 * u + c, 64) | (size_t)(u32)__shfl((int)at_hi, 16 * u + c, 64) << 32;
+                const i32x4* const src = reinterpret_cast<const i32x4*>(a.bounds + from * 2 * D) + g;
 #pragma unroll
                 for (int s = 0; s < KS; ++s) b[u][s] = src[4 * s];
-                st[u] = a.steps[at];
-                pg[u] = ok;
             }
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int j = j0 + 16 * u + c;
+            for (int u = 0; u < 4; ++u) {
+                if (j0 + 16 * u >= j1) break;
+                const float st = __shfl(step, 16 * u + c, 64);
 #pragma unroll
                 for (int t = 0; t < MT; ++t) {
                     i32x4 s4 = {0, 0, 0, 0};
 #pragma unroll
                     for (int s = 0; s < KS; ++s) s4 = __builtin_amdgcn_mfma_i32_16x16x64_i8(av[t][s], b[u][s], s4, 0, 0, 0);
+                    u32* const dst = dst0 + (size_t)(8 * t + 2 * g) * a.stride + j0 + 16 * u + c;      // product rows 4 g + 2 x, + 1: query row 8 t + 2 g + x
+                    if (QT == 1 && g) continue;
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) {                    // product rows 4 g + 2 x, + 1: query row 8 t + 2 g + x
-                        const int r = 8 * t + 2 * g + x;
-                        if (j < j1 && r < QT) keys[(size_t)r * a.stride + j] = pg[u] ? score_key((float)(s4[2 * x] + 64 * s4[2 * x + 1]) * st[u]) : 0;
-                    }
+                    for (int x = 0; x < (QT == 1 ? 1 : 2); ++x)
+                        if (j0 + 16 * u + c < j1) dst[x * a.stride] = st == st ? score_key((float)(s4[2 * x] + 64 * s4[2 * x + 1]) * st) : 0;
                 }
             }
         }
+        if constexpr (SPLIT) return;
         __syncthreads();
         for (int r = ra + (QT > 1 ? wave : 0); r < rb; r += QT > 1 ? W : 1) {
             const int mine = (s_len[r] + a.block - 1) / a.block, cand = mine - a.first - a.last, need = a.top - a.first - a.last;
@@ -522,6 +567,29 @@ __global__ __launch_bounds__(64 * W) void k_block_select(SelectArgs a) {
         __syncthreads();
         ra = rb;
     }
+}
+
+// a row and kv head whose keys lie in the workspace
+template <int W>
+__global__ __launch_bounds__(64 * W) void k_block_choose(SelectArgs a) {
+    __shared__ int red[5][16];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i = blockIdx.x / a.Hkv, req = a.q_req[i];
+    int n = a.q_kvlen[i];
+    if (n <= 0 || req < 0 || req >= a.n_req || a.max_kvlen <= 0) return;
+    n = min(n, a.max_kvlen);
+    int* const out = a.blocks + (size_t)blockIdx.x * a.top;
+    const u32* const key = a.keys + (size_t)blockIdx.x * a.stride;
+    const int mine = (n - 1) / a.block + 1, cand = mine - a.first - a.last, need = a.top - a.first - a.last;
+    if (mine <= a.top) {
+        for (int j = tid; j < a.top; j += 64 * W) out[j] = j < mine ? j : -1;
+        return;
+    }
+#define CHOOSE(KPL) choose<KPL, W>(key, a.first, cand, need, a.first, a.last, mine, a.top, out, lane, wave, red)
+    if (cand <= 2 * 64 * W) CHOOSE(2);
+    else if (cand <= 4 * 64 * W) CHOOSE(4);
+    else if (cand <= 8 * 64 * W) CHOOSE(8);
+    else CHOOSE(32);
+#undef CHOOSE
 }
 
 // ================================================================================================
@@ -576,7 +644,6 @@ struct BlockAttnArgs {
     int n_rows, n_req, Hq, Hkv, max_kvlen, n_pages, page_size, block, top;
     int splits, head_tiles, cols, q_al, out_al, negate;      // cols: columns of a wave in the merge's LDS
 };
-#define ATTN_CUS 256                     // of an MI355X
 #define ATTN_WINDOW 4096                 // blocks whose rows' bits lie in LDS at a time (rows of several: 8 KB)
 
 // The entries of a row's list that count, 64 at a time, by one wave: f(j, counts) for every lane.  first: the lane's entry of the first 64.
@@ -1234,9 +1301,26 @@ static int check_select(const vox_block_select_args* a) {
     if (a->q_stride < 0) return vox_fail(VOX_ERR_INVALID, "block_select: a stride is negative");
     return VOX_OK;
 }
+// How a call's rows are laid out: rows a block of threads, waves, parts of a row's blocks (above 1: their scores go through the workspace).
+struct SelectShape { int qt, W, splits, stride; };
+static SelectShape select_shape(const vox_block_select_args* a) {
+    const vox_block_rows& r = a->rows;
+    const int most = (int)(((int64_t)r.max_kvlen + a->cache.block - 1) / a->cache.block);
+    // rows a tile: 16 while their keys take half a CU's LDS, 8 while they take most of it (4096 blocks), else (and for rows of different requests) one
+    const bool many = r.n_own > 0 && r.n_rows >= 2 * (int64_t)r.n_own;
+    SelectShape s{many && most <= 1024 ? 16 : many && most <= 4096 ? 8 : 1, 8, 1, 0};
+    s.stride = most + (s.qt > 1 ? SEL_PAD : 0);
+    if (s.qt > 1) return s;
+    s.W = most <= 512 ? 4 : 16;
+    // One CU draws some 35 bytes a ns: a row's bounds over several CUs where there are CUs left and a row has more than 512 blocks.
+    const int64_t pairs = (int64_t)r.n_rows * a->cache.kv_heads, z = pairs ? ATTN_CUS / pairs : 0, parts = (most + 255) / 256;
+    if (most > 512 && z >= 2) s.splits = (int)(z < parts ? z : parts);
+    return s;
+}
 int64_t vox_block_select_workspace_bytes(const vox_block_select_args* a) {
     if (check_select(a) != VOX_OK) return -1;
-    return 0;
+    const SelectShape s = select_shape(a);
+    return s.splits > 1 ? (int64_t)a->rows.n_rows * a->cache.kv_heads * s.stride * 4 : 0;
 }
 int vox_block_select(vox_ctx* ctx, void* stream, const vox_block_select_args* a) {
     (void)ctx;
@@ -1245,20 +1329,26 @@ int vox_block_select(vox_ctx* ctx, void* stream, const vox_block_select_args* a)
     const vox_block_rows& r = a->rows;
     if (r.n_rows == 0) return VOX_OK;
     if (!a->q || !a->blocks || (size_t)a->q & 1) return vox_fail(VOX_ERR_INVALID, "block_select: an operand is NULL, or does not lie on its type");
-    const int most = (r.max_kvlen + c.block - 1) / c.block;
-    // rows a tile: 16 while their keys take half a CU's LDS, 8 while they take most of it (4096 blocks), else (and for rows of different requests) one
-    const bool many = r.n_own > 0 && r.n_rows >= 2 * r.n_own;
-    const int qt = many && most <= 1024 ? 16 : many && most <= 4096 ? 8 : 1;
-    const int W = qt > 1 ? 8 : most <= 512 ? 4 : 16;
+    const SelectShape z = select_shape(a);
+    const int per = c.page_size / c.block, qt = z.qt, W = z.W;
+    const int64_t room = z.splits > 1 ? (int64_t)r.n_rows * c.kv_heads * z.stride * 4 : 0;
+    if (room && (!a->workspace || (size_t)a->workspace & 15 || a->workspace_bytes < room))
+        return vox_fail(VOX_ERR_INVALID, "block_select: a workspace of %lld bytes on 16, %lld are wanted", (long long)(a->workspace ? a->workspace_bytes : 0), (long long)room);
     SelectArgs s{(const bf16_t*)a->q, c.bounds, c.steps, r.q_req, r.q_kvlen, r.kv_indptr, r.kv_indices, a->blocks, (long)a->q_stride,
-                 r.n_rows, r.n_req, r.heads, c.kv_heads, r.max_kvlen, c.n_pages, c.page_size, c.block, a->top, a->first, a->last, most + (qt > 1 ? SEL_PAD : 0)};
-    const int64_t grid = (int64_t)((r.n_rows + qt - 1) / qt) * c.kv_heads;
+                 r.n_rows, r.n_req, r.heads, c.kv_heads, r.max_kvlen, c.n_pages, c.page_size, c.block, a->top, a->first, a->last, z.stride,
+                 ((size_t)a->q & 15) == 0 && a->q_stride % 8 == 0, z.splits, (u32*)a->workspace, per > 1 ? (u32)((1ull << 32) / per + 1) : 0u};
+    const int64_t grid = (int64_t)((r.n_rows + qt - 1) / qt) * c.kv_heads * z.splits;
     if (grid > 0x7fffffff) return vox_fail(VOX_ERR_INVALID, "block_select: %d rows of %d kv heads are more than a launch holds", r.n_rows, c.kv_heads);
-#define SELECT_OF(QT, W) (c.dtype == VOX_DTYPE_F16 ? (c.head_dim == 128 ? (const void*)k_block_select<1, 128, QT, W> : (const void*)k_block_select<1, 64, QT, W>) \
-                                                  : (c.head_dim == 128 ? (const void*)k_block_select<0, 128, QT, W> : (const void*)k_block_select<0, 64, QT, W>))
-    const void* kern = qt == 16 ? SELECT_OF(16, 8) : qt == 8 ? SELECT_OF(8, 8) : W == 4 ? SELECT_OF(1, 4) : SELECT_OF(1, 16);
+#define SELECT_OF(QT, W, SPLIT) (c.dtype == VOX_DTYPE_F16 ? (c.head_dim == 128 ? (const void*)k_block_select<1, 128, QT, W, SPLIT> : (const void*)k_block_select<1, 64, QT, W, SPLIT>) \
+                                                         : (c.head_dim == 128 ? (const void*)k_block_select<0, 128, QT, W, SPLIT> : (const void*)k_block_select<0, 64, QT, W, SPLIT>))
+    const int words = z.splits == 1 && z.stride > c.head_dim ? z.stride : c.head_dim;
+    if (z.splits > 1) {
+        VOX_TRY(launch(SELECT_OF(1, 4, true), dim3((unsigned)grid), 256, (size_t)words * 4, (hipStream_t)stream, s));
+        return launch((const void*)k_block_choose<16>, dim3((unsigned)(grid / z.splits)), 1024, 0, (hipStream_t)stream, s);
+    }
+    const void* kern = qt == 16 ? SELECT_OF(16, 8, false) : qt == 8 ? SELECT_OF(8, 8, false) : W == 4 ? SELECT_OF(1, 4, false) : SELECT_OF(1, 16, false);
 #undef SELECT_OF
-    return launch(kern, dim3((unsigned)grid), 64 * W, (size_t)qt * s.stride * 4, (hipStream_t)stream, s);
+    return launch(kern, dim3((unsigned)grid), 64 * W, (size_t)qt * words * 4, (hipStream_t)stream, s);
 }
 
 static int check_attention(const vox_block_attention_args* a) {

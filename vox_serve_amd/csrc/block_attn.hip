@@ -33,6 +33,29 @@ __device__ __forceinline__ float finite_abs(float x) {
     return a < __uint_as_float(0x7f800000u) ? a : 0.0f;             // NaN and infinities: 0
 }
 
+// lane ^ 16 and lane ^ 32, and f over a whole wave, f commutative: partners by swaps and DPP moves (vox_device.h's xor_add), not by the LDS crossbar
+template <int OFF>                       // 16 or 32
+__device__ __forceinline__ float xor_max(float s) {
+    vox_u2 r;
+    if constexpr (OFF == 32) r = __builtin_amdgcn_permlane32_swap(__float_as_uint(s), __float_as_uint(s), false, false);
+    else r = __builtin_amdgcn_permlane16_swap(__float_as_uint(s), __float_as_uint(s), false, false);
+    return fmaxf(__uint_as_float(r.x), __uint_as_float(r.y));
+}
+template <class F>
+__device__ __forceinline__ u32 wave_all(u32 x, F f) {
+    vox_u2 r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    x = f(r.x, r.y);
+    r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = f(r.x, r.y);
+    x = f(x, (u32)__builtin_amdgcn_update_dpp((int)x, (int)x, 0x128, 0xF, 0xF, false));      // lane ^ 8
+    int y = __builtin_amdgcn_update_dpp((int)x, (int)x, 0x104, 0xF, 0x5, false);             // lane ^ 4
+    y = __builtin_amdgcn_update_dpp(y, (int)x, 0x114, 0xF, 0xA, false);
+    x = f(x, (u32)y);
+    x = f(x, (u32)__builtin_amdgcn_update_dpp((int)x, (int)x, 0x4E, 0xF, 0xF, false));       // lane ^ 2
+    x = f(x, (u32)__builtin_amdgcn_update_dpp((int)x, (int)x, 0xB1, 0xF, 0xF, false));       // lane ^ 1
+    return __builtin_amdgcn_readfirstlane(x);
+}
+
 #define ATTN_CUS 256                     // of an MI355X
 
 static int check_cache(const char* who, const vox_block_cache& c, bool bounds) {
@@ -114,18 +137,17 @@ __global__ __launch_bounds__(256) void k_rope_append_any(RopeAppendArgs a) {
     dst[i1] = y;
 }
 
-// The bounds of one block, by one wave: D / 8 lanes hold a key, 512 / D keys at once.  key(l, t): channels 8 l .. 8 l + 7 of token t.
-template <int F16, int D, class K>
-__device__ __forceinline__ void block_bounds(int lane, int block, int8_t* bounds, float* step_out, K key) {
+// The bounds of one block, by one wave: D / 8 lanes hold a key, 512 / D keys at once, eight such loads in flight.  The first `count` keys are in the cache, one more may
+// come from own(l), channels 8 l .. 8 l + 7.  (A key twice changes no bound: places behind the last take the last.)
+template <int F16, int D, class O>
+__device__ __forceinline__ void block_bounds(int lane, const bf16_t* keys, size_t row_el, int count, bool more, int8_t* bounds, float* step_out, O own) {
     constexpr int LPT = D / 8, TPI = 64 / LPT;
     const float inf = __uint_as_float(0x7f800000u);
     const int l = lane % LPT;
     float hi[8], lo[8], amax = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) { hi[i] = -inf; lo[i] = inf; }
-#pragma unroll 4
-    for (int t = lane / LPT; t < block; t += TPI) {
-        const uint4 v = key(l, t);
+    auto take = [&](const uint4& v) {
         const u32 w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -134,16 +156,23 @@ __device__ __forceinline__ void block_bounds(int lane, int block, int8_t* bounds
             lo[i] = x < lo[i] ? x : lo[i];
             amax = fmaxf(amax, finite_abs(x));                      // (of all keys: infinities would stand in front of it in the bounds)
         }
+    };
+    const bf16_t* const from = keys + 8 * l;
+    for (int t0 = 0; t0 < count; t0 += 8 * TPI) {
+        uint4 v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[u] = *reinterpret_cast<const uint4*>(from + (size_t)min(t0 + u * TPI + lane / LPT, count - 1) * row_el);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) take(v[u]);
     }
+    if (more) take(own(l));
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-        for (int o = LPT; o < 64; o <<= 1) {
-            hi[i] = fmaxf(hi[i], __shfl_xor(hi[i], o, 64));
-            lo[i] = fminf(lo[i], __shfl_xor(lo[i], o, 64));
-        }
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) amax = fmaxf(amax, __shfl_xor(amax, o, 64));
+    for (int i = 0; i < 8; ++i) {
+        if constexpr (LPT == 8) { hi[i] = fmaxf(hi[i], __shfl_xor(hi[i], 8, 64)); lo[i] = fminf(lo[i], __shfl_xor(lo[i], 8, 64)); }
+        hi[i] = xor_max<32>(xor_max<16>(hi[i]));
+        lo[i] = -xor_max<32>(xor_max<16>(-lo[i]));
+    }
+    amax = __uint_as_float(wave_all(__float_as_uint(amax), [](u32 x, u32 y) { return max(x, y); }));
     const float step = step_of(amax), inv = 1.0f / step;
     if (lane < LPT) {
         u32 wh[2] = {0, 0}, wl[2] = {0, 0};
@@ -175,8 +204,7 @@ __global__ __launch_bounds__(256) void k_rope_append(RopeAppendArgs a) {
         const bf16_t* const base = a.kv + ((size_t)pg * 2 * a.page_size + slot + 1 - a.block) * a.Hkv * D + (size_t)h * D;
         const bf16_t* const own = a.k + n * a.k_stride + (size_t)h * D;
         const size_t to = ((size_t)pg * a.Hkv + h) * per + slot / a.block;
-        block_bounds<F16, D>(threadIdx.x & 63, a.block, a.bounds + to * 2 * D, a.steps + to, [&](int l, int t) {
-            if (t + 1 < a.block) return *reinterpret_cast<const uint4*>(base + (size_t)t * a.Hkv * D + 8 * l);
+        block_bounds<F16, D>(threadIdx.x & 63, base, (size_t)a.Hkv * D, a.block - 1, true, a.bounds + to * 2 * D, a.steps + to, [&](int l) {
             bf16_t e[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -260,19 +288,19 @@ struct BoundsArgs {
     const int *page, *slot;
     int n_rows, n_pages, page_size, block, Hkv;
 };
-// 64 rows and a kv head a block of threads; its waves share the rows that complete a block
+// 64 rows and a kv head a block of threads; its waves share the rows that complete a block (blocks of 16: one each)
 template <int F16, int D>
 __global__ __launch_bounds__(256) void k_block_bounds(BoundsArgs a) {
-    const int n0 = blockIdx.x * 64, h = blockIdx.y, lane = threadIdx.x & 63;
+    const int n = blockIdx.x * 64 + (threadIdx.x & 63), h = blockIdx.y, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int pg = -1, slot = 0;
-    const bool done = n0 + lane < a.n_rows && row_place(a.page, a.slot, n0 + lane, a.n_pages, a.page_size, pg, slot) && (slot + 1) % a.block == 0;
+    const bool done = n < a.n_rows && row_place(a.page, a.slot, n, a.n_pages, a.page_size, pg, slot) && (slot + 1) % a.block == 0;
     unsigned long long left = __ballot(done);
     for (int i = 0; left; ++i, left &= left - 1) {
-        if ((i & 3) != (int)(threadIdx.x >> 6)) continue;
-        const int from = __builtin_ctzll(left), p = __shfl(pg, from, 64), s = __shfl(slot, from, 64);
+        if ((i & 3) != wave) continue;
+        const int from = __builtin_ctzll(left), p = __builtin_amdgcn_readlane(pg, from), s = __builtin_amdgcn_readlane(slot, from);
         const bf16_t* const k = a.kv + ((size_t)p * 2 * a.page_size + s + 1 - a.block) * a.Hkv * D + (size_t)h * D;
         const size_t to = ((size_t)p * a.Hkv + h) * (a.page_size / a.block) + s / a.block;
-        block_bounds<F16, D>(lane, a.block, a.bounds + to * 2 * D, a.steps + to, [&](int l, int t) { return *reinterpret_cast<const uint4*>(k + (size_t)t * a.Hkv * D + 8 * l); });
+        block_bounds<F16, D>(lane, k, (size_t)a.Hkv * D, a.block, false, a.bounds + to * 2 * D, a.steps + to, [](int) { return make_uint4(0, 0, 0, 0); });
     }
 }
 
@@ -300,21 +328,6 @@ __device__ __forceinline__ int q_steps(float x, float inv) {
     return x == x ? (int)t : 0;
 }
 typedef int i32x4 __attribute__((ext_vector_type(4)));
-// f over all lanes of a wave, f commutative: partners by swaps and DPP moves (vox_device.h's xor_add), not by the LDS crossbar
-template <class F>
-__device__ __forceinline__ u32 wave_all(u32 x, F f) {
-    vox_u2 r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
-    x = f(r.x, r.y);
-    r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
-    x = f(r.x, r.y);
-    x = f(x, (u32)__builtin_amdgcn_update_dpp((int)x, (int)x, 0x128, 0xF, 0xF, false));      // lane ^ 8
-    int y = __builtin_amdgcn_update_dpp((int)x, (int)x, 0x104, 0xF, 0x5, false);             // lane ^ 4
-    y = __builtin_amdgcn_update_dpp(y, (int)x, 0x114, 0xF, 0xA, false);
-    x = f(x, (u32)y);
-    x = f(x, (u32)__builtin_amdgcn_update_dpp((int)x, (int)x, 0x4E, 0xF, 0xF, false));       // lane ^ 2
-    x = f(x, (u32)__builtin_amdgcn_update_dpp((int)x, (int)x, 0xB1, 0xF, 0xF, false));       // lane ^ 1
-    return __builtin_amdgcn_readfirstlane(x);
-}
 
 // The scores of QT rows of one request (or of one row) and a kv head, then their choice.
 //   sum over heads and channels of max(a hi, a lo) = sum over channels of P hi + N lo, P = sum over heads of max(a, 0), N of min(a, 0): one product of 2 dim
@@ -620,13 +633,6 @@ template <int F16>
 __device__ __forceinline__ u32 pack2(float lo, float hi) {
     if constexpr (F16) return (u32)f_elem<1>(lo) | ((u32)f_elem<1>(hi) << 16);
     else return pack_bf2(lo, hi);
-}
-template <int OFF>                       // 16 or 32
-__device__ __forceinline__ float xor_max(float s) {
-    vox_u2 r;
-    if constexpr (OFF == 32) r = __builtin_amdgcn_permlane32_swap(__float_as_uint(s), __float_as_uint(s), false, false);
-    else r = __builtin_amdgcn_permlane16_swap(__float_as_uint(s), __float_as_uint(s), false, false);
-    return fmaxf(__uint_as_float(r.x), __uint_as_float(r.y));
 }
 template <int F16>
 __device__ __forceinline__ u32 halves_not_finite(u32 w) {          // 0xffff where a half is an infinity or NaN

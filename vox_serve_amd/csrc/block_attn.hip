@@ -648,7 +648,7 @@ struct BlockAttnArgs {
     long q_stride;
     float scale2;                        // |scale| log2 e, a little above zero (a lower score is a larger one where the scale is negative: q changes its sign)
     int n_rows, n_req, Hq, Hkv, max_kvlen, n_pages, page_size, block, top;
-    int splits, head_tiles, cols, q_al, out_al, negate;      // cols: columns of a wave in the merge's LDS
+    int splits, head_tiles, cols, q_al, out_al, negate, k_at;      // k_at: byte of the waves' K in LDS (rows of several)      // cols: columns of a wave in the merge's LDS
 };
 #define ATTN_WINDOW 4096                 // blocks whose rows' bits lie in LDS at a time (rows of several: 8 KB)
 
@@ -677,22 +677,53 @@ __device__ __forceinline__ void row_entries(const int* list, int first, int top,
 }
 __device__ __forceinline__ int first_entry(const int* list, int top, int lane) { return lane < top ? list[lane] : -1; }
 
-// T tiles of 16 tokens as a wave's registers: K's rows, V's rows.  (Loads of one tile; at: its first token's place in the cache, [page][2][page_size] flat)
-template <int D, int T>
-struct AttnTiles {
-    static constexpr int CPL = D / 16, KS = D / 32;
-    uint4 k[T][KS];
-    u32 v[T][4][CPL / 2];
-    // (a scalar base and 32 bits a lane: the lane's part of every address stays one register)
-    __device__ __forceinline__ void load(int x, const bf16_t* kv, u32 at, size_t row_el, size_t v_el, int c, int g) {
-        const char* const kb = reinterpret_cast<const char*>(kv + (size_t)at * row_el);
-        const char* const vb = kb + 2 * v_el;
-        const u32 ko = 2 * ((u32)c * (u32)row_el + 8 * g), vo = 2 * (4 * g * (u32)row_el + CPL * c);
+// A tile is 16 tokens.  K comes to a wave's own part of LDS (memory to LDS, no registers, no barrier: the wave waits for its own) and from there to the product's lanes: a lane has
+// 16 bytes of a token, its neighbour the next token's, and loads of that pattern go through at 16 bytes a clock and CU, a quarter of what rows in order do (the chunk of
+// 1024 rows was held up by it 77 % of its time, a row's block of threads drew 35 bytes a ns).  Place in LDS: 16 bytes of a row at position chunk ^ swizzle(row), so
+// that 16 rows' same chunk lie on all banks.
+template <int D>
+__device__ __forceinline__ u32 tile_place(int row, int chunk) {      // byte of a tile's [16][D]
+    return D == 128 ? (u32)(row * 256 + ((chunk ^ row) << 4)) : (u32)(row * 128 + ((chunk ^ (row >> 1 & 7)) << 4));
+}
+template <int D>
+struct KLane {
+    static constexpr int PIECES = 32 * D / 1024;                     // wave loads a tile: 64 lanes of 16 bytes, 512 / D rows
+    u32 from, step, at;                                              // the lane's byte of a tile's first piece in memory and of each piece's further rows; its place of step 0
+    __device__ __forceinline__ KLane(int lane, u32 row_bytes) {
+        const int r = lane / (D / 8);
+        from = (u32)r * row_bytes;
+        step = lane % (D / 8);
+        at = tile_place<D>(lane & 15, lane >> 4);
+    }
+    // a tile's K on its way: base its first token's (scalar), to LDS byte `to` (scalar)
+    __device__ __forceinline__ void fetch(const char* base, u32 row_bytes, u32 to, int lane) const {
 #pragma unroll
-        for (int s = 0; s < KS; ++s) k[x][s] = *reinterpret_cast<const uint4*>(kb + 64 * s + ko);
+        for (int i = 0; i < PIECES; ++i) {
+            const int r = i * (512 / D) + lane / (D / 8);            // (what tile_place puts at this lane's position)
+            const u32 chunk = D == 128 ? step ^ (u32)r : step ^ (u32)(r >> 1 & 7);
+            lds_dma16(base + (size_t)(i * (512 / D)) * row_bytes, from + 16 * chunk, to + 1024 * i);
+        }
+    }
+    // scores of a tile of columns: step s of the lane's token at `at` ^ 64 s (the step's bits and the chunk's are apart)
+    template <int F16, class Q>
+    __device__ __forceinline__ f32x4 scores(const char* tile, Q q) const {
+        f32x4 s4 = {0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < D / 32; ++s) s4 = mma32<F16>(*reinterpret_cast<const uint4*>(tile + (at ^ 64 * s)), q(s), s4);
+        return s4;
+    }
+};
+__device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// T tiles' V as a wave's registers
+template <int D, int T>
+struct VTiles {
+    static constexpr int CPL = D / 16;
+    u32 v[T][4][CPL / 2];
+    // (a scalar base and 32 bits a lane)
+    __device__ __forceinline__ void load(int x, const char* vb, size_t row_bytes, u32 off) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const char* const src = vb + 2 * i * row_el + vo;
+            const char* const src = vb + i * row_bytes + off;
             if constexpr (CPL == 8) {
                 const uint4 t = *reinterpret_cast<const uint4*>(src);
                 v[x][i][0] = t.x; v[x][i][1] = t.y; v[x][i][2] = t.z; v[x][i][3] = t.w;
@@ -729,19 +760,13 @@ __device__ __forceinline__ float vmax(float x, float y) {            // (fmaxf o
     asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(x), "v"(y));
     return r;
 }
+// the weights of T tiles of scores, as two 16-bit terms (one: the first, not zero where the weight is not); o and l go to a new base if they have to
 template <int F16, int D, int T, bool CAREFUL>
-__device__ __forceinline__ void attend_tiles(const AttnTiles<D, T>& f, const uint4 (&vt)[T / 2][D / 16], const uint4 (&q)[D / 32], const int (&sees)[T], float scale2, float& m, float& l, f32x4 (&o)[D / 16]) {
-    constexpr int CPL = D / 16, KS = D / 32;
+__device__ __forceinline__ void weigh(f32x4 (&s4)[T], const int (&sees)[T], float scale2, float& m, float& l, f32x4 (&o)[D / 16], uint4 (&bh)[T / 2], uint4 (&bl)[T / 2], uint4 (&one)[T / 2]) {
     const float inf = __uint_as_float(0x7f800000u);
-    f32x4 s4[T];
     bool part = CAREFUL;
 #pragma unroll
-    for (int x = 0; x < T; ++x) {
-        s4[x] = f32x4{0, 0, 0, 0};
-#pragma unroll
-        for (int s = 0; s < KS; ++s) s4[x] = mma32<F16>(f.k[x][s], q[s], s4[x]);
-        part |= sees[x] > 0 && sees[x] < 4;
-    }
+    for (int x = 0; x < T; ++x) part |= sees[x] > 0 && sees[x] < 4;
     if (__ballot(part)) {
 #pragma unroll
         for (int x = 0; x < T; ++x)
@@ -757,7 +782,7 @@ __device__ __forceinline__ void attend_tiles(const AttnTiles<D, T>& f, const uin
         m = now;
         l *= keep;
 #pragma unroll
-        for (int t = 0; t < CPL; ++t) o[t] *= keep;
+        for (int t = 0; t < D / 16; ++t) o[t] *= keep;
     }
     const float base = m == -inf ? 0.0f : -m;
     float p[4 * T], sum[T];
@@ -779,26 +804,33 @@ __device__ __forceinline__ void attend_tiles(const AttnTiles<D, T>& f, const uin
             ph[i] = pack2<F16>(w[2 * i], w[2 * i + 1]);
             pl[i] = pack2<F16>(w[2 * i] - elem_f<F16>((bf16_t)ph[i]), w[2 * i + 1] - elem_f<F16>((bf16_t)(ph[i] >> 16)));
         }
-        const uint4 bh = make_uint4(ph[0], ph[1], ph[2], ph[3]), bl = make_uint4(pl[0], pl[1], pl[2], pl[3]);
+        bh[y] = make_uint4(ph[0], ph[1], ph[2], ph[3]);
+        bl[y] = make_uint4(pl[0], pl[1], pl[2], pl[3]);
         if constexpr (CAREFUL) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)                              // (one term, not zero where the weight is not)
-                ph[i] |= (w[2 * i] > 0.0f && !(ph[i] & 0xffffu) ? 1u : 0u) | (w[2 * i + 1] > 0.0f && !(ph[i] >> 16) ? 0x10000u : 0u);
-            const uint4 one = make_uint4(ph[0], ph[1], ph[2], ph[3]);
+            for (int i = 0; i < 4; ++i) ph[i] |= (w[2 * i] > 0.0f && !(ph[i] & 0xffffu) ? 1u : 0u) | (w[2 * i + 1] > 0.0f && !(ph[i] >> 16) ? 0x10000u : 0u);
+            one[y] = make_uint4(ph[0], ph[1], ph[2], ph[3]);
+        }
+    }
+}
+// o += V^T P^T over a pair of tiles; vt(t): channel CPL c + t of the lane's eight tokens
+template <int F16, int D, bool CAREFUL, class V>
+__device__ __forceinline__ void weighted(V vt, const uint4& bh, const uint4& bl, const uint4& one, f32x4 (&o)[D / 16]) {
+    if constexpr (CAREFUL) {
 #pragma unroll
-            for (int t = 0; t < CPL; ++t) {
-                const uint4 a = vt[y][t], odd = make_uint4(a.x & halves_not_finite<F16>(a.x), a.y & halves_not_finite<F16>(a.y), a.z & halves_not_finite<F16>(a.z), a.w & halves_not_finite<F16>(a.w));
-                const uint4 fine = make_uint4(a.x ^ odd.x, a.y ^ odd.y, a.z ^ odd.z, a.w ^ odd.w);
-                o[t] = mma32<F16>(odd, one, o[t]);
-                o[t] = mma32<F16>(fine, bh, o[t]);
-                o[t] = mma32<F16>(fine, bl, o[t]);
-            }
-        } else {
+        for (int t = 0; t < D / 16; ++t) {
+            const uint4 a = vt(t), odd = make_uint4(a.x & halves_not_finite<F16>(a.x), a.y & halves_not_finite<F16>(a.y), a.z & halves_not_finite<F16>(a.z), a.w & halves_not_finite<F16>(a.w));
+            const uint4 fine = make_uint4(a.x ^ odd.x, a.y ^ odd.y, a.z ^ odd.z, a.w ^ odd.w);
+            o[t] = mma32<F16>(odd, one, o[t]);
+            o[t] = mma32<F16>(fine, bh, o[t]);
+            o[t] = mma32<F16>(fine, bl, o[t]);
+        }
+    } else {
 #pragma unroll
-            for (int t = 0; t < CPL; ++t) {
-                o[t] = mma32<F16>(vt[y][t], bh, o[t]);
-                o[t] = mma32<F16>(vt[y][t], bl, o[t]);
-            }
+        for (int t = 0; t < D / 16; ++t) {
+            const uint4 a = vt(t);
+            o[t] = mma32<F16>(a, bh, o[t]);
+            o[t] = mma32<F16>(a, bl, o[t]);
         }
     }
 }
@@ -873,7 +905,7 @@ __device__ __forceinline__ void load_q(uint4 (&q)[D / 32], const bf16_t* src, in
 }
 
 // A row (and up to 16 of its heads of a kv head); its list split over `splits` blocks of threads.  A wave takes 64 tokens at a time, all of their K and V asked for at
-// once.  A list of up to 64 entries lies in each wave's lanes (LONG: in LDS).
+// once, K first.  A list of up to 64 entries lies in each wave's lanes (LONG: in LDS).
 template <int F16, int D, int W, bool LONG>
 __global__ __launch_bounds__(64 * W, 1) void k_block_attn_row(BlockAttnArgs a) {
     constexpr int CPL = D / 16, T = 4;
@@ -936,7 +968,10 @@ __global__ __launch_bounds__(64 * W, 1) void k_block_attn_row(BlockAttnArgs a) {
         });
         count = __builtin_amdgcn_readfirstlane(count);
     }
-    float* const s_o = reinterpret_cast<float*>(lds + (LONG ? (size_t)a.top * 8 + 15 & ~(size_t)15 : 0));
+    const u32 list_bytes = LONG ? (u32)(a.top * 8 + 15 & ~15) : 0, k_lds = list_bytes + wave * T * 32 * D, lds0 = (u32)(size_t)(__attribute__((address_space(3))) char*)lds;
+    const u32 row_bytes = 2 * (u32)row_el, v_off = 4 * g * row_bytes + 2 * CPL * c;
+    const KLane<D> kl(lane, row_bytes);
+    float* const s_o = reinterpret_cast<float*>(lds + list_bytes);   // (where K was)
     float2* const s_ml = reinterpret_cast<float2*>(s_o + W * a.cols * (D + 4));
     const int units = ((count << sub_shift) + T - 1) / T, u0 = (int)((long)units * split / a.splits), u1 = (int)((long)units * (split + 1) / a.splits);
 
@@ -946,34 +981,42 @@ __global__ __launch_bounds__(64 * W, 1) void k_block_attn_row(BlockAttnArgs a) {
 #pragma unroll
         for (int t = 0; t < CPL; ++t) o[t] = f32x4{0, 0, 0, 0};
         auto go = [&](auto is_careful) {
+            constexpr bool CAREFUL = decltype(is_careful)::value;
             for (int u = u0 + wave; u < u1; u += W) {
-                AttnTiles<D, T> f;
+                VTiles<D, T> f;
                 int sees[T], tok[T];
+                u32 place[T];
 #pragma unroll
                 for (int x = 0; x < T; ++x) {
                     const int sub = T * u + x, e = sub >> sub_shift, part = 16 * (sub & ((1 << sub_shift) - 1)), at = min(e, count - 1);
                     // (scalars: what a wave's branches go by, for a matrix instruction runs whatever the lanes' mask says)
-                    u32 block, place;
-                    if constexpr (LONG) { const uint2 ent = list[at]; block = __builtin_amdgcn_readfirstlane(ent.x); place = __builtin_amdgcn_readfirstlane(ent.y); }
-                    else { block = __builtin_amdgcn_readlane(e_block, at); place = __builtin_amdgcn_readlane(e_at, at); }
+                    u32 block;
+                    if constexpr (LONG) { const uint2 ent = list[at]; block = __builtin_amdgcn_readfirstlane(ent.x); place[x] = __builtin_amdgcn_readfirstlane(ent.y) + part; }
+                    else { block = __builtin_amdgcn_readlane(e_block, at); place[x] = __builtin_amdgcn_readlane(e_at, at) + part; }
                     tok[x] = e < count ? (int)block * a.block + part : n;             // (behind the list's end: nothing)
-                    f.load(x, kv, place + part, row_el, v_el, c, g);
+                    kl.fetch(reinterpret_cast<const char*>(kv + (size_t)place[x] * row_el), row_bytes, lds0 + k_lds + x * 32 * D, lane);
                 }
+#pragma unroll
+                for (int x = 0; x < T; ++x) f.load(x, reinterpret_cast<const char*>(kv + (size_t)place[x] * row_el + v_el), row_bytes, v_off);
+                asm volatile("s_waitcnt vmcnt(%0)" ::"n"(4 * T) : "memory");          // K is there (V, 4 T loads, came behind it)
+                f32x4 s4[T];
 #pragma unroll
                 for (int x = 0; x < T; ++x) {
+                    s4[x] = kl.template scores<F16>(lds + k_lds + x * 32 * D, [&](int s) { return q[s]; });
                     sees[x] = n - tok[x] - 4 * g;
-                    if (tok[x] + 16 > n) f.drop_v(x, n - tok[x], g);
                 }
-                uint4 vt[T / 2][CPL];
 #pragma unroll
-                for (int y = 0; y < T / 2; ++y)
+                for (int x = 0; x < T; ++x)
+                    if (tok[x] + 16 > n) f.drop_v(x, n - tok[x], g);
+                uint4 bh[T / 2], bl[T / 2], one[T / 2];
+                weigh<F16, D, T, CAREFUL>(s4, sees, a.scale2, m, l, o, bh, bl, one);
 #pragma unroll
-                    for (int t = 0; t < CPL; ++t) vt[y][t] = f.vt(y, t);
-                attend_tiles<F16, D, T, decltype(is_careful)::value>(f, vt, q, sees, a.scale2, m, l, o);
+                for (int y = 0; y < T / 2; ++y) weighted<F16, D, CAREFUL>([&](int t) { return f.vt(y, t); }, bh[y], bl[y], one[y], o);
             }
         };
         if (__builtin_expect(careful, 0)) go(std::true_type{});
         else go(std::false_type{});
+        __syncthreads();                                             // (everyone's K has been read)
         put_columns<D>(s_o, s_ml, wave, a.cols, c, g, m, l, o);
         __syncthreads();
         bool bad = false;
@@ -993,12 +1036,6 @@ __global__ __launch_bounds__(64 * W, 1) void k_block_attn_row(BlockAttnArgs a) {
 
 // NC tiles of 16 columns whose rows share a request's blocks.  The waves of a block share the list's tokens, 32 in turn, each keeps all columns, and they meet in LDS
 // at the end.
-template <int D>
-struct AttnUnit {
-    AttnTiles<D, 2> f;
-    int tok[2];
-    u32 rows[2];
-};
 template <int F16, int D, int W, int NC>
 __global__ __launch_bounds__(64 * W, 2) void k_block_attn_rows(BlockAttnArgs a) {
     constexpr int CPL = D / 16;
@@ -1031,9 +1068,11 @@ __global__ __launch_bounds__(64 * W, 2) void k_block_attn_rows(BlockAttnArgs a) 
     const int sub_shift = a.block == 16 ? 0 : a.block == 32 ? 1 : a.block == 64 ? 2 : 3, per = a.page_size / a.block;
     const size_t row_el = (size_t)a.Hkv * D, v_el = (size_t)a.page_size * row_el;      // elements between tokens, from K to V
     const bf16_t* const kv = a.kv + (size_t)h * D;
+    const u32 row_bytes = 2 * (u32)row_el, v_off = 4 * g * row_bytes + 2 * CPL * c, k_lds = a.k_at + wave * 128 * D, lds0 = (u32)(size_t)(__attribute__((address_space(3))) char*)lds;
+    const KLane<D> kl(lane, row_bytes);
     u32* const s_bits = reinterpret_cast<u32*>(lds);                 // two blocks' rows a word
     uint2* const list = reinterpret_cast<uint2*>(lds) + ATTN_WINDOW / 4;     // {block from the window's first << 16 | rows; its first token's place}
-    float* const s_o = reinterpret_cast<float*>(lds);                // after the loop
+    float* const s_o = reinterpret_cast<float*>(lds);                // after the loops (where list and K were)
     float2* const s_ml = reinterpret_cast<float2*>(s_o + W * 16 * (D + 4));
 
     for (int ra = 0; ra < R;) {
@@ -1115,43 +1154,58 @@ __global__ __launch_bounds__(64 * W, 2) void k_block_attn_rows(BlockAttnArgs a) 
                 }
                 if (seen) atomicOr(&s_seen, (int)seen);
                 __syncthreads();
-                const int units = ((count << sub_shift) + 1) / 2;
-                auto load = [&](AttnUnit<D>& u, int at_unit) {
+                const int tiles = count << sub_shift, units = (tiles + 1) / 2;
+                u32 place[2];
+                auto fetch = [&](int u, u32 to) {
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
-                        const int sub = 2 * at_unit + x, e = sub >> sub_shift, part = 16 * (sub & ((1 << sub_shift) - 1));
-                        const uint2 ent = list[min(e, count - 1)];
-                        const u32 word = __builtin_amdgcn_readfirstlane(ent.x), place = __builtin_amdgcn_readfirstlane(ent.y);      // (scalars, as above)
-                        u.rows[x] = e < count ? word & 0xffffu : 0u; // (the odd last tile of blocks of 16: nobody's)
-                        u.tok[x] = (w0 + (int)(word >> 16)) * a.block + part;
-                        u.f.load(x, kv, place + part, row_el, v_el, c, g);
-                    }
-                };
-                auto work = [&](AttnUnit<D>& u, auto is_careful) {
-                    constexpr bool CAREFUL = decltype(is_careful)::value;
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {                    // V that nobody, or not the careful row, may see
-                        const bool none = u.rows[x] == 0 || (CAREFUL && !(u.rows[x] >> careful & 1));
-                        if (none || u.tok[x] + 16 > v_len) u.f.drop_v(x, none ? 0 : v_len - u.tok[x], g);
-                    }
-                    uint4 vt[1][CPL];
-#pragma unroll
-                    for (int t = 0; t < CPL; ++t) vt[0][t] = u.f.vt(0, t);
-#pragma unroll
-                    for (int n = 0; n < NC; ++n) {
-                        if (NC > 1 && !((u.rows[0] | u.rows[1]) >> (n * rpt) & ((1u << rpt) - 1))) continue;      // no row of this tile lists these tokens
-                        int sees[2];
-#pragma unroll
-                        for (int x = 0; x < 2; ++x) sees[x] = u.rows[x] >> (n * rpt + rc) & 1 ? own[n] - u.tok[x] - 4 * g : 0;
-                        attend_tiles<F16, D, 2, CAREFUL>(u.f, vt, q[n], sees, a.scale2, m[n], l[n], o[n]);
+                        const int sub = min(2 * u + x, tiles - 1);
+                        place[x] = __builtin_amdgcn_readfirstlane(list[sub >> sub_shift].y) + 16 * (sub & ((1 << sub_shift) - 1));
+                        kl.fetch(reinterpret_cast<const char*>(kv + (size_t)place[x] * row_el), row_bytes, to + x * 32 * D, lane);
                     }
                 };
                 auto go = [&](auto is_careful) {
+                    constexpr bool CAREFUL = decltype(is_careful)::value;
+                    u32 buf = 0;                                     // the wave's two K buffers in turn
+                    fetch(wave, lds0 + k_lds);
                     for (int u = wave; u < units; u += W) {
-                        AttnUnit<D> f;
-                        load(f, u);
-                        work(f, is_careful);
+                        dma_wait();                                  // (V of the unit before has been used: only this K is on its way)
+                        VTiles<D, 2> f;
+                        u32 rows[2];
+                        int tok[2];
+                        const u32 here[2] = {place[0], place[1]};
+                        fetch(min(u + W, units - 1), lds0 + k_lds + (buf ^ 64 * D));      // (behind the last: asked for once more and not used)
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            const int sub = min(2 * u + x, tiles - 1), e = sub >> sub_shift;
+                            const u32 word = __builtin_amdgcn_readfirstlane(list[e].x);               // (scalars, as above)
+                            rows[x] = 2 * u + x < tiles ? word & 0xffffu : 0u;                        // (the odd last tile of blocks of 16: nobody's)
+                            tok[x] = (w0 + (int)(word >> 16)) * a.block + 16 * (sub & ((1 << sub_shift) - 1));
+                            f.load(x, reinterpret_cast<const char*>(kv + (size_t)here[x] * row_el + v_el), row_bytes, v_off);
+                        }
+                        f32x4 s4[NC][2];
+#pragma unroll
+                        for (int n = 0; n < NC; ++n)
+#pragma unroll
+                            for (int x = 0; x < 2; ++x) s4[n][x] = kl.template scores<F16>(lds + k_lds + buf + x * 32 * D, [&](int s) { return q[n][s]; });
+                        buf ^= 64 * D;
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {                // V that nobody, or not the careful row, may see
+                            const bool none = rows[x] == 0 || (CAREFUL && !(rows[x] >> careful & 1));
+                            if (none || tok[x] + 16 > v_len) f.drop_v(x, none ? 0 : v_len - tok[x], g);
+                        }
+#pragma unroll
+                        for (int n = 0; n < NC; ++n) {
+                            if (NC > 1 && !((rows[0] | rows[1]) >> (n * rpt) & ((1u << rpt) - 1))) continue;      // no row of this tile lists these tokens
+                            int sees[2];
+#pragma unroll
+                            for (int x = 0; x < 2; ++x) sees[x] = rows[x] >> (n * rpt + rc) & 1 ? own[n] - tok[x] - 4 * g : 0;
+                            uint4 bh[1], bl[1], one[1];
+                            weigh<F16, D, 2, CAREFUL>(s4[n], sees, a.scale2, m[n], l[n], o[n], bh, bl, one);
+                            weighted<F16, D, CAREFUL>([&](int t) { return f.vt(0, t); }, bh[0], bl[0], one[0], o[n]);
+                        }
                     }
+                    dma_wait();                                      // (nothing may land in LDS that is used anew)
                 };
                 if (wave < units) {
                     if (__builtin_expect(careful < 0, 1)) go(std::false_type{});
@@ -1407,13 +1461,13 @@ int vox_block_attention(vox_ctx* ctx, void* stream, const vox_block_attention_ar
     const bool one = z.tiles == 0;
     const float scale2 = fabsf(a->scale) * 1.44269504088896340736f;
     const int W = one ? 8 : 4, G = r.heads / c.kv_heads, cols = one && G < 16 ? G : 16;
+    const bool big = a->top > 64;
+    const size_t entries = (size_t)a->top * z.per_tile, merge = (size_t)W * cols * (c.head_dim + 4 + 2) * 4;
+    const size_t lists = one ? (big ? ((size_t)a->top * 8 + 15 & ~(size_t)15) : 0) : ATTN_WINDOW * 2 + ((entries < ATTN_WINDOW ? entries : ATTN_WINDOW) * 8 + 15 & ~(size_t)15);
+    const size_t keys = (size_t)W * 128 * c.head_dim, lds = one ? lists + (merge > keys ? merge : keys) : merge > lists + keys ? merge : lists + keys;
     BlockAttnArgs s{(const bf16_t*)a->q, (const bf16_t*)c.kv, r.q_req, r.q_kvlen, r.kv_indptr, r.kv_indices, a->blocks, (bf16_t*)a->out, (float*)a->workspace,
                     (float*)a->workspace + rows * c.head_dim, (long)a->q_stride, scale2 > 1e-30f ? scale2 : 1e-30f, r.n_rows, r.n_req, r.heads, c.kv_heads, r.max_kvlen, c.n_pages,
-                    c.page_size, c.block, a->top, z.splits, z.head_tiles, cols, ((size_t)a->q & 15) == 0 && a->q_stride % 8 == 0, ((size_t)a->out & 7) == 0, a->scale < 0.0f};
-    const size_t merge = (size_t)W * cols * (c.head_dim + 4 + 2) * 4, entries = (size_t)a->top * z.per_tile;
-    const size_t lists = ATTN_WINDOW * 2 + (entries < ATTN_WINDOW ? entries : ATTN_WINDOW) * 8;
-    const bool big = a->top > 64;
-    const size_t lds = one ? merge + (big ? ((size_t)a->top * 8 + 15 & ~(size_t)15) : 0) : merge > lists ? merge : lists;
+                    c.page_size, c.block, a->top, z.splits, z.head_tiles, cols, ((size_t)a->q & 15) == 0 && a->q_stride % 8 == 0, ((size_t)a->out & 7) == 0, a->scale < 0.0f, (int)lists};
 #define ATTN_OF(KERN, ...) (c.dtype == VOX_DTYPE_F16 ? (c.head_dim == 128 ? (const void*)KERN<1, 128, __VA_ARGS__> : (const void*)KERN<1, 64, __VA_ARGS__>) \
                                                      : (c.head_dim == 128 ? (const void*)KERN<0, 128, __VA_ARGS__> : (const void*)KERN<0, 64, __VA_ARGS__>))
     const void* kern = one ? (big ? ATTN_OF(k_block_attn_row, 8, true) : ATTN_OF(k_block_attn_row, 8, false)) : z.tiles == 2 ? ATTN_OF(k_block_attn_rows, 4, 2) : ATTN_OF(k_block_attn_rows, 4, 1);

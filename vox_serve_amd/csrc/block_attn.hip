@@ -56,6 +56,13 @@ __device__ __forceinline__ u32 wave_all(u32 x, F f) {
     return __builtin_amdgcn_readfirstlane(x);
 }
 
+// Sixteen rows of 2 D bytes in LDS: 16 bytes of a row at position chunk ^ swizzle(row), so that 16 rows' same chunk lie on all banks
+template <int D>
+__device__ __forceinline__ u32 tile_place(int row, int chunk) {      // byte of a tile's [16][D]
+    return D == 128 ? (u32)(row * 256 + ((chunk ^ row) << 4)) : (u32)(row * 128 + ((chunk ^ (row >> 1 & 7)) << 4));
+}
+__device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
 #define ATTN_CUS 256                     // of an MI355X
 
 static int check_cache(const char* who, const vox_block_cache& c, bool bounds) {
@@ -64,6 +71,7 @@ static int check_cache(const char* who, const vox_block_cache& c, bool bounds) {
     if (c.dtype != VOX_DTYPE_BF16 && c.dtype != VOX_DTYPE_F16) return vox_fail(VOX_ERR_INVALID, "%s: dtype %d", who, c.dtype);
     if ((size_t)c.kv & 15) return vox_fail(VOX_ERR_INVALID, "%s: the cache does not lie on 16 bytes", who);
     if (!bounds) return VOX_OK;
+    if ((int64_t)c.n_pages * (c.page_size / (c.block > 0 ? c.block : 1)) * c.kv_heads > 0xffffffffll) return vox_fail(VOX_ERR_INVALID, "%s: %d pages of %d tokens and %d kv heads are 2^32 blocks or more", who, c.n_pages, c.page_size, c.kv_heads);
     if ((int64_t)c.n_pages * c.page_size > 0x7fffffff) return vox_fail(VOX_ERR_INVALID, "%s: %d pages of %d tokens are 2^31 or more", who, c.n_pages, c.page_size);
     if (c.block != 16 && c.block != 32 && c.block != 64 && c.block != 128) return vox_fail(VOX_ERR_INVALID, "%s: blocks of %d tokens (16, 32, 64 or 128)", who, c.block);
     if (c.page_size % c.block) return vox_fail(VOX_ERR_INVALID, "%s: pages of %d tokens are not whole blocks of %d", who, c.page_size, c.block);
@@ -314,7 +322,7 @@ struct SelectArgs {
     const int *q_req, *q_kvlen, *indptr, *indices;
     int* blocks;
     long q_stride;
-    int n_rows, n_req, Hq, Hkv, max_kvlen, n_pages, page_size, block, top, first, last, stride, q_al, splits;
+    int n_rows, n_req, Hq, Hkv, max_kvlen, n_pages, page_size, block, top, first, last, stride, q_al, splits, stage_at;      // stage_at: byte of the waves' blocks in LDS
     u32* keys;                           // splits > 1: [row][kv head][stride]
     u32 per_magic;                       // j / per = umulhi(j, per_magic) for j < 2^16 (0: per is 1)
 };
@@ -449,7 +457,9 @@ __device__ __forceinline__ void choose(const u32* key, int lo, int cand, int nee
 
 // QT > 1: tiles of QT rows, a wave a row in the choice; QT == 1: a row, all waves together
 // SPLIT (QT == 1): the scores alone, of one part of the row's blocks, into the workspace
-template <int F16, int D, int QT, int W, bool SPLIT>
+// NT: tiles of 16 blocks that a wave brings to its part of LDS at a time, in rows of memory (a lane's 16 bytes of a block beside the next block's 16 would go through the
+// address unit at a quarter of the rate); 0, where the keys leave no room for it: straight to registers
+template <int F16, int D, int QT, int W, bool SPLIT, int NT>
 __global__ __launch_bounds__(64 * W, QT == 16 ? 4 : 2) void k_block_select(SelectArgs a) {
     constexpr int MT = (2 * QT + 15) / 16, KS = 2 * D / 64;          // tiles of 16 product rows, steps of 64 numbers
     extern __shared__ __attribute__((aligned(16))) u32 keys[];       // [QT][a.stride]; before: [QT][D], N and P of a channel in the halves
@@ -514,6 +524,8 @@ __global__ __launch_bounds__(64 * W, QT == 16 ? 4 : 2) void k_block_select(Selec
 #pragma unroll
         for (int s = 0; s < KS; ++s) av[t][s] = *reinterpret_cast<const i32x4*>(&s_a[16 * t + c][64 * s + 16 * g]);
 
+    const u32 stage_at = a.stage_at + wave * NT * 32 * D, stage0 = (u32)(size_t)(__attribute__((address_space(3))) u32*)keys + stage_at, place = tile_place<D>(c, g);
+    const char* const stage = reinterpret_cast<const char*>(keys) + stage_at;
     for (int ra = 0; ra < R;) {
         const int req = __builtin_amdgcn_readfirstlane(s_req[ra]);
         if (req < 0) { ++ra; continue; }
@@ -531,31 +543,56 @@ __global__ __launch_bounds__(64 * W, QT == 16 ? 4 : 2) void k_block_select(Selec
             int pg = -1;
             if (j < j1 && pj < np) pg = a.indices[p0 + pj];
             const bool ok = pg >= 0 && pg < a.n_pages;
-            const size_t at = ok ? ((size_t)pg * a.Hkv + h) * per + (j - pj * per) : 0;
+            const u32 at = ok ? ((u32)pg * a.Hkv + h) * per + (j - pj * per) : 0;
             const float step = ok ? a.steps[at] : __uint_as_float(0x7fc00000u);      // (NaN: a block without a page)
-            const u32 at_lo = (u32)at, at_hi = (u32)(at >> 32);
-            i32x4 b[4][KS];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const size_t from = (size_t)(u32)__shfl((int)at_lo, 16 * u + c, 64) | (size_t)(u32)__shfl((int)at_hi, 16 * u + c, 64) << 32;
-                const i32x4* const src = reinterpret_cast<const i32x4*>(a.bounds + from * 2 * D) + g;
-#pragma unroll
-                for (int s = 0; s < KS; ++s) b[u][s] = src[4 * s];
-            }
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                if (j0 + 16 * u >= j1) break;
+            auto score = [&](int u, const i32x4 (&b)[KS]) {
                 const float st = __shfl(step, 16 * u + c, 64);
 #pragma unroll
                 for (int t = 0; t < MT; ++t) {
                     i32x4 s4 = {0, 0, 0, 0};
 #pragma unroll
-                    for (int s = 0; s < KS; ++s) s4 = __builtin_amdgcn_mfma_i32_16x16x64_i8(av[t][s], b[u][s], s4, 0, 0, 0);
+                    for (int s = 0; s < KS; ++s) s4 = __builtin_amdgcn_mfma_i32_16x16x64_i8(av[t][s], b[s], s4, 0, 0, 0);
                     u32* const dst = dst0 + (size_t)(8 * t + 2 * g) * a.stride + j0 + 16 * u + c;      // product rows 4 g + 2 x, + 1: query row 8 t + 2 g + x
                     if (QT == 1 && g) continue;
 #pragma unroll
                     for (int x = 0; x < (QT == 1 ? 1 : 2); ++x)
                         if (j0 + 16 * u + c < j1) dst[x * a.stride] = st == st ? score_key((float)(s4[2 * x] + 64 * s4[2 * x + 1]) * st) : 0;
+                }
+            };
+            if constexpr (NT > 0) {
+                constexpr int LPR = D / 8, PIECES = 32 * D / 1024;   // lanes a row, loads a tile
+#pragma unroll
+                for (int u0 = 0; u0 < 4; u0 += NT) {
+                    if (j0 + 16 * u0 >= j1) break;
+#pragma unroll
+                    for (int u = 0; u < NT; ++u)
+#pragma unroll
+                        for (int i = 0; i < PIECES; ++i) {
+                            const int row = i * (64 / LPR) + lane / LPR, chunk = lane % LPR ^ (D == 128 ? row : row >> 1 & 7);      // (what tile_place puts at this lane's position)
+                            const u32 from = (u32)__shfl((int)at, 16 * (u0 + u) + row, 64);
+                            lds_dma16(a.bounds + (size_t)from * (2 * D) + 16 * chunk, stage0 + (u32)(u * 32 * D + i * 1024));
+                        }
+                    dma_wait();
+#pragma unroll
+                    for (int u = 0; u < NT; ++u) {
+                        i32x4 b[KS];
+#pragma unroll
+                        for (int s = 0; s < KS; ++s) b[s] = *reinterpret_cast<const i32x4*>(stage + u * 32 * D + (place ^ 64 * s));
+                        score(u0 + u, b);
+                    }
+                }
+            } else {
+                i32x4 b[4][KS];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const i32x4* const src = reinterpret_cast<const i32x4*>(a.bounds + (size_t)(u32)__shfl((int)at, 16 * u + c, 64) * (2 * D)) + g;
+#pragma unroll
+                    for (int s = 0; s < KS; ++s) b[u][s] = src[4 * s];
+                }
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    if (j0 + 16 * u >= j1) break;
+                    score(u, b[u]);
                 }
             }
         }
@@ -679,12 +716,7 @@ __device__ __forceinline__ int first_entry(const int* list, int top, int lane) {
 
 // A tile is 16 tokens.  K comes to a wave's own part of LDS (memory to LDS, no registers, no barrier: the wave waits for its own) and from there to the product's lanes: a lane has
 // 16 bytes of a token, its neighbour the next token's, and loads of that pattern go through at 16 bytes a clock and CU, a quarter of what rows in order do (the chunk of
-// 1024 rows was held up by it 77 % of its time, a row's block of threads drew 35 bytes a ns).  Place in LDS: 16 bytes of a row at position chunk ^ swizzle(row), so
-// that 16 rows' same chunk lie on all banks.
-template <int D>
-__device__ __forceinline__ u32 tile_place(int row, int chunk) {      // byte of a tile's [16][D]
-    return D == 128 ? (u32)(row * 256 + ((chunk ^ row) << 4)) : (u32)(row * 128 + ((chunk ^ (row >> 1 & 7)) << 4));
-}
+// 1024 rows was held up by it 77 % of its time, a row's block of threads drew 35 bytes a ns).
 template <int D>
 struct KLane {
     static constexpr int PIECES = 32 * D / 1024;                     // wave loads a tile: 64 lanes of 16 bytes, 512 / D rows
@@ -713,7 +745,6 @@ struct KLane {
         return s4;
     }
 };
-__device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 // T tiles' V as a wave's registers
 template <int D, int T>
 struct VTiles {
@@ -1394,21 +1425,24 @@ int vox_block_select(vox_ctx* ctx, void* stream, const vox_block_select_args* a)
     const int64_t room = z.splits > 1 ? (int64_t)r.n_rows * c.kv_heads * z.stride * 4 : 0;
     if (room && (!a->workspace || (size_t)a->workspace & 15 || a->workspace_bytes < room))
         return vox_fail(VOX_ERR_INVALID, "block_select: a workspace of %lld bytes on 16, %lld are wanted", (long long)(a->workspace ? a->workspace_bytes : 0), (long long)room);
+    const int words = z.splits == 1 && z.stride > c.head_dim ? z.stride : c.head_dim;
+    const size_t lds = (size_t)qt * words * 4 + 15 & ~(size_t)15, tile = 32 * (size_t)c.head_dim;
     SelectArgs s{(const bf16_t*)a->q, c.bounds, c.steps, r.q_req, r.q_kvlen, r.kv_indptr, r.kv_indices, a->blocks, (long)a->q_stride,
                  r.n_rows, r.n_req, r.heads, c.kv_heads, r.max_kvlen, c.n_pages, c.page_size, c.block, a->top, a->first, a->last, z.stride,
-                 ((size_t)a->q & 15) == 0 && a->q_stride % 8 == 0, z.splits, (u32*)a->workspace, per > 1 ? (u32)((1ull << 32) / per + 1) : 0u};
+                 ((size_t)a->q & 15) == 0 && a->q_stride % 8 == 0, z.splits, (int)lds, (u32*)a->workspace, per > 1 ? (u32)((1ull << 32) / per + 1) : 0u};
     const int64_t grid = (int64_t)((r.n_rows + qt - 1) / qt) * c.kv_heads * z.splits;
     if (grid > 0x7fffffff) return vox_fail(VOX_ERR_INVALID, "block_select: %d rows of %d kv heads are more than a launch holds", r.n_rows, c.kv_heads);
-#define SELECT_OF(QT, W, SPLIT) (c.dtype == VOX_DTYPE_F16 ? (c.head_dim == 128 ? (const void*)k_block_select<1, 128, QT, W, SPLIT> : (const void*)k_block_select<1, 64, QT, W, SPLIT>) \
-                                                         : (c.head_dim == 128 ? (const void*)k_block_select<0, 128, QT, W, SPLIT> : (const void*)k_block_select<0, 64, QT, W, SPLIT>))
-    const int words = z.splits == 1 && z.stride > c.head_dim ? z.stride : c.head_dim;
+#define SELECT_OF(QT, W, SPLIT, NT) (c.dtype == VOX_DTYPE_F16 ? (c.head_dim == 128 ? (const void*)k_block_select<1, 128, QT, W, SPLIT, NT> : (const void*)k_block_select<1, 64, QT, W, SPLIT, NT>) \
+                                                             : (c.head_dim == 128 ? (const void*)k_block_select<0, 128, QT, W, SPLIT, NT> : (const void*)k_block_select<0, 64, QT, W, SPLIT, NT>))
     if (z.splits > 1) {
-        VOX_TRY(launch(SELECT_OF(1, 4, true), dim3((unsigned)grid), 256, (size_t)words * 4, (hipStream_t)stream, s));
+        VOX_TRY(launch(SELECT_OF(1, 4, true, 4), dim3((unsigned)grid), 256, lds + 16 * tile, (hipStream_t)stream, s));
         return launch((const void*)k_block_choose<16>, dim3((unsigned)(grid / z.splits)), 1024, 0, (hipStream_t)stream, s);
     }
-    const void* kern = qt == 16 ? SELECT_OF(16, 8, false) : qt == 8 ? SELECT_OF(8, 8, false) : W == 4 ? SELECT_OF(1, 4, false) : SELECT_OF(1, 16, false);
+    if (qt == 16) return launch(SELECT_OF(16, 8, false, 1), dim3((unsigned)grid), 512, lds + 8 * tile, (hipStream_t)stream, s);
+    if (qt == 8) return launch(SELECT_OF(8, 8, false, 0), dim3((unsigned)grid), 512, lds, (hipStream_t)stream, s);
+    return W == 4 ? launch(SELECT_OF(1, 4, false, 4), dim3((unsigned)grid), 256, lds + 16 * tile, (hipStream_t)stream, s)
+                  : launch(SELECT_OF(1, 16, false, 0), dim3((unsigned)grid), 1024, lds, (hipStream_t)stream, s);
 #undef SELECT_OF
-    return launch(kern, dim3((unsigned)grid), 64 * W, (size_t)qt * words * 4, (hipStream_t)stream, s);
 }
 
 static int check_attention(const vox_block_attention_args* a) {

@@ -166,6 +166,8 @@ typedef struct {
 } vox_block_select_args;
 int64_t vox_block_select_workspace_bytes(const vox_block_select_args* a);
 int vox_block_select(vox_ctx* ctx, void* stream, const vox_block_select_args* a);
+/* Which launch serves the call, decided on the host: rows a block of threads (16, 8 or 1), or minus the parts that a row's scores are split into; 0: refused. */
+int vox_block_select_form(const vox_block_select_args* a);
 
 /* out[i, h] = softmax(scale q . K) V over the tokens < q_kvlen[i] of the blocks in row i's list of h's kv head; out [n_rows,heads,head_dim] contiguous.  An entry
  * counts if it is a block of the row and larger than every entry before it.  A row without any such entry is zero.  Scores, sums and
@@ -184,6 +186,8 @@ typedef struct {
 } vox_block_attention_args;
 int64_t vox_block_attention_workspace_bytes(const vox_block_attention_args* a);
 int vox_block_attention(vox_ctx* ctx, void* stream, const vox_block_attention_args* a);
+/* The same: rows a block of threads (1 to 16), or minus the parts that a row's list is split into; 0: refused. */
+int vox_block_attention_form(const vox_block_attention_args* a);
 
 /* nn.Linear on bf16 (qwen3_tts.py:562-601): y[b,n] = bf16(dot(W[n,:],x[b,:]) + bias[n]);
  * residual != NULL: y = bf16(residual + y).  act: 0 none, 1 SiLU applied to the rounded output. */

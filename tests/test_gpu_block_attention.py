@@ -642,3 +642,222 @@ def test_offsets_beyond_32_bits(dev):
     k = s.rnd(1, h, d)
     B.rope_append(q, k, k, kv, None, s.q_kvlen, torch.tensor([total - 1], device=dev), torch.tensor([100], device=dev))
     assert torch.equal(kv[total - 1, :, 100], k.expand(2, -1, -1))
+
+
+# ---------------------------------------------------------------- every launch
+def select_form(s, hq, block, top, most, n_req, first=1, last=2):
+    from vox_serve_amd import _native as N
+    from vox_serve_amd import block_attention as B
+    return N.lib().vox_block_select_form(B._SELECT.pack(0, 16, 16, s.kv.shape[0], s.page, block, s.h, s.d, B._DTYPES[s.dtype], 16, 16, 16, 16, s.n, len(s.kv_lens), n_req, hq, most, 0, 16, 16, 0, 0, 0, top,
+                                                        first, last))
+
+
+def attend_form(s, hq, block, top, n_req):
+    from vox_serve_amd import _native as N
+    from vox_serve_amd import block_attention as B
+    return N.lib().vox_block_attention_form(B._ATTEND.pack(16, 0, 0, s.kv.shape[0], s.page, block, s.h, s.d, B._DTYPES[s.dtype], 16, 16, 16, 16, s.n, len(s.kv_lens), n_req, hq, 2 ** 31 - 1, 0, 16, 16, 16,
+                                                           0, 0, 0, top, 1.0))
+
+
+def some(n, count, seed):
+    """The first and last rows and some between."""
+    r = np.random.default_rng(seed)
+    return sorted(i for i in ({0, n - 1} if count < 3 else {0, 1, 15, 16, 17, n - 2, n - 1}) | set(int(x) for x in r.integers(0, n, count)) if 0 <= i < n)
+
+
+SELECT_FORMS = [  # form, heads, kv heads, dim, page, block, top, kv lengths, new rows, max_kvlen
+    (16, 16, 8, 128, 32, 16, 7, [300, 200, 90], [60, 30, 1], 300),
+    (16, 28, 2, 64, 64, 32, 6, [2000], [601], 2000),
+    (16, 8, 8, 64, 48, 16, 5, [400, 350], [90, 3], 16384),          # as many blocks as sixteen rows' keys may be
+    (8, 16, 8, 128, 16, 16, 9, [280, 150], [85, 9], 16385),         # one more
+    (8, 4, 4, 64, 128, 32, 20, [9000], [190], 40000),
+    (8, 4, 4, 64, 128, 16, 33, [40000], [190], 40000),              # thousands of candidates
+    (1, 4, 4, 64, 128, 16, 33, [300], [190], 65537),                # more than eight rows' keys may be
+    (1, 8, 8, 128, 128, 16, 20, [9000, 700], [40, 1], 9000),
+    (1, 4, 4, 64, 64, 64, 5, [640, 130], [1, 1], 640),
+    (-64, 4, 2, 128, 128, 16, 40, [20000, 16399], [1, 1], 524288),  # parts without a block among them
+    (-5, 32, 2, 64, 128, 16, 17, [18000], [25], 18000),
+]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("form,hq,h,d,page,block,top,kv_lens,q_lens,most", SELECT_FORMS)
+def test_select_of_every_form(dev, dtype, form, hq, h, d, page, block, top, kv_lens, q_lens, most):
+    from vox_serve_amd import block_attention as B
+    s = Paged(dev, TYPES[dtype], h, d, page, kv_lens, q_lens, seed=top)
+    assert select_form(s, hq, block, top, most, len(q_lens)) == form
+    q = s.rnd(s.n, hq, d)
+    bounds, steps = B.new_bounds(s.kv, block)
+    per = page // block
+    B.update_bounds(s.kv, bounds, steps, torch.arange(s.kv.shape[0], device=dev).repeat_interleave(per), torch.arange(block - 1, page, block, device=dev).repeat(s.kv.shape[0]))
+    # the cache's first page, by the oracle: the choice below is of these bounds
+    for g in range(h):
+        for j in range(per):
+            wb, ws = R.bounds(f64(s.kv[0, 0, j * block:(j + 1) * block, g]))
+            assert np.array_equal(bounds[0, g, j].cpu().numpy(), wb) and float(steps[0, g, j]) == ws
+    got = B.select_blocks(q, bounds, steps, *s.plan, block=block, top=top, max_kvlen=most, n_req=len(q_lens)).cpu().numpy()
+    nb, ns = bounds.cpu().numpy(), steps.cpu().numpy()
+    long = max(kv_lens) // block > 500
+    for i in some(s.n, 2 if long else 25, top):
+        assert np.array_equal(got[i], R.select(f64(q[i]), nb, ns, s.pages[s.req[i]], s.kvlen[i], block, top, 1, 2)), i
+    # every row's by another launch
+    one = torch.cat([B.select_blocks(q[i:i + 1], bounds, steps, s.q_req[i:i + 1], s.q_kvlen[i:i + 1], s.indptr, s.indices, block=block, top=top, max_kvlen=max(kv_lens)) for i in range(s.n)])
+    assert np.array_equal(got, one.cpu().numpy())
+
+
+ATTEND_FORMS = [  # form, heads, kv heads, dim, page, block, top, kv lengths, new rows
+    (16, 16, 8, 128, 32, 16, 6, [220, 150, 60], [180, 40, 9]),
+    (16, 8, 8, 64, 16, 16, 5, [260, 100], [190, 35]),
+    (8, 32, 8, 64, 64, 32, 4, [300, 64], [140, 20]),
+    (10, 24, 8, 128, 128, 64, 3, [400], [190]),
+    (4, 28, 4, 128, 48, 16, 7, [290], [260]),
+    (2, 64, 4, 64, 32, 32, 4, [300, 33], [160, 33]),
+    (2, 60, 4, 128, 16, 16, 9, [240], [200]),
+    (1, 72, 4, 64, 16, 16, 5, [150], [140]),                # 18 heads on a kv head
+    (-16, 16, 2, 128, 128, 128, 32, [5000, 4200], [1, 1]),
+    (-5, 4, 4, 64, 64, 16, 100, [1700], [30]),
+    (-64, 1, 1, 64, 128, 128, 128, [17000], [1]),
+    (1, 4, 4, 128, 32, 32, 32, [1100], [30]),
+]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("form,hq,h,d,page,block,top,kv_lens,q_lens", ATTEND_FORMS)
+def test_attention_of_every_form(dev, dtype, form, hq, h, d, page, block, top, kv_lens, q_lens):
+    from vox_serve_amd import block_attention as B
+    s = Paged(dev, TYPES[dtype], h, d, page, kv_lens, q_lens, seed=block + top)
+    assert attend_form(s, hq, block, top, len(q_lens)) == form
+    q = s.rnd(s.n, hq, d)
+    blocks = random_lists(s, h, block, top, top)
+    got = B.block_attention(q, s.kv, blocks, *s.plan, block=block, n_req=len(q_lens))
+    check_attend(s, q, got, blocks, block, d ** -0.5, some(s.n, 12, top))
+    # all rows against the launch of a row each: both are within half a step, and fp32's share, of the same value
+    other = B.block_attention(q, s.kv, blocks, *s.plan, block=block, n_req=0).double()
+    a = got.double()
+    step = torch.finfo(s.dtype).eps
+    assert ((a - other).abs() <= step * torch.maximum(a.abs(), other.abs()) + 2.0 ** -13).all()
+    # operands and results that lie on their type alone
+    loose = torch.empty(s.n * hq * d + 3, dtype=s.dtype, device=dev)
+    q2, out = loose[1:1 + s.n * hq * d].view(s.n, hq, d), torch.empty(s.n * hq * d + 1, dtype=s.dtype, device=dev)[1:].view(s.n, hq, d)
+    q2.copy_(q)
+    B.block_attention(q2, s.kv, blocks, *s.plan, block=block, n_req=len(q_lens), out=out)
+    assert torch.equal(out, got)
+
+
+@pytest.mark.parametrize("hq,h,d", [(16, 8, 128), (8, 8, 64), (28, 4, 64)])
+def test_rows_together_masked_places(dev, hq, h, d):
+    """As test_attention_masked_places, where rows of a chunk share a launch's blocks: what one row may not see, or does not list, and another does, reaches the
+    other alone, bit for bit."""
+    from vox_serve_amd import block_attention as B
+    for dtype in (torch.bfloat16, torch.float16):
+        q_lens, kv_lens = [230, 40, 9], [300, 90, 37]
+        s = Paged(dev, dtype, h, d, 32, kv_lens, q_lens, seed=d)
+        assert attend_form(s, hq, 16, 6, 3) > 1
+        q = s.rnd(s.n, hq, d)
+        blocks = random_lists(s, h, 16, 6, 5)
+        want = B.block_attention(q, s.kv, blocks, *s.plan, block=16, n_req=3)
+        check_attend(s, q, want, blocks, 16, d ** -0.5, some(s.n, 8, d))
+        lists = blocks.cpu().numpy()
+        for fill in (float("nan"), float("inf"), float("-inf"), torch.finfo(dtype).min):
+            b = s.kv.clone()
+            owned = {p for pages in s.pages for p in pages}
+            for p in range(b.shape[0]):
+                if p not in owned:
+                    b[p] = fill
+            for r, n in enumerate(kv_lens):
+                for t in range(n, len(s.pages[r]) * 32):
+                    b[s.pages[r][t // 32], :, t % 32] = fill
+            assert torch.equal(B.block_attention(q, b, blocks, *s.plan, block=16, n_req=3), want)
+            # one token in the middle of the chunk
+            token = 200
+            b = s.kv.clone()
+            b[s.pages[0][token // 32], :, token % 32] = fill
+            got = B.block_attention(q, b, blocks, *s.plan, block=16, n_req=3)
+            feel = np.array([[s.req[i] == 0 and s.kvlen[i] > token and token // 16 in lists[i, g].tolist() for g in range(h)] for i in range(s.n)])
+            assert feel.any() and not feel.all()
+            feel = torch.from_numpy(feel).to(dev).repeat_interleave(hq // h, 1)
+            assert torch.equal(got[~feel], want[~feel])
+            if fill != fill:
+                assert torch.isnan(got[feel]).all()
+        # an infinite value alone: that channel of the rows that see it, no other
+        b = s.kv.clone()
+        b[s.pages[0][token // 32], 1, token % 32, 0, 7] = float("inf")
+        got = B.block_attention(q, b, blocks, *s.plan, block=16, n_req=3)
+        feel = torch.tensor([s.req[i] == 0 and s.kvlen[i] > token and token // 16 in lists[i, 0].tolist() for i in range(s.n)], device=dev)
+        g0 = hq // h
+        assert torch.isposinf(got[feel][:, :g0, 7]).all()
+        keep = torch.ones(d, dtype=torch.bool)
+        keep[7] = False
+        assert torch.equal(got[:, :, keep], want[:, :, keep]) and torch.equal(got[~feel], want[~feel]) and torch.equal(got[:, g0:], want[:, g0:])
+
+
+def test_rows_together_entries_that_do_not_count(dev):
+    """Lists that are not ascending, blocks far behind the sequence, pages that do not exist, rows that are passed over in the middle of others, in the launch of rows
+    together; lists that lie thousands of blocks apart."""
+    from vox_serve_amd import block_attention as B
+    s = Paged(dev, torch.bfloat16, 8, 64, 16, [72000], [230], seed=3)
+    hq = 16
+    q = s.rnd(s.n, hq, 64)
+    r = np.random.default_rng(1)
+    lists = np.full((s.n, 8, 7), -1, np.int32)
+    for i in range(s.n):
+        for g in range(8):
+            lists[i, g] = [0, 4499, 4498, 2 ** 31 - 1, 4499, 3, -7] if (i + g) % 3 == 0 else r.integers(-2, 4500, 7) if (i + g) % 3 == 1 else np.sort(r.permutation(4500)[:7])
+    plain = np.full_like(lists, -1)
+    for i in range(s.n):
+        for g in range(8):
+            seen, out = -1, []
+            for j in lists[i, g].tolist():
+                if j > seen:
+                    seen = j
+                    if j * 16 < s.kvlen[i]:
+                        out.append(j)
+            plain[i, g, :len(out)] = out
+    lens, req = s.q_kvlen.clone(), s.q_req.clone()
+    lens[5], lens[40], req[17], req[100] = 0, -3, -1, 1
+    indices = s.indices.clone()
+    indices[4499], indices[1000:1500] = -1, 10 ** 9
+    plain[np.isin(plain, [4499] + list(range(1000, 1500)))] = -2        # (not listed)
+    assert attend_form(s, hq, 16, 7, 1) == 16
+    out = torch.full((s.n, hq, 64), 3.0, dtype=s.dtype, device=dev)
+    B.block_attention(q, s.kv, torch.from_numpy(lists).to(dev), req, lens, s.indptr, indices, block=16, n_req=1, out=out)
+    over = [5, 17, 40, 100]
+    assert (out[over] == 3).all()
+    rows = [i for i in some(s.n, 40, 2) if i not in over]
+    ok = np.where(plain == -2, -1, plain)
+    ok = np.stack([[np.concatenate([x[x >= 0], x[x < 0]]) for x in row] for row in ok])
+    check_attend(s, q, out, torch.from_numpy(ok), 16, 0.125, rows)
+
+
+def test_captured_rows_together(dev):
+    """The launch of many rows captured beside selection and append, replayed with new inputs."""
+    from vox_serve_amd import _native as N
+    from vox_serve_amd import block_attention as B
+    hq, h, d, page, block, top = 16, 8, 128, 64, 16, 12
+    s = Paged(dev, torch.bfloat16, h, d, page, [600, 333, 128], [200, 31, 70], seed=4)
+    assert attend_form(s, hq, block, top, 3) == 16 and select_form(s, hq, block, top, 600, 3) == 16
+    qkv = s.rnd(s.n, (hq + 2 * h) * d)
+    q, k, v = (x.unflatten(1, (-1, d)) for x in qkv.split([hq * d, h * d, h * d], 1))
+    pos, cs = s.q_kvlen - 1, table(dev, 1024, d // 2)
+    bounds, steps = s.bounds(block)
+    qr, blocks, out = torch.empty(s.n, hq, d, dtype=s.dtype, device=dev), torch.empty(s.n, h, top, dtype=torch.int32, device=dev), torch.empty(s.n, hq, d, dtype=s.dtype, device=dev)
+
+    def calls(kv, b, st, qr, blocks, out):
+        B.rope_append(q, k, v, kv, cs, pos, s.row_page, s.row_slot, bounds=b, steps=st, n_req=3, out=qr)
+        B.select_blocks(qr, b, st, *s.plan, block=block, top=top, max_kvlen=600, n_req=3, out=blocks)
+        B.block_attention(qr, kv, blocks, *s.plan, block=block, n_req=3, out=out)
+
+    calls(s.kv, bounds, steps, qr, blocks, out)
+    with N.graph_capture() as cap:
+        calls(s.kv, bounds, steps, qr, blocks, out)
+    for _ in range(4):
+        qkv.copy_(s.rnd(*qkv.shape))
+        kv2, b2, s2 = s.kv.clone(), bounds.clone(), steps.clone()
+        N.check(N.lib().vox_graph_launch(cap.graph, N.stream()))
+        got = [x.clone() for x in (qr, blocks, out, s.kv, bounds, steps)]
+        want = [torch.empty_like(x) for x in (qr, blocks, out)]
+        calls(kv2, b2, s2, *want)
+        torch.cuda.synchronize()
+        for x, y in zip(got, want + [kv2, b2, s2]):
+            assert torch.equal(x, y)
+    N.lib().vox_graph_destroy(cap.graph)

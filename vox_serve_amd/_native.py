@@ -88,6 +88,8 @@ _SIGS = {
     "vox_block_select": (c_int, [c_void_p, c_void_p, c_char_p]),
     "vox_block_attention_workspace_bytes": (c_int64, [c_char_p]),
     "vox_block_attention": (c_int, [c_void_p, c_void_p, c_char_p]),
+    "vox_block_select_form": (c_int, [c_char_p]),
+    "vox_block_attention_form": (c_int, [c_char_p]),
     "vox_attention_form": (c_int, [c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
     "vox_linear": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
                            c_int]),

@@ -1,5 +1,7 @@
 // Long contexts: rows rotated into a paged cache, the bounds of its blocks, the blocks that a row reads, and attention over them
 // (voxhip.h: vox_rope_append, vox_block_bounds, vox_block_select, vox_block_attention).
+#include <math.h>
+
 #include <type_traits>
 
 #include "vox_internal.h"
@@ -1398,7 +1400,9 @@ static SelectShape select_shape(const vox_block_select_args* a) {
     const vox_block_rows& r = a->rows;
     const int most = (int)(((int64_t)r.max_kvlen + a->cache.block - 1) / a->cache.block);
     // rows a tile: 16 while their keys take half a CU's LDS, 8 while they take most of it (4096 blocks), else (and for rows of different requests) one
-    const bool many = r.n_own > 0 && r.n_rows >= 2 * (int64_t)r.n_own;
+    // where there are enough of them: us, a row / 16 rows together, 256 blocks: 16 heads on 8 of 128, 64 rows (512 blocks of threads) 12.2 / 14.6, 128 20.8 / 15.0; 32 on 8,
+    // 64 rows 12.0 / 16.1, 128 20.2 / 16.0; 32 on 2, 128 rows (256) 11.2 / 21.5, 512 20.9 / 21.9; 8 on 8 of 64, 128 rows 12.3 / 13.4, 512 38.4 / 13.6.
+    const bool many = r.n_own > 0 && r.n_rows >= 2 * (int64_t)r.n_own && (int64_t)r.n_rows * a->cache.kv_heads >= 640 + 32 * (r.heads / a->cache.kv_heads);
     SelectShape s{many && most <= 1024 ? 16 : many && most <= 4096 ? 8 : 1, 8, 1, 0};
     s.stride = most + (s.qt > 1 ? SEL_PAD : 0);
     if (s.qt > 1) return s;
@@ -1412,6 +1416,11 @@ int64_t vox_block_select_workspace_bytes(const vox_block_select_args* a) {
     if (check_select(a) != VOX_OK) return -1;
     const SelectShape s = select_shape(a);
     return s.splits > 1 ? (int64_t)a->rows.n_rows * a->cache.kv_heads * s.stride * 4 : 0;
+}
+int vox_block_select_form(const vox_block_select_args* a) {
+    if (check_select(a) != VOX_OK) return 0;
+    const SelectShape s = select_shape(a);
+    return s.splits > 1 ? -s.splits : s.qt;
 }
 int vox_block_select(vox_ctx* ctx, void* stream, const vox_block_select_args* a) {
     (void)ctx;
@@ -1459,10 +1468,17 @@ static AttnShape attn_shape(const vox_block_attention_args* a, int cus) {
     const vox_block_rows& r = a->rows;
     const int G = r.heads / a->cache.kv_heads;
     AttnShape s{0, 1, 1, (G + 15) / 16};
-    if (r.n_own > 0 && r.n_rows >= 2 * r.n_own && G <= 16) {
-        s.tiles = G > 1 ? 2 : 1;
-        s.per_tile = s.tiles * (16 / G);
-        return s;
+    // Rows together pay once there are enough of them: a tile's blocks of threads go through what all its rows list, some 1.7 us for 128 tokens however few there are, a
+    // row's through its own list, 15 to the us once the card is full.  What R neighbouring rows list between them is some R^0.45 lists.  us, a row / rows together, lists
+    // of 2048 tokens: 16 heads on 8 of 128, 64 rows (512 blocks of threads) 40 / 104, 128 70 / 102, 512 247 / 101; 32 on 8, 64 rows 38 / 72, 128 69 / 71,
+    // 512 242 / 88; 32 on 2, 128 rows (256) 33 / 45, 512 72 / 57; 14 on 2 of 64, 128 rows 24 / 42, 512 51 / 43; 8 on 8 of 64, 128 rows 50 / 75, 512 174 / 76.
+    if (r.n_own > 0 && r.n_rows >= 2 * (int64_t)r.n_own && G <= 16) {
+        const int tiles = G > 1 ? 2 : 1, per_tile = tiles * (16 / G);
+        if ((double)r.n_rows * a->cache.kv_heads >= 470.0 * pow(per_tile, 0.45)) {
+            s.tiles = tiles;
+            s.per_tile = per_tile;
+            return s;
+        }
     }
     const long tokens = (long)a->top * a->cache.block, blocks = (long)r.n_rows * a->cache.kv_heads * s.head_tiles;
     if (tokens > 1024) {
@@ -1477,6 +1493,11 @@ int64_t vox_block_attention_workspace_bytes(const vox_block_attention_args* a) {
     if (check_attention(a) != VOX_OK) return -1;
     const AttnShape s = attn_shape(a, ATTN_CUS);
     return s.splits > 1 ? (int64_t)a->rows.n_rows * a->rows.heads * s.splits * (a->cache.head_dim + 2) * 4 : 0;
+}
+int vox_block_attention_form(const vox_block_attention_args* a) {
+    if (check_attention(a) != VOX_OK) return 0;
+    const AttnShape s = attn_shape(a, ATTN_CUS);
+    return s.splits > 1 ? -s.splits : s.tiles ? s.per_tile : 1;
 }
 int vox_block_attention(vox_ctx* ctx, void* stream, const vox_block_attention_args* a) {
     (void)ctx;

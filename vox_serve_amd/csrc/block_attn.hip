@@ -65,6 +65,14 @@ __device__ __forceinline__ u32 tile_place(int row, int chunk) {      // byte of 
 }
 __device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
+// Rows ra, ra + 1, .. of a tile that belong to one request (a lane has its row's request, -1: passed over): one past the last, and the most tokens one of them sees
+__device__ __forceinline__ int run_of(int my_req, int my_len, int ra, int R, int lane, int req, int& n_most) {
+    const unsigned long long same = __ballot(lane < R && my_req == req) >> ra;
+    const int rb = ra + (int)__builtin_ctzll(~same);                 // (R is below 64: a zero follows)
+    n_most = (int)wave_all(lane >= ra && lane < rb ? (u32)my_len : 0u, [](u32 x, u32 y) { return max(x, y); });
+    return rb;
+}
+
 #define ATTN_CUS 256                     // of an MI355X
 
 static int check_cache(const char* who, const vox_block_cache& c, bool bounds) {
@@ -528,16 +536,16 @@ __global__ __launch_bounds__(64 * W, QT == 16 ? 4 : 2) void k_block_select(Selec
 
     const u32 stage_at = a.stage_at + wave * NT * 32 * D, stage0 = (u32)(size_t)(__attribute__((address_space(3))) u32*)keys + stage_at, place = tile_place<D>(c, g);
     const char* const stage = reinterpret_cast<const char*>(keys) + stage_at;
+    const int my_req = lane < R ? s_req[lane] : -1, my_len = lane < R ? s_len[lane] : 0;
     for (int ra = 0; ra < R;) {
-        const int req = __builtin_amdgcn_readfirstlane(s_req[ra]);
+        const int req = __builtin_amdgcn_readlane(my_req, ra);
         if (req < 0) { ++ra; continue; }
-        int rb = ra + 1;
-        while (rb < R && __builtin_amdgcn_readfirstlane(s_req[rb]) == req) ++rb;
         const int p0 = a.indptr[req], np = a.indptr[req + 1] - p0;
-        int n_most = 0;
-        for (int r = ra; r < rb; ++r) n_most = max(n_most, s_len[r]);
-        n_most = __builtin_amdgcn_readfirstlane(n_most);
-        const int have = (n_most + a.block - 1) / a.block, j1 = have > a.top ? have - a.last : 0;      // blocks to score: [first, j1)
+        int n_most;
+        int rb = 1;
+        if constexpr (QT == 1) n_most = __builtin_amdgcn_readfirstlane(my_len);
+        else rb = run_of(my_req, my_len, ra, R, lane, req, n_most);
+        const int have = (n_most - 1) / a.block + 1, j1 = have > a.top ? have - a.last : 0;      // blocks to score: [first, j1)
         // 64 blocks a step: a lane looks up one of them, four tiles of 16 go through the product
         u32* const dst0 = SPLIT ? a.keys + ((size_t)i0 * a.Hkv + h) * a.stride : keys;
         for (int j0 = a.first + (split * W + wave) * 64; j0 < j1; j0 += (SPLIT ? a.splits : 1) * W * 64) {
@@ -601,7 +609,7 @@ __global__ __launch_bounds__(64 * W, QT == 16 ? 4 : 2) void k_block_select(Selec
         if constexpr (SPLIT) return;
         __syncthreads();
         for (int r = ra + (QT > 1 ? wave : 0); r < rb; r += QT > 1 ? W : 1) {
-            const int mine = (s_len[r] + a.block - 1) / a.block, cand = mine - a.first - a.last, need = a.top - a.first - a.last;
+            const int mine = (__builtin_amdgcn_readlane(my_len, r) - 1) / a.block + 1, cand = mine - a.first - a.last, need = a.top - a.first - a.last;
             int* const out = a.blocks + ((size_t)(i0 + r) * a.Hkv + h) * a.top;
             if (mine <= a.top) {
                 for (int j = QT > 1 ? lane : tid; j < a.top; j += QT > 1 ? 64 : 64 * W) out[j] = j < mine ? j : -1;
@@ -1108,15 +1116,13 @@ __global__ __launch_bounds__(64 * W, 2) void k_block_attn_rows(BlockAttnArgs a) 
     float* const s_o = reinterpret_cast<float*>(lds);                // after the loops (where list and K were)
     float2* const s_ml = reinterpret_cast<float2*>(s_o + W * 16 * (D + 4));
 
+    const int my_req = lane < R ? s_req[lane] : -1, my_len = lane < R ? s_len[lane] : 0;
     for (int ra = 0; ra < R;) {
-        const int req = __builtin_amdgcn_readfirstlane(s_req[ra]);
+        const int req = __builtin_amdgcn_readlane(my_req, ra);
         if (req < 0) { ++ra; continue; }
-        int rb = ra + 1;
-        while (rb < R && __builtin_amdgcn_readfirstlane(s_req[rb]) == req) ++rb;
-        int n_most = 0;
-        for (int r = ra; r < rb; ++r) n_most = max(n_most, s_len[r]);
-        n_most = __builtin_amdgcn_readfirstlane(n_most);
         const int p0 = a.indptr[req], np = a.indptr[req + 1] - p0;
+        int n_most;
+        const int rb = run_of(my_req, my_len, ra, R, lane, req, n_most);
         int own[NC];                                                 // tokens that the column's row sees
 #pragma unroll
         for (int n = 0; n < NC; ++n) {
@@ -1132,7 +1138,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_block_attn_rows(BlockAttnArgs a) 
 #pragma unroll
                 for (int t = 0; t < CPL; ++t) o[n][t] = f32x4{0, 0, 0, 0};
             }
-            const int v_len = careful >= 0 ? __builtin_amdgcn_readfirstlane(s_len[careful]) : n_most;     // V of tokens from here on is taken as zero
+            const int v_len = careful >= 0 ? __builtin_amdgcn_readlane(my_len, careful) : n_most;     // V of tokens from here on is taken as zero
             if (tid == 0) s_seen = 0;
             for (int w0 = 0; w0 >= 0;) {                             // windows of blocks
                 for (int i = tid; i < ATTN_WINDOW / 2; i += 64 * W) s_bits[i] = 0;
@@ -1140,7 +1146,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_block_attn_rows(BlockAttnArgs a) 
                 __syncthreads();
                 for (int r = ra + wave; r < rb; r += W) {
                     const int* const from = lists + (size_t)r * a.Hkv * a.top;
-                    row_entries(from, first_entry(from, a.top, lane), a.top, (s_len[r] - 1) / a.block + 1, lane, [&](int j, bool ok) {
+                    row_entries(from, first_entry(from, a.top, lane), a.top, (__builtin_amdgcn_readlane(my_len, r) - 1) / a.block + 1, lane, [&](int j, bool ok) {
                         if (!ok || j < w0) return;
                         if (j - w0 < ATTN_WINDOW) atomicOr(&s_bits[(j - w0) >> 1], 1u << (r + 16 * ((j - w0) & 1)));
                         else atomicMin(&s_next, j);

@@ -861,3 +861,39 @@ def test_captured_rows_together(dev):
         for x, y in zip(got, want + [kv2, b2, s2]):
             assert torch.equal(x, y)
     N.lib().vox_graph_destroy(cap.graph)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("rows", [1, 240])
+def test_many_small_weights(dev, dtype, rows):
+    """One token with nearly all of the weight and 16 thousand with 2^-25 of it each: together they are more than a step of the output."""
+    from vox_serve_amd import block_attention as B
+    h, d, n = 8 if rows > 1 else 2, 64, 16384
+    s = Paged(dev, TYPES[dtype], h, d, 128, [n], [rows], seed=rows)
+    s.kv[:, 0] = 0
+    s.kv[:, 1] = 1.0
+    s.kv[s.pages[0][3], 0, 7] = 2.0
+    s.kv[s.pages[0][3], 1, 7] = 0.0
+    q = torch.full((rows, 2 * h, d), 1.0, dtype=s.dtype, device=dev)
+    blocks = torch.arange(128, dtype=torch.int32, device=dev).repeat(rows, h, 1).contiguous()
+    scale = 25 * np.log(2) / 128                              # the token's score is 25 log 2 above the others'
+    assert (attend_form(s, 2 * h, 128, 128, 1) > 1) == (rows > 1)
+    got = B.block_attention(q, s.kv, blocks, *s.plan, block=128, scale=float(scale), n_req=1)
+    check_attend(s, q, got, blocks, 128, np.float32(scale).astype(np.float64), [0] if rows == 1 else [0, 100])
+    assert (got > 4e-4).all()
+
+
+def test_select_takes_nothing_but_the_ends(dev):
+    from vox_serve_amd import block_attention as B
+    s = Paged(dev, torch.bfloat16, 8, 64, 16, [500, 320], [120, 1], seed=1)
+    q = s.rnd(s.n, 16, 64)
+    bounds, steps = s.bounds(16)
+    for n_req in (0, 2):
+        got = B.select_blocks(q, bounds, steps, *s.plan, block=16, top=5, first=2, last=3, max_kvlen=500, n_req=n_req)
+        for i in range(s.n):
+            have = -(-s.kvlen[i] // 16)
+            assert (got[i].cpu() == torch.tensor([0, 1, have - 3, have - 2, have - 1])).all()
+    # no row may see anything: nothing is written
+    out = torch.full((s.n, 8, 5), 9, dtype=torch.int32, device=dev)
+    B.select_blocks(q, bounds, steps, *s.plan, block=16, top=5, max_kvlen=0, out=out)
+    assert (out == 9).all()

@@ -796,6 +796,7 @@ struct VTiles {
 // column's last token lies in it.  What was a third more vector instructions a tile is the same to fp32 rounding.  CAREFUL: every score is masked, and
 // V that is not finite meets the weight as one term.
 #define ATTN_AHEAD 8.0f
+#define ATTN_LIFT 7.0f                   // fp16: weights 2^7 up, 2^15 at most, so that small ones keep their bits (2^17 tokens of a weight below 2^-24 would else be lost together)
 __device__ __forceinline__ float vmax(float x, float y) {            // (fmaxf of values that are no signalling NaN: without the two instructions that would quiet them)
     float r;
     asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(x), "v"(y));
@@ -825,7 +826,7 @@ __device__ __forceinline__ void weigh(f32x4 (&s4)[T], const int (&sees)[T], floa
 #pragma unroll
         for (int t = 0; t < D / 16; ++t) o[t] *= keep;
     }
-    const float base = m == -inf ? 0.0f : -m;
+    const float base = m == -inf ? 0.0f : (F16 ? ATTN_LIFT : 0.0f) - m;
     float p[4 * T], sum[T];
 #pragma unroll
     for (int x = 0; x < T; ++x) {
@@ -1044,6 +1045,7 @@ __global__ __launch_bounds__(64 * W, 1) void k_block_attn_row(BlockAttnArgs a) {
 #pragma unroll
                 for (int x = 0; x < T; ++x) {
                     s4[x] = kl.template scores<F16>(lds + k_lds + x * 32 * D, [&](int s) { return q[s]; });
+                    if (tok[x] >= n) s4[x] = f32x4{0, 0, 0, 0};      // (whatever lies behind the row's end: not worth the careful pass)
                     sees[x] = n - tok[x] - 4 * g;
                 }
 #pragma unroll
@@ -1229,6 +1231,11 @@ __global__ __launch_bounds__(64 * W, 2) void k_block_attn_rows(BlockAttnArgs a) 
                             for (int x = 0; x < 2; ++x) s4[n][x] = kl.template scores<F16>(lds + k_lds + buf + x * 32 * D, [&](int s) { return q[n][s]; });
                         buf ^= 64 * D;
 #pragma unroll
+                        for (int x = 0; x < 2; ++x)                  // (whatever lies behind the rows' end: not worth the careful passes)
+                            if (rows[x] == 0 || tok[x] >= n_most)
+#pragma unroll
+                                for (int n = 0; n < NC; ++n) s4[n][x] = f32x4{0, 0, 0, 0};
+#pragma unroll
                         for (int x = 0; x < 2; ++x) {                // V that nobody, or not the careful row, may see
                             const bool none = rows[x] == 0 || (CAREFUL && !(rows[x] >> careful & 1));
                             if (none || tok[x] + 16 > v_len) f.drop_v(x, none ? 0 : v_len - tok[x], g);
@@ -1365,7 +1372,7 @@ int vox_rope_append(vox_ctx* ctx, void* stream, const vox_rope_append_args* a) {
     // 16 channels a thread: everything on 16 bytes, and no pair of eight across the border of what turns
     const bool vec = D % 16 == 0 && a->rot % 16 == 0 && (((size_t)a->q | (size_t)a->k | (size_t)a->v | (size_t)a->q_out | (a->rot ? (size_t)a->table : 0)) & 15) == 0 &&
                      a->q_stride % 8 == 0 && a->k_stride % 8 == 0 && a->v_stride % 8 == 0;
-    const bool with = vec && c.bounds && a->n_own == a->n_rows;      // the bounds in the same launch
+    const bool with = vec && c.bounds && a->n_own == a->n_rows && (int64_t)a->n_rows * c.kv_heads < 0x7fffffff;      // the bounds in the same launch
     int64_t blocks;
     if (vec) {
         if ((int64_t)a->n_rows * heads * (D / 16) >= APPEND_MANY && heads > 8) r.slots = 8;

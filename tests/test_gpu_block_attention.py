@@ -715,7 +715,7 @@ ATTEND_FORMS = [  # form, heads, kv heads, dim, page, block, top, kv lengths, ne
     (2, 60, 4, 128, 16, 16, 9, [240], [200]),
     (1, 72, 4, 64, 16, 16, 5, [150], [140]),                # 18 heads on a kv head
     (-16, 16, 2, 128, 128, 128, 32, [5000, 4200], [1, 1]),
-    (-5, 4, 4, 64, 64, 16, 100, [1700], [30]),
+    (-3, 4, 4, 64, 64, 16, 100, [1700], [30]),
     (-64, 1, 1, 64, 128, 128, 128, [17000], [1]),
     (1, 4, 4, 128, 32, 32, 32, [1100], [30]),
 ]

@@ -1328,7 +1328,9 @@ __global__ __launch_bounds__(256) void k_block_attn_merge(BlockAttnArgs a) {
 // ================================================================================================
 // entry points
 // ================================================================================================
-#define APPEND_MANY (1 << 18)             // 16-channel pieces of a call from which on threads go through several heads
+// 16-channel pieces of a call from which on threads go through several heads.  us in a captured graph, a slot a head / eight slots a row, 32 + 16 heads of 128: 64 rows 3.5 / 4.6,
+// 300 4.0 / 4.8, 700 (268800 pieces) 5.4 / 5.5, 1500 9.1 / 8.1, 4000 18.9 / 17.4; 16 + 16, 16384 rows 51.7 / 46.6.
+#define APPEND_MANY (1 << 18)
 #define BY_TYPE_AND_DIM(KERN, c) \
     ((c).dtype == VOX_DTYPE_F16 ? ((c).head_dim == 128 ? (const void*)KERN<1, 128> : (const void*)KERN<1, 64>) \
                                 : ((c).head_dim == 128 ? (const void*)KERN<0, 128> : (const void*)KERN<0, 64>))
@@ -1494,11 +1496,12 @@ static AttnShape attn_shape(const vox_block_attention_args* a, int cus) {
         }
     }
     const long tokens = (long)a->top * a->cache.block, blocks = (long)r.n_rows * a->cache.kv_heads * s.head_tiles;
+    // A row's list over several blocks of threads, one for each CU that has none, 256 tokens at least; a second launch joins them (some 3 us of host time, so not for 1024
+    // tokens, 11.4 / 9.4).  us in a captured graph, one block of threads a row / parts: 16 heads on 8 of 128, 1 row of 2048 tokens 19.4 / 10.2, 4 rows 25.8 / 16.7, 16 rows
+    // 39.1 / 36.5; 32 on 2, 1 row of 4096 28.4 / 9.6, 4 rows of 8192 57 / 16.6, 16 rows 92 / 35 (two for each CU: 40); 32 on 8 of 64, 8 rows of 2048 21.2 / 16.9.
     if (tokens > 1024) {
-        long z = (2L * cus + blocks - 1) / blocks;
-        const long most = (tokens + 255) / 256;
-        if (z > most) z = most;
-        s.splits = (int)(z < 1 ? 1 : z > 64 ? 64 : z);
+        const long z = (cus + blocks - 1) / blocks, most = (tokens + 255) / 256, parts = z < most ? z : most;
+        s.splits = (int)(parts < 1 ? 1 : parts > 64 ? 64 : parts);
     }
     return s;
 }

@@ -675,6 +675,9 @@ SELECT_FORMS = [  # form, heads, kv heads, dim, page, block, top, kv lengths, ne
     (1, 4, 4, 64, 128, 16, 33, [300], [190], 65537),                # more than eight rows' keys may be
     (1, 8, 8, 128, 128, 16, 20, [9000, 700], [40, 1], 9000),
     (1, 4, 4, 64, 64, 64, 5, [640, 130], [1, 1], 640),
+    (1, 16, 8, 128, 64, 16, 12, [9000, 8300], [17, 16], 9000),      # 513 to 4096 blocks, no CU left
+    (1, 16, 8, 64, 128, 16, 12, [700, 40], [17, 16], 65536),
+    (1, 16, 8, 64, 128, 16, 12, [66000, 40], [1, 32], 66000),       # more than 4096
     (-64, 4, 2, 128, 128, 16, 40, [20000, 16399], [1, 1], 524288),  # parts without a block among them
     (-5, 32, 2, 64, 128, 16, 17, [18000], [25], 18000),
 ]

@@ -618,7 +618,8 @@ __global__ __launch_bounds__(64 * W, QT == 16 ? 4 : 2) void k_block_select(Selec
             const u32* const key = keys + (size_t)r * a.stride;
             constexpr int GW = QT > 1 ? 1 : W;
 #define CHOOSE(KPL) choose<KPL, GW>(key, a.first, cand, need, a.first, a.last, mine, a.top, out, lane, wave, red)
-            if (cand <= 4 * 64 * GW) CHOOSE(4);
+            if (cand <= 2 * 64 * GW) CHOOSE(2);
+            else if (cand <= 4 * 64 * GW) CHOOSE(4);
             else if (cand <= 8 * 64 * GW) CHOOSE(8);
             else if (cand <= 16 * 64 * GW) CHOOSE(16);
             else if constexpr (QT == 1 || QT == 8) { if (cand <= 32 * 64 * GW) CHOOSE(32); else CHOOSE(64); }
@@ -1421,7 +1422,9 @@ static SelectShape select_shape(const vox_block_select_args* a) {
     SelectShape s{many && most <= 1024 ? 16 : many && most <= 4096 ? 8 : 1, 8, 1, 0};
     s.stride = most + (s.qt > 1 ? SEL_PAD : 0);
     if (s.qt > 1) return s;
-    s.W = most <= 512 ? 4 : 16;
+    // us in a captured graph, 4 / 8 / 16 waves a row: 32 rows of 512 blocks 14.0 / 13.6 / 15.9, 128 of 256 17.0 / 23.6 / 44, 64 of 1024 31.0 / 30.7 / 37.8, 64 of 1500 (dim 64) 30.4 / 26.9 /
+    // 37.1, 32 of 4096 71 / 58.9 / 57.8; beyond that the keys leave no room for the bounds on their way, and 16 waves take them to registers.
+    s.W = most <= 512 ? 4 : most <= 4096 ? 8 : 16;
     // One CU draws some 35 bytes a ns: a row's bounds over several CUs where there are CUs left and a row has more than 512 blocks.
     const int64_t pairs = (int64_t)r.n_rows * a->cache.kv_heads, z = pairs ? ATTN_CUS / pairs : 0, parts = (most + 255) / 256;
     if (most > 512 && z >= 2) s.splits = (int)(z < parts ? z : parts);
@@ -1459,12 +1462,13 @@ int vox_block_select(vox_ctx* ctx, void* stream, const vox_block_select_args* a)
 #define SELECT_OF(QT, W, SPLIT, NT) (c.dtype == VOX_DTYPE_F16 ? (c.head_dim == 128 ? (const void*)k_block_select<1, 128, QT, W, SPLIT, NT> : (const void*)k_block_select<1, 64, QT, W, SPLIT, NT>) \
                                                              : (c.head_dim == 128 ? (const void*)k_block_select<0, 128, QT, W, SPLIT, NT> : (const void*)k_block_select<0, 64, QT, W, SPLIT, NT>))
     if (z.splits > 1) {
-        VOX_TRY(launch(SELECT_OF(1, 4, true, 4), dim3((unsigned)grid), 256, lds + 16 * tile, (hipStream_t)stream, s));
+        VOX_TRY(launch(SELECT_OF(1, 4, true, 2), dim3((unsigned)grid), 256, lds + 8 * tile, (hipStream_t)stream, s));
         return launch((const void*)k_block_choose<16>, dim3((unsigned)(grid / z.splits)), 1024, 0, (hipStream_t)stream, s);
     }
     if (qt == 16) return launch(SELECT_OF(16, 8, false, 1), dim3((unsigned)grid), 512, lds + 8 * tile, (hipStream_t)stream, s);
     if (qt == 8) return launch(SELECT_OF(8, 8, false, 0), dim3((unsigned)grid), 512, lds, (hipStream_t)stream, s);
-    return W == 4 ? launch(SELECT_OF(1, 4, false, 4), dim3((unsigned)grid), 256, lds + 16 * tile, (hipStream_t)stream, s)
+    if (W == 8) return launch(SELECT_OF(1, 8, false, 2), dim3((unsigned)grid), 512, lds + 16 * tile, (hipStream_t)stream, s);
+    return W == 4 ? launch(SELECT_OF(1, 4, false, 2), dim3((unsigned)grid), 256, lds + 8 * tile, (hipStream_t)stream, s)
                   : launch(SELECT_OF(1, 16, false, 0), dim3((unsigned)grid), 1024, lds, (hipStream_t)stream, s);
 #undef SELECT_OF
 }

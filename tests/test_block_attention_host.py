@@ -145,3 +145,11 @@ def test_python_functions_refuse():
         B._bounds_of(kv, bounds.int(), steps)
     with pytest.raises(ValueError, match="out is"):
         B._out(torch.zeros(3, 4, 64), q.shape, torch.bfloat16, q.device)
+
+
+def test_bounds_and_steps_come_together():
+    kv = torch.zeros(2, 2, 32, 2, 64, dtype=torch.bfloat16)
+    bounds, steps = B.new_bounds(kv, 16)
+    for pair in ((bounds, None), (None, steps)):
+        with pytest.raises(ValueError, match="come together"):
+            B._bounds_of(kv, *pair)

@@ -604,6 +604,38 @@ def test_two_graphs_at_once(dev):
         N.lib().vox_graph_destroy(x[5])
 
 
+def test_graph_keeps_what_its_calls_made(dev):
+    """A run captured with int64 plans, q of heads that lie apart and results that only the next call takes: the graph's memory stays its own."""
+    from vox_serve_amd import _native as N
+    from vox_serve_amd import block_attention as B
+    hq, h, d, block, top = 8, 2, 64, 16, 6
+    s = Paged(dev, torch.bfloat16, h, d, 32, [700, 480], [1, 1], seed=8)
+    bounds, steps = s.bounds(block)
+    wide, k, v = s.rnd(2, hq, 2 * d), s.rnd(2, h, d), s.rnd(2, h, d)
+    cs, plan = table(dev, 1024, d // 2), [x.long() for x in s.plan]
+    where = (s.q_kvlen - 1).long(), s.row_page.long(), s.row_slot.long()
+
+    def run():
+        q = B.rope_append(wide[:, :, :d], k, v, s.kv, cs, *where, bounds=bounds, steps=steps, n_req=2)
+        return B.block_attention(q, s.kv, B.select_blocks(q, bounds, steps, *plan, block=block, top=top, max_kvlen=700, n_req=2), *plan, block=block, n_req=2)
+
+    want = run()
+    torch.cuda.synchronize()
+    with N.graph_capture() as cap:
+        got = run()
+    with torch.cuda.stream(N._capture_streams[torch.cuda.current_device()]):      # what this stream let go of would be handed out again here
+        others = [torch.full((n,), 3, dtype=torch.int32, device=dev) for n in (2, 3, 12, 24, 100, 128, 512, 1024) for _ in range(8)]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        got.zero_()
+        N.check(N.lib().vox_graph_launch(cap.graph, N.stream()))
+        torch.cuda.synchronize()
+        assert torch.equal(got, want) and all(bool((x == 3).all()) for x in others)
+        for x in others:
+            x.fill_(3)
+    N.lib().vox_graph_destroy(cap.graph)
+
+
 def test_results_do_not_depend_on_the_batch(dev):
     """The choice and the appended rows of a request are the same alone and among others."""
     from vox_serve_amd import block_attention as B

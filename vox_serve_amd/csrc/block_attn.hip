@@ -618,11 +618,13 @@ __global__ __launch_bounds__(64 * W, QT == 16 ? 4 : 2) void k_block_select(Selec
             const u32* const key = keys + (size_t)r * a.stride;
             constexpr int GW = QT > 1 ? 1 : W;
 #define CHOOSE(KPL) choose<KPL, GW>(key, a.first, cand, need, a.first, a.last, mine, a.top, out, lane, wave, red)
-            if (cand <= 2 * 64 * GW) CHOOSE(2);
-            else if (cand <= 4 * 64 * GW) CHOOSE(4);
-            else if (cand <= 8 * 64 * GW) CHOOSE(8);
-            else if (cand <= 16 * 64 * GW) CHOOSE(16);
-            else if constexpr (QT == 1 || QT == 8) { if (cand <= 32 * 64 * GW) CHOOSE(32); else CHOOSE(64); }
+            constexpr int MOST = QT == 16 ? 16 : QT == 8 ? 64 : W == 4 ? 2 : W == 8 ? 8 : 32;      // by 64 GW: the blocks that the launch was chosen for
+            if (cand <= 2 * 64 * GW) { CHOOSE(2); continue; }
+            if constexpr (MOST > 2) if (cand <= 4 * 64 * GW) { CHOOSE(4); continue; }
+            if constexpr (MOST > 4) if (cand <= 8 * 64 * GW) { CHOOSE(8); continue; }
+            if constexpr (MOST > 8) if (cand <= 16 * 64 * GW) { CHOOSE(16); continue; }
+            if constexpr (MOST > 16) if (cand <= 32 * 64 * GW) { CHOOSE(32); continue; }
+            if constexpr (MOST > 32) CHOOSE(64);
 #undef CHOOSE
         }
         __syncthreads();

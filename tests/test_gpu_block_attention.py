@@ -932,3 +932,24 @@ def test_select_takes_nothing_but_the_ends(dev):
     out = torch.full((s.n, 8, 5), 9, dtype=torch.int32, device=dev)
     B.select_blocks(q, bounds, steps, *s.plan, block=16, top=5, max_kvlen=0, out=out)
     assert (out == 9).all()
+
+
+@pytest.mark.parametrize("alike", [0, 1, 5, 40])
+@pytest.mark.parametrize("top", [4, 40, 70, 99, 130])
+def test_rows_together_choose_among_many(dev, top, alike):
+    """Few and many of 130 to 900 blocks, all different, all the same, or of a few kinds: what a wave narrows its search to fits its lanes or does not."""
+    from vox_serve_amd import block_attention as B
+    hq, h, d, block = 4, 4, 64, 16
+    s = Paged(dev, torch.bfloat16, h, d, 32, [14400, 4500, 2150], [170, 30, 30], seed=top + alike)
+    assert select_form(s, hq, block, top, 14400, 3) == 16
+    if alike:                                                # every block of a page and a kind holds the same keys
+        kinds = s.rnd(alike, h, d)
+        s.kv[:, 0] = kinds[torch.arange(s.kv.shape[0], device=dev) % alike][:, None]
+    q, (bounds, steps), pages = s.rnd(s.n, hq, d), B.new_bounds(s.kv, block), torch.arange(s.kv.shape[0], device=dev)
+    B.update_bounds(s.kv, bounds, steps, pages.repeat_interleave(2), torch.tensor([15, 31], device=dev).repeat(s.kv.shape[0]))
+    got = B.select_blocks(q, bounds, steps, *s.plan, block=block, top=top, max_kvlen=14400, n_req=3).cpu().numpy()
+    nb, ns = bounds.cpu().numpy(), steps.cpu().numpy()
+    for i in [0, 169, 170, 199, 200, 229]:
+        assert np.array_equal(got[i], R.select(f64(q[i]), nb, ns, s.pages[s.req[i]], s.kvlen[i], block, top, 1, 2)), i
+    one = torch.cat([B.select_blocks(q[i:i + 1], bounds, steps, s.q_req[i:i + 1], s.q_kvlen[i:i + 1], s.indptr, s.indices, block=block, top=top, max_kvlen=14400) for i in range(s.n)])
+    assert np.array_equal(got, one.cpu().numpy())

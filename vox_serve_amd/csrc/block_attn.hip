@@ -65,6 +65,11 @@ __device__ __forceinline__ u32 tile_place(int row, int chunk) {      // byte of 
 }
 __device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
+// n and the bits of m below the lane's own
+__device__ __forceinline__ int lanes_below(unsigned long long m, int n) {
+    return (int)__builtin_amdgcn_mbcnt_hi((u32)(m >> 32), __builtin_amdgcn_mbcnt_lo((u32)m, (u32)n));
+}
+
 // Rows ra, ra + 1, .. of a tile that belong to one request (a lane has its row's request, -1: passed over): one past the last, and the most tokens one of them sees
 __device__ __forceinline__ int run_of(int my_req, int my_len, int ra, int R, int lane, int req, int& n_most) {
     const unsigned long long same = __ballot(lane < R && my_req == req) >> ra;
@@ -210,6 +215,8 @@ __device__ __forceinline__ void block_bounds(int lane, const bf16_t* keys, size_
 // Vectors: a thread has 16 channels of a head that turn (two runs of eight whose pairs they are: halves, or 16 in a row: neighbours) or do not, and goes through the
 // row's heads slot, slot + slots, ..: the angles are loaded once.  Calls of few rows take a slot a head (everything in flight at once), calls of many rows eight
 // slots a row (the angles, 64 bytes a thread, would be as much to load as the channels).
+// Bound by memory: 16384 rows of 32 + 2 x 8 heads of 128 are 411 MB with their angles, 75 us (5.5 TB/s: requests share angles), their bounds 14 us more;
+// 48 rows 7 us, one row 2.3, the launch.
 // With rows of different requests the launch has more blocks of threads behind these: a wave a row and kv head, which leaves at once unless the row
 // completes a block; the other keys of the block are in the cache from earlier calls, the row's own is turned here once more.
 template <int F16, int IL, int D>        // D: 64 or 128 with bounds, else 0 (any)
@@ -306,7 +313,8 @@ struct BoundsArgs {
     const int *page, *slot;
     int n_rows, n_pages, page_size, block, Hkv;
 };
-// 64 rows and a kv head a block of threads; its waves share the rows that complete a block (blocks of 16: one each)
+// 64 rows and a kv head a block of threads; its waves share the rows that complete a block (blocks of 16: one each).  16384 rows' 256 blocks of 64 and 8 kv heads, 34 MB: 14 us, some 7 of
+// them at the memory's rate; a wave has its block's keys in flight 32 at a time.
 template <int F16, int D>
 __global__ __launch_bounds__(256) void k_block_bounds(BoundsArgs a) {
     const int n = blockIdx.x * 64 + (threadIdx.x & 63), h = blockIdx.y, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -352,11 +360,15 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 // whole numbers however many heads there are.  P and N have up to 13 bits; 64 times their high part and their low six bits are two rows of an 8-bit matrix
 // product, so 16 rows of it are 8 query rows, and 16 blocks its columns: C's lanes have both rows of a query beside each other.
 // A tile of 16 (or 8) query rows reads the bounds of a request's blocks once; what a choice costs is its rounds over the keys, in a wave's registers.
-// The keys of all candidates lie in LDS: [row][SEL_STRIDE(blocks)].
+// The keys of all candidates lie in LDS: [row][stride].
+// 4096 rows of a request, 16 heads on 8 of 128, 512 blocks each: 63 us, floor 7 (the product, far from what bounds it).  With
+// one part left out at a time: choosing 27 us, products and the 268 MB of bounds on their way 13, q to matrix rows 8 (16 with eight lanes to a bank and one
+// address for a row's maximum), the rest 18: a chain of row, pages, steps and bounds, with two blocks of threads a CU to hide it.
+// One row of 2048 blocks of 2 kv heads: 5.7 us for its scores over 16 blocks of threads, 6.5 to choose; 32 rows of 512 blocks and 8 kv heads 12 us, floor 5.5.
 #define SEL_PAD 8
 // keys of one row, a wave's or W waves' (W > 1: all threads call): the need largest, older first where equal, written in order of their index
 template <int KPL, int W>
-__device__ __forceinline__ void choose(const u32* key, int lo, int cand, int need, int first, int last, int have, int top, int* out, int lane, int wave, int (*red)[16]) {
+__device__ __forceinline__ void choose(u32* key, int lo, int cand, int need, int first, int last, int have, int top, int* out, int lane, int wave, int (*red)[16]) {
     u32 k[KPL];
     const int c0 = W > 1 ? wave * KPL * 64 : 0;
     u32 least = 0xffffffffu, most = 0;
@@ -394,6 +406,68 @@ __device__ __forceinline__ void choose(const u32* key, int lo, int cand, int nee
     }
     u32 a = least, t = least;
     unsigned long long b = (unsigned long long)most + 1;
+    // A wave with many keys looks at the largest of each 128th of them first: what `need` of those reach, at least `need` keys reach, and few more (of 512 keys and 29
+    // some 40).  These keys move together, and the search goes on over one or two a lane: 4096 rows of 512 blocks 63 us, 75 with every round over all keys.
+    if constexpr (W == 1 && KPL >= 4) {
+        constexpr int R = KPL >= 8 ? 2 : 1;                          // keys a lane that the row has room for, beside their indexes
+        if (need > 0 && need <= 48 * R) {
+            u32 m[2] = {k[0], k[1]};
+#pragma unroll
+            for (int i = 2; i < KPL; ++i) m[i & 1] = max(m[i & 1], k[i]);
+            unsigned long long hi = b;
+            for (int n = 128; n > need + 8 && hi - a > 1;) {
+                const u32 mid = a + (u32)((hi - a) >> 1);
+                const int reach = (int)__popcll(__ballot(m[0] >= mid)) + (int)__popcll(__ballot(m[1] >= mid));
+                if (reach >= need) { a = mid; n = reach; } else hi = mid;
+            }
+            // (a = 0: lanes outside reach it)
+            u32* const row = key + lo;                               // (the keys are in registers: their row is free)
+            int total = 0;
+            if (a > 0)
+#pragma unroll
+                for (int i = 0; i < KPL; ++i) {
+                    const unsigned long long r = __ballot(k[i] >= a);
+                    const int to = lanes_below(r, total);
+                    if (k[i] >= a && to < 64 * R) { row[to] = k[i]; row[64 * R + to] = (u32)(lo + i * 64 + lane); }
+                    total += (int)__popcll(r);
+                }
+            asm volatile("" ::: "memory");                           // (a wave's LDS instructions are in order)
+            auto rest = [&](auto regs) {
+                constexpr int N = decltype(regs)::value;
+                u32 x[N], index[N];
+#pragma unroll
+                for (int i = 0; i < N; ++i) { x[i] = 64 * i + lane < total ? row[64 * i + lane] : 0; index[i] = row[64 * R + 64 * i + lane]; }
+                bool exact = total == need;
+                while (!exact && b - a > 1) {
+                    const u32 mid = a + (u32)((b - a) >> 1);
+                    int n = 0;
+#pragma unroll
+                    for (int i = 0; i < N; ++i) n += (int)__popcll(__ballot(x[i] >= mid));
+                    if (n >= need) a = mid; else b = mid;
+                    exact = n == need;
+                }
+                int gt = 0;
+#pragma unroll
+                for (int i = 0; i < N; ++i) gt += (int)__popcll(__ballot(exact ? x[i] >= a : x[i] > a));
+                int ties = need - gt, to = first;
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const bool e = x[i] == a && !exact, g = exact ? x[i] >= a : x[i] > a;
+                    const unsigned long long be = __ballot(e);
+                    const bool take = g || (e && lanes_below(be, 0) < ties);
+                    const unsigned long long bt = __ballot(take);
+                    if (take) out[lanes_below(bt, to)] = (int)index[i];
+                    to += (int)__popcll(bt);
+                    ties -= min(ties, (int)__popcll(be));
+                }
+                for (int j = lane; j < first; j += 64) out[j] = j;
+                for (int j = lane; j < last; j += 64) out[top - last + j] = have - last + j;
+            };
+            if (total >= need && total <= 64) return rest(std::integral_constant<int, 1>{});
+            if constexpr (R == 2) if (total >= need && total <= 128) return rest(std::integral_constant<int, 2>{});
+            t = a;
+        }
+    }
     bool exact = need == 0;                                          // exactly `need` keys reach t: no ties to break
     while (!exact && b - a > 1) {
         if constexpr (W > 1) {
@@ -445,7 +519,6 @@ __device__ __forceinline__ void choose(const u32* key, int lo, int cand, int nee
         }
     }
     int ties = exact ? 0 : need - gt_all;                            // equal ones to take, from the oldest
-    const unsigned long long below = lane ? ~0ull >> (64 - lane) : 0ull;
     int at = first + gt_before + min(eq_before, ties);
     ties = max(ties - eq_before, 0);
 #pragma unroll
@@ -453,9 +526,9 @@ __device__ __forceinline__ void choose(const u32* key, int lo, int cand, int nee
         if (c0 + i * 64 >= cand || need == 0) break;
         const bool in = c0 + i * 64 + lane < cand, e = in && !exact && k[i] == t, g = in && (exact ? k[i] >= t : k[i] > t);
         const unsigned long long be = __ballot(e);
-        const bool take = g || (e && (int)__popcll(be & below) < ties);
+        const bool take = g || (e && lanes_below(be, 0) < ties);
         const unsigned long long bt = __ballot(take);
-        if (take) out[at + (int)__popcll(bt & below)] = lo + c0 + i * 64 + lane;
+        if (take) out[lanes_below(bt, at)] = lo + c0 + i * 64 + lane;
         at += (int)__popcll(bt);
         ties -= min(ties, (int)__popcll(be));
     }
@@ -490,6 +563,24 @@ __global__ __launch_bounds__(64 * W, QT == 16 ? 4 : 2) void k_block_select(Selec
         s_len[tid] = n; s_req[tid] = r;
         s_amax[tid] = 0;
     }
+    // The first row's pages, steps and first tile of bounds: asked for here, a link of the chain before each barrier that waits for the memory anyway.
+    const int e_req = a.q_req[i0];
+    const bool early = a.q_kvlen[i0] > 0 && e_req >= 0 && e_req < a.n_req && a.max_kvlen > 0;
+    const int e_p0 = early ? a.indptr[e_req] : 0, e_np = early ? a.indptr[e_req + 1] - e_p0 : 0;
+    auto page_of = [&](int j, int& pj, int p0, int np) {
+        pj = a.per_magic ? (int)__umulhi((u32)j, a.per_magic) : j;
+        const int pg = pj < np ? a.indices[p0 + pj] : -1;
+        return pg;
+    };
+    auto block_of = [&](int j, int pj, int pg, float& step) {
+        const bool ok = pg >= 0 && pg < a.n_pages;
+        const u32 at = ok ? ((u32)pg * a.Hkv + h) * per + (j - pj * per) : 0;
+        step = ok ? a.steps[at] : __uint_as_float(0x7fc00000u);      // (NaN: a block without a page)
+        return at;
+    };
+    const int e_j = a.first + (split * W + wave) * 64 + lane;
+    int e_pj;
+    const int e_pg = page_of(e_j, e_pj, e_p0, e_np);
     for (int x = tid; x < QT * D; x += 64 * W) keys[x] = 0;
     if constexpr (QT < 8) for (int x = tid; x < (MT * 16 - 2 * QT) * 2 * D / 4; x += 64 * W) reinterpret_cast<int*>(s_a[2 * QT])[x] = 0;
     // P and N of the rows: eight channels of a head a thread
@@ -501,15 +592,35 @@ __global__ __launch_bounds__(64 * W, QT == 16 ? 4 : 2) void k_block_select(Selec
     };
     const uint4 mine = tid < R * chunks ? piece(tid) : make_uint4(0, 0, 0, 0);
     __syncthreads();
+    float e_step;
+    const u32 e_at = block_of(e_j, e_pj, e_pg, e_step);
     for (int it = tid; it < R * chunks; it += 64 * W) {
         const uint4 x = it == tid ? mine : piece(it);
         const u32 w[4] = {x.x, x.y, x.z, x.w};
         float amax = 0.0f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) amax = fmaxf(amax, finite_abs(elem_f<F16>((bf16_t)(w[e / 2] >> (16 * (e % 2))))));
-        atomicMax(&s_amax[it / chunks], __float_as_uint(amax));
+        u32 most = __float_as_uint(amax);                            // (pieces of a row come in eights: one of them writes)
+        most = max(most, (u32)__builtin_amdgcn_update_dpp((int)most, (int)most, 0xB1, 0xF, 0xF, false));       // lane ^ 1
+        most = max(most, (u32)__builtin_amdgcn_update_dpp((int)most, (int)most, 0x4E, 0xF, 0xF, false));       // lane ^ 2
+        most = max(most, (u32)__builtin_amdgcn_update_dpp((int)most, (int)most, 0x141, 0xF, 0xF, false));      // lane ^ 7
+        if (lane % 8 == 0) atomicMax(&s_amax[it / chunks], most);
     }
     __syncthreads();
+    const u32 stage_at = a.stage_at + wave * NT * 32 * D, stage0 = (u32)(size_t)(__attribute__((address_space(3))) u32*)keys + stage_at, place = tile_place<D>(c, g);
+    const char* const stage = reinterpret_cast<const char*>(keys) + stage_at;
+    auto fetch = [&](int u0, u32 at) {                               // NT tiles of a step's four, from u0 on
+        constexpr int LPR = D / 8, PIECES = 32 * D / 1024;           // lanes a row, loads a tile
+#pragma unroll
+        for (int u = 0; u < NT; ++u)
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) {
+                const int row = i * (64 / LPR) + lane / LPR, chunk = lane % LPR ^ (D == 128 ? row : row >> 1 & 7);      // (what tile_place puts at this lane's position)
+                const u32 from = (u32)__shfl((int)at, 16 * (u0 + u) + row, 64);
+                lds_dma16(a.bounds + (size_t)from * (2 * D) + 16 * chunk, stage0 + (u32)(u * 32 * D + i * 1024));
+            }
+    };
+    if constexpr (NT > 0) fetch(0, e_at);
     for (int it = tid; it < R * chunks; it += 64 * W) {
         const uint4 x = it == tid ? mine : piece(it);
         const u32 w[4] = {x.x, x.y, x.z, x.w};
@@ -518,12 +629,14 @@ __global__ __launch_bounds__(64 * W, QT == 16 ? 4 : 2) void k_block_select(Selec
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const int s = q_steps(elem_f<F16>((bf16_t)(w[e / 2] >> (16 * (e % 2)))), inv);
-            atomicAdd(&keys[r * D + d + e], s >= 0 ? (u32)s : (u32)-s << 16);
+            atomicAdd(&keys[r * D + (e * (D / 8) + d / 8 + 16 * r) % D], s >= 0 ? (u32)s : (u32)-s << 16);      // (neighbouring lanes and rows on banks of their own)
         }
     }
     __syncthreads();
     for (int x = tid; x < R * D; x += 64 * W) {
-        const int r = x / D, d = x % D, p = (int)(keys[x] & 0xffffu), m = -(int)(keys[x] >> 16);
+        const int r = x / D, d = x % D;
+        const u32 both = keys[r * D + (d % 8 * (D / 8) + d / 8 + 16 * r) % D];
+        const int p = (int)(both & 0xffffu), m = -(int)(both >> 16);
         s_a[2 * r][d] = (int8_t)(p & 63); s_a[2 * r + 1][d] = (int8_t)(p >> 6);
         s_a[2 * r][D + d] = (int8_t)(m & 63); s_a[2 * r + 1][D + d] = (int8_t)(m >> 6);
     }
@@ -534,13 +647,12 @@ __global__ __launch_bounds__(64 * W, QT == 16 ? 4 : 2) void k_block_select(Selec
 #pragma unroll
         for (int s = 0; s < KS; ++s) av[t][s] = *reinterpret_cast<const i32x4*>(&s_a[16 * t + c][64 * s + 16 * g]);
 
-    const u32 stage_at = a.stage_at + wave * NT * 32 * D, stage0 = (u32)(size_t)(__attribute__((address_space(3))) u32*)keys + stage_at, place = tile_place<D>(c, g);
-    const char* const stage = reinterpret_cast<const char*>(keys) + stage_at;
+    if constexpr (NT > 0) dma_wait();                                // (also where no step follows: nothing may be on its way to LDS that is let go of)
     const int my_req = lane < R ? s_req[lane] : -1, my_len = lane < R ? s_len[lane] : 0;
     for (int ra = 0; ra < R;) {
         const int req = __builtin_amdgcn_readlane(my_req, ra);
         if (req < 0) { ++ra; continue; }
-        const int p0 = a.indptr[req], np = a.indptr[req + 1] - p0;
+        const int p0 = early && ra == 0 ? e_p0 : a.indptr[req], np = early && ra == 0 ? e_np : a.indptr[req + 1] - p0;
         int n_most;
         int rb = 1;
         if constexpr (QT == 1) n_most = __builtin_amdgcn_readfirstlane(my_len);
@@ -549,12 +661,14 @@ __global__ __launch_bounds__(64 * W, QT == 16 ? 4 : 2) void k_block_select(Selec
         // 64 blocks a step: a lane looks up one of them, four tiles of 16 go through the product
         u32* const dst0 = SPLIT ? a.keys + ((size_t)i0 * a.Hkv + h) * a.stride : keys;
         for (int j0 = a.first + (split * W + wave) * 64; j0 < j1; j0 += (SPLIT ? a.splits : 1) * W * 64) {
-            const int j = j0 + lane, pj = a.per_magic ? (int)__umulhi((u32)j, a.per_magic) : j;
-            int pg = -1;
-            if (j < j1 && pj < np) pg = a.indices[p0 + pj];
-            const bool ok = pg >= 0 && pg < a.n_pages;
-            const u32 at = ok ? ((u32)pg * a.Hkv + h) * per + (j - pj * per) : 0;
-            const float step = ok ? a.steps[at] : __uint_as_float(0x7fc00000u);      // (NaN: a block without a page)
+            u32 at = e_at;
+            float step = e_step;
+            const bool ready = early && ra == 0 && j0 == a.first + (split * W + wave) * 64;
+            if (!ready) {
+                int pj;
+                const int j = j0 + lane, pg = page_of(j, pj, p0, np);
+                at = block_of(j, pj, pg, step);
+            }
             auto score = [&](int u, const i32x4 (&b)[KS]) {
                 const float st = __shfl(step, 16 * u + c, 64);
 #pragma unroll
@@ -570,18 +684,10 @@ __global__ __launch_bounds__(64 * W, QT == 16 ? 4 : 2) void k_block_select(Selec
                 }
             };
             if constexpr (NT > 0) {
-                constexpr int LPR = D / 8, PIECES = 32 * D / 1024;   // lanes a row, loads a tile
 #pragma unroll
                 for (int u0 = 0; u0 < 4; u0 += NT) {
                     if (j0 + 16 * u0 >= j1) break;
-#pragma unroll
-                    for (int u = 0; u < NT; ++u)
-#pragma unroll
-                        for (int i = 0; i < PIECES; ++i) {
-                            const int row = i * (64 / LPR) + lane / LPR, chunk = lane % LPR ^ (D == 128 ? row : row >> 1 & 7);      // (what tile_place puts at this lane's position)
-                            const u32 from = (u32)__shfl((int)at, 16 * (u0 + u) + row, 64);
-                            lds_dma16(a.bounds + (size_t)from * (2 * D) + 16 * chunk, stage0 + (u32)(u * 32 * D + i * 1024));
-                        }
+                    if (u0 || !ready) fetch(u0, at);
                     dma_wait();
 #pragma unroll
                     for (int u = 0; u < NT; ++u) {
@@ -615,7 +721,7 @@ __global__ __launch_bounds__(64 * W, QT == 16 ? 4 : 2) void k_block_select(Selec
                 for (int j = QT > 1 ? lane : tid; j < a.top; j += QT > 1 ? 64 : 64 * W) out[j] = j < mine ? j : -1;
                 continue;
             }
-            const u32* const key = keys + (size_t)r * a.stride;
+            u32* const key = keys + (size_t)r * a.stride;
             constexpr int GW = QT > 1 ? 1 : W;
 #define CHOOSE(KPL) choose<KPL, GW>(key, a.first, cand, need, a.first, a.last, mine, a.top, out, lane, wave, red)
             constexpr int MOST = QT == 16 ? 16 : QT == 8 ? 64 : W == 4 ? 2 : W == 8 ? 8 : 32;      // by 64 GW: the blocks that the launch was chosen for
@@ -641,7 +747,7 @@ __global__ __launch_bounds__(64 * W) void k_block_choose(SelectArgs a) {
     if (n <= 0 || req < 0 || req >= a.n_req || a.max_kvlen <= 0) return;
     n = min(n, a.max_kvlen);
     int* const out = a.blocks + (size_t)blockIdx.x * a.top;
-    const u32* const key = a.keys + (size_t)blockIdx.x * a.stride;
+    u32* const key = a.keys + (size_t)blockIdx.x * a.stride;
     const int mine = (n - 1) / a.block + 1, cand = mine - a.first - a.last, need = a.top - a.first - a.last;
     if (mine <= a.top) {
         for (int j = tid; j < a.top; j += 64 * W) out[j] = j < mine ? j : -1;
@@ -669,6 +775,10 @@ __global__ __launch_bounds__(64 * W) void k_block_choose(SelectArgs a) {
 // What a column must not see is kept from it by its score alone (weight 0), which holds as long as V is finite; where a result is not, the rows are gone through
 // again one by one in the same order with V's masked tokens as zero, and a value that is not finite multiplied by the weight as one term (an infinity times the
 // two terms would be inf - inf).  Rows that see no such value come out bit for bit as if it were not there.
+// What bounds it, and measured (bf16, dim 128, unless said): 64 rows of 2048 tokens, 32 heads on 8 of 64, fp16: 50 us for 268 MB, 5.4 TB/s - the memory.  4 rows of 8192, 32 heads on 2:
+// 9.6 us in 64 parts and 3.9 to join them, 34 MB - the launches and one pass of latency.  A row of 512 tokens, 16 heads on 8: 7.9 us, chain of list, pages, K, V alone.
+// A chunk of 1024 rows of 2048 tokens, 16 heads on 8: 125 us, 17 GFLOP (26 with the weights' second term): tiles of 16 rows meet all that any of them lists, some
+// 3.5 times one row's list, and a tile's tokens are masked, weighed and moved by vector instructions for 32 columns only.
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef half_t f16x8 __attribute__((ext_vector_type(8)));
@@ -1289,7 +1399,8 @@ __global__ __launch_bounds__(64 * W, 2) void k_block_attn_rows(BlockAttnArgs a) 
     }
 }
 
-// the splits of a row and head, a block of threads each: four channels a thread, the splits over the groups of D / 4 threads
+// the splits of a row and head, a block of threads each: four channels a thread, the splits over the groups of D / 4 threads, all loads on their way at once (128 rows and heads
+// of 64 splits: 3.9 us, 4.3 MB; a launch of nothing is 2)
 template <int F16, int D>
 __global__ __launch_bounds__(256) void k_block_attn_merge(BlockAttnArgs a) {
     constexpr int LPD = D / 4, GROUPS = 256 / LPD, MOST = 64 / GROUPS;
@@ -1417,10 +1528,12 @@ struct SelectShape { int qt, W, splits, stride; };
 static SelectShape select_shape(const vox_block_select_args* a) {
     const vox_block_rows& r = a->rows;
     const int most = (int)(((int64_t)r.max_kvlen + a->cache.block - 1) / a->cache.block);
-    // rows a tile: 16 while their keys take half a CU's LDS, 8 while they take most of it (4096 blocks), else (and for rows of different requests) one
-    // where there are enough of them: us, a row / 16 rows together, 256 blocks: 16 heads on 8 of 128, 64 rows (512 blocks of threads) 12.2 / 14.6, 128 20.8 / 15.0; 32 on 8,
-    // 64 rows 12.0 / 16.1, 128 20.2 / 16.0; 32 on 2, 128 rows (256) 11.2 / 21.5, 512 20.9 / 21.9; 8 on 8 of 64, 128 rows 12.3 / 13.4, 512 38.4 / 13.6.
-    const bool many = r.n_own > 0 && r.n_rows >= 2 * (int64_t)r.n_own && (int64_t)r.n_rows * a->cache.kv_heads >= 640 + 32 * (r.heads / a->cache.kv_heads);
+    // rows a tile: 16 while their keys take half a CU's LDS, 8 while they take most of it (4096 blocks), else (and for rows of different requests) one; together only
+    // where there are enough of them, the more the more channels a row has to bring to matrix rows first.  us in a captured graph, a row / 16 rows together, 256 blocks, for
+    // 64, 128, 256 and 512 rows: 16 heads on 8 of 128 10.6 / 12.3, 13.6 / 12.8, 21 / 13, 37 / 13.3; 32 on 8 10 / 13.6, 12.5 / 13.7, 21.5 / 13.8, 37 / 14.3; 32 on 2 8.8 / 19.4,
+    // 8.8 / 19.8, 10.3 / 19.9, 14.1 / 20; 8 on 8 of 64 9.7 / 11.3, 10.6 / 11.3, 15.2 / 11.4, 25.2 / 11.8.
+    const int G = r.heads / a->cache.kv_heads;
+    const bool many = r.n_own > 0 && r.n_rows >= 2 * (int64_t)r.n_own && (int64_t)r.n_rows * a->cache.kv_heads >= 576 + G * a->cache.head_dim / 2;
     SelectShape s{many && most <= 1024 ? 16 : many && most <= 4096 ? 8 : 1, 8, 1, 0};
     s.stride = most + (s.qt > 1 ? SEL_PAD : 0);
     if (s.qt > 1) return s;

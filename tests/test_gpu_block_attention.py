@@ -749,6 +749,9 @@ ATTEND_FORMS = [  # form, heads, kv heads, dim, page, block, top, kv lengths, ne
     (2, 64, 4, 64, 32, 32, 4, [300, 33], [160, 33]),
     (2, 60, 4, 128, 16, 16, 9, [240], [200]),
     (1, 72, 4, 64, 16, 16, 5, [150], [140]),                # 18 heads on a kv head
+    (16, 64, 32, 64, 32, 16, 4, [130, 60], [90, 60]),       # more tiles than CUs
+    (16, 32, 32, 128, 16, 16, 4, [130, 60], [90, 60]),
+    (16, 16, 8, 128, 16, 16, 200, [4000], [210]),           # lists that leave no room for eight waves' keys
     (-16, 16, 2, 128, 128, 128, 32, [5000, 4200], [1, 1]),
     (-3, 4, 4, 64, 64, 16, 100, [1700], [30]),
     (-64, 1, 1, 64, 128, 128, 128, [17000], [1]),
@@ -779,7 +782,7 @@ def test_attention_of_every_form(dev, dtype, form, hq, h, d, page, block, top, k
     assert torch.equal(out, got)
 
 
-@pytest.mark.parametrize("hq,h,d", [(16, 8, 128), (8, 8, 64), (28, 4, 64)])
+@pytest.mark.parametrize("hq,h,d", [(16, 8, 128), (8, 8, 64), (28, 4, 64), (64, 32, 64)])
 def test_rows_together_masked_places(dev, hq, h, d):
     """As test_attention_masked_places, where rows of a chunk share a launch's blocks: what one row may not see, or does not list, and another does, reaches the
     other alone, bit for bit."""

@@ -1597,20 +1597,25 @@ static int check_attention(const vox_block_attention_args* a) {
     return VOX_OK;
 }
 // How a call's rows are laid out: rows a tile, and the parts that a row's list is split into.
-struct AttnShape { int tiles, per_tile, splits, head_tiles; };      // tiles of columns (0: a row a block of threads), rows a block, ..
+struct AttnShape { int tiles, per_tile, splits, head_tiles, W; };      // tiles of columns (0: a row a block of threads), rows a block, .., waves
 static AttnShape attn_shape(const vox_block_attention_args* a, int cus) {
     const vox_block_rows& r = a->rows;
     const int G = r.heads / a->cache.kv_heads;
-    AttnShape s{0, 1, 1, (G + 15) / 16};
-    // Rows together pay once there are enough of them: a tile's blocks of threads go through what all its rows list, some 1.7 us for 128 tokens however few there are, a
-    // row's through its own list, 15 to the us once the card is full.  What R neighbouring rows list between them is some R^0.45 lists.  us, a row / rows together, lists
-    // of 2048 tokens: 16 heads on 8 of 128, 64 rows (512 blocks of threads) 40 / 104, 128 70 / 102, 512 247 / 101; 32 on 8, 64 rows 38 / 72, 128 69 / 71,
-    // 512 242 / 88; 32 on 2, 128 rows (256) 33 / 45, 512 72 / 57; 14 on 2 of 64, 128 rows 24 / 42, 512 51 / 43; 8 on 8 of 64, 128 rows 50 / 75, 512 174 / 76.
+    AttnShape s{0, 1, 1, (G + 15) / 16, 8};
+    // Rows together pay once there are enough of them: a tile's block of threads goes through what all its rows list, however few of them there are, a row's through its own list, 15 to
+    // the us once the card is full; what R neighbouring rows list between them is some R^0.4 lists.  us, a row / rows together, lists of 2048 tokens, for 96, 128, 192 and 512 rows: 16 heads on
+    // 8 of 128 55 / 74, 70 / 73, 98 / 74, 242 / 77; 32 on 8 51 / 56, 65 / 56, 94 / 57, 235 / 93; 8 on 8 of 64 38 / 55, 49 / 54, 70 / 56, 175 / 58; 14 on 2 of 64 24 / 35, 19 / 35, 28 / 36,
+    // 52 / 37; 32 on 2 of 128, 256 rows 38 / 40, 384 53 / 57, 512 70 / 60.
+    // Eight waves a tile while that is a block of threads a CU, four where there are two (4 / 8 waves: 16 heads on 8, 512 rows 102 / 77, 1024 141 / 151; 8 on 8 of 64, 700 rows 66 / 70).
     if (r.n_own > 0 && r.n_rows >= 2 * (int64_t)r.n_own && G <= 16) {
         const int tiles = G > 1 ? 2 : 1, per_tile = tiles * (16 / G);
-        if ((double)r.n_rows * a->cache.kv_heads >= 470.0 * pow(per_tile, 0.45)) {
+        const bool room = a->cache.head_dim == 64 || (int64_t)a->top * per_tile <= 2048;      // (eight waves' K at dim 128 are 128 of a CU's 160 KB, their lists 8 KB and 8 bytes an entry)
+        const int waves = room && ((int64_t)r.n_rows + per_tile - 1) / per_tile * a->cache.kv_heads <= cus ? 8 : 4;
+        const double pairs = waves == 8 ? 430.0 * pow(per_tile, 0.34) : 470.0 * pow(per_tile, 0.45);
+        if ((double)r.n_rows * a->cache.kv_heads >= pairs) {
             s.tiles = tiles;
             s.per_tile = per_tile;
+            s.W = waves;
             return s;
         }
     }
@@ -1650,7 +1655,7 @@ int vox_block_attention(vox_ctx* ctx, void* stream, const vox_block_attention_ar
     if (!(fabsf(a->scale) < 3e38f)) return vox_fail(VOX_ERR_INVALID, "block_attention: the scale is not finite");
     const bool one = z.tiles == 0;
     const float scale2 = fabsf(a->scale) * 1.44269504088896340736f;
-    const int W = one ? 8 : 4, G = r.heads / c.kv_heads, cols = one && G < 16 ? G : 16;
+    const int W = z.W, G = r.heads / c.kv_heads, cols = one && G < 16 ? G : 16;
     const bool big = a->top > 64;
     const size_t entries = (size_t)a->top * z.per_tile, merge = (size_t)W * cols * (c.head_dim + 4 + 2) * 4;
     const size_t lists = one ? (big ? ((size_t)a->top * 8 + 15 & ~(size_t)15) : 0) : ATTN_WINDOW * 2 + ((entries < ATTN_WINDOW ? entries : ATTN_WINDOW) * 8 + 15 & ~(size_t)15);
@@ -1660,7 +1665,8 @@ int vox_block_attention(vox_ctx* ctx, void* stream, const vox_block_attention_ar
                     c.page_size, c.block, a->top, z.splits, z.head_tiles, cols, ((size_t)a->q & 15) == 0 && a->q_stride % 8 == 0, ((size_t)a->out & 7) == 0, a->scale < 0.0f, (int)lists};
 #define ATTN_OF(KERN, ...) (c.dtype == VOX_DTYPE_F16 ? (c.head_dim == 128 ? (const void*)KERN<1, 128, __VA_ARGS__> : (const void*)KERN<1, 64, __VA_ARGS__>) \
                                                      : (c.head_dim == 128 ? (const void*)KERN<0, 128, __VA_ARGS__> : (const void*)KERN<0, 64, __VA_ARGS__>))
-    const void* kern = one ? (big ? ATTN_OF(k_block_attn_row, 8, true) : ATTN_OF(k_block_attn_row, 8, false)) : z.tiles == 2 ? ATTN_OF(k_block_attn_rows, 4, 2) : ATTN_OF(k_block_attn_rows, 4, 1);
+    const void* kern = one ? (big ? ATTN_OF(k_block_attn_row, 8, true) : ATTN_OF(k_block_attn_row, 8, false))
+                     : z.tiles == 2 ? (W == 8 ? ATTN_OF(k_block_attn_rows, 8, 2) : ATTN_OF(k_block_attn_rows, 4, 2)) : W == 8 ? ATTN_OF(k_block_attn_rows, 8, 1) : ATTN_OF(k_block_attn_rows, 4, 1);
 #undef ATTN_OF
     VOX_TRY(launch(kern, dim3((unsigned)grid), 64 * W, lds, (hipStream_t)stream, s));
     if (z.splits == 1) return VOX_OK;

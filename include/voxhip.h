@@ -171,7 +171,7 @@ int vox_block_select_form(const vox_block_select_args* a);
 
 /* out[i, h] = softmax(scale q . K) V over the tokens < q_kvlen[i] of the blocks in row i's list of h's kv head; out [n_rows,heads,head_dim] contiguous.  An entry
  * counts if it is a block of the row and larger than every entry before it.  A row without any such entry is zero.  Scores, sums and
- * the output are fp32 until its one rounding (the softmax weights enter the matrix cores as two 16-bit terms).  What a masked or unlisted
+ * the output are fp32 until its one rounding (the softmax weights enter the matrix cores as three bf16 or two fp16 terms, which hold what fp32 does).  What a masked or unlisted
  * token holds, NaN and infinities included, does not reach a row. */
 typedef struct {
     vox_block_cache cache;   /* bounds and steps are not read */

@@ -87,8 +87,8 @@ def attend(q, kv, blocks, pages, n, block, scale):
             p /= p.sum()
             out[i] = p @ v
             # a score in fp32: d products summed in any order, the scale (and log2 e) on top: (d + 4) 2^-24 of the terms' magnitudes; the weights take
-            # twice the largest such error (numerator and sum), 2^-21 for the exponential and its argument's rounding (8 half steps), 2^-15 for the two
-            # 16-bit terms of a weight (a half step of a half step each, and their sum), and the sums over the tokens (T + 64) 2^-23
+            # twice the largest such error (numerator and sum), 2^-21 for the exponential and its argument's rounding (8 half steps), 2^-15 for a weight
+            # in 16-bit terms (two of them, a half step of a half step each, and their sum), and the sums over the tokens (T + 64) 2^-23
             err = (d + 4) * 2.0 ** -24 * abs(scale) * (np.abs(k) @ np.abs(q[i])).max() + 2.0 ** -23 * np.abs(z - z.max()).max()
             off[i] = (2 * err + 2.0 ** -21 + 2.0 ** -15 + (len(tokens) + 64) * 2.0 ** -23) * (p @ np.abs(v))
     return out, off

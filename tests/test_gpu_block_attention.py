@@ -956,3 +956,58 @@ def test_rows_together_choose_among_many(dev, top, alike):
         assert np.array_equal(got[i], R.select(f64(q[i]), nb, ns, s.pages[s.req[i]], s.kvlen[i], block, top, 1, 2)), i
     one = torch.cat([B.select_blocks(q[i:i + 1], bounds, steps, s.q_req[i:i + 1], s.q_kvlen[i:i + 1], s.indptr, s.indices, block=block, top=top, max_kvlen=14400) for i in range(s.n)])
     assert np.array_equal(got, one.cpu().numpy())
+
+
+def in_terms(p, n):
+    """Weights as the sum of n bf16 terms."""
+    out, left = np.zeros_like(p), p.copy()
+    for _ in range(n):
+        term = torch.from_numpy(left).to(torch.bfloat16).double().numpy()
+        out, left = out + term, left - term
+    return out
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("hq,h,d,rows,top,form", [(16, 8, 128, 240, 3, 16), (8, 8, 64, 240, 3, 16), (4, 2, 128, 3, 3, 1), (32, 8, 64, 5, 3, 1), (4, 2, 128, 2, 100, -7)])
+def test_weights_keep_their_bits(dev, dtype, hq, h, d, rows, top, form):
+    """Three tokens of a block whose weighted values cancel to 2^-16 and less of themselves: what a softmax weight loses on its way into a product shows in the output, not below
+    its rounding."""
+    from vox_serve_amd import block_attention as B
+    t, many = TYPES[dtype], 48 if top < 48 else 100
+    s = Paged(dev, t, h, d, 64, [many * 16 + rows], [rows], seed=d + rows)
+    assert attend_form(s, hq, 16, top, 1) == form
+    g = torch.Generator().manual_seed(rows)
+    as_type = lambda x: torch.from_numpy(x).to(t).double().numpy()
+    z = as_type((2 * torch.rand(many, 16, h, generator=g, dtype=torch.float64) - 1).numpy())
+    p, v = np.exp(z), np.zeros((many, 16, h, d))
+    v[:, 3] = as_type((1 + torch.rand(many, h, d, generator=g, dtype=torch.float64)).numpy())
+    v[:, 6] = as_type(-v[:, 3] * (p[:, 3] / p[:, 6])[..., None])
+    v[:, 13] = as_type(-(v[:, 3] * p[:, 3, :, None] + v[:, 6] * p[:, 6, :, None]) / p[:, 13, :, None])
+    s.kv.zero_()
+    for j in range(many):
+        page, at = s.pages[0][j // 4], j % 4 * 16
+        s.kv[page, 0, at:at + 16, :, 0] = torch.from_numpy(z[j]).to(t).to(dev)
+        s.kv[page, 1, at:at + 16] = torch.from_numpy(v[j]).to(t).to(dev)
+    factor = 1 + np.arange(hq // h) / 64                     # the heads' q: what one of them cancels, the others of its kv head do not
+    q = torch.zeros(rows, hq, d, dtype=t, device=dev)
+    q[:, :, 0] = torch.from_numpy(np.tile(factor, h)).to(t).to(dev)
+    lists = torch.full((rows, h, top), -1, dtype=torch.int32, device=dev)
+    mine = [[i % many] if top < 48 else list(range(100)) for i in range(rows)]
+    for i, m in enumerate(mine):
+        lists[i, :, :len(m)] = torch.tensor(m, dtype=torch.int32, device=dev)
+    got = f64(B.block_attention(q, s.kv, lists, *s.plan, block=16, scale=1.0, n_req=1)).reshape(rows, h, -1, d)
+    half, seen = torch.finfo(t).eps / 2, False
+    for i, m in enumerate(mine):
+        w = np.exp(z[m][:, :, :, None] * factor)              # [blocks, 16, kv heads, heads of one]
+        total = w.sum((0, 1))[..., None]
+        want, size = (np.einsum("bthg,bthd->hgd", w, x) / total for x in (v[m], np.abs(v[m])))
+        # A score is one product, exact.  A weight: its exponent's rounding, |z| log2 e < 4 (2^-23), log2 e's own (2^-24 of it, below 2^-23), the exponential's (2^-23) and
+        # two fp16 terms' (2^-23; three of bf16 have all bits); three tokens of three terms, an addition each, 2^-23 where it cuts bits off; the parts' factors in
+        # a list of many blocks are exponentials once more (2^-23 and its argument's, 2^-23), and its 3 x 100 tokens meet in sums of 32 that are added up (100 x 2^-23 of what
+        # stands there, the blocks' own remainders).  The sum of the weights is in all of a column: (1600 + 64) 2^-23 of the output itself.
+        rest = np.abs(np.einsum("bthg,bthd->bhgd", w, v[m]) / total).sum(0)
+        tol = half * np.abs(want) + (13 if len(m) == 1 else 15) * 2.0 ** -23 * size + 1664 * 2.0 ** -23 * rest + torch.finfo(t).smallest_normal * half
+        assert (np.abs(got[i] - want) <= tol).all(), (i, float((np.abs(got[i] - want) / tol).max()))
+        if dtype == "bf16":
+            seen |= bool((np.abs(np.einsum("bthg,bthd->hgd", in_terms(w, 2), v[m]) / total - want) > tol).any())
+    assert seen or dtype != "bf16" or len(mine[0]) > 1       # two terms would be outside

@@ -770,14 +770,15 @@ __global__ __launch_bounds__(64 * W) void k_block_choose(SelectArgs a) {
 //   O^T = V^T P^T   B: these same scores' weights, where they are - the order of the 32 tokens inside a product is free, so V's lanes take tokens 4 g ..
 //                   4 g + 3 of each tile too.  A lane loads 8 neighbouring channels (D = 128) of its 8 tokens, whole rows a sixteen lanes, and a tile t of
 //                   the product takes channel 8 m + t of each: halves of registers by v_perm, no LDS.
-// Maximum and sum of a column stay with its lanes (online softmax, exponents of two, fp32).  A weight enters as the sum of two 16-bit terms: one alone would
-// cost as much precision as the output's own rounding.
+// Maximum and sum of a column stay with its lanes (online softmax, exponents of two, fp32).  A weight enters as the sum of three bf16 terms or of two fp16 ones: all
+// that fp32 has of it.  (One term would cost as much as the output's own rounding; two of bf16 drop 2^-17 of a weight, which shows where values cancel.  The third costs a chunk of
+// 1024 rows of 2048 tokens 140 us for 129, a row nothing that can be measured.)
 // What a column must not see is kept from it by its score alone (weight 0), which holds as long as V is finite; where a result is not, the rows are gone through
-// again one by one in the same order with V's masked tokens as zero, and a value that is not finite multiplied by the weight as one term (an infinity times the
-// two terms would be inf - inf).  Rows that see no such value come out bit for bit as if it were not there.
+// again one by one in the same order with V's masked tokens as zero, and a value that is not finite multiplied by the weight as one term (an infinity times
+// several of them would be inf - inf).  Rows that see no such value come out bit for bit as if it were not there.
 // What bounds it, and measured (bf16, dim 128, unless said): 64 rows of 2048 tokens, 32 heads on 8 of 64, fp16: 50 us for 268 MB, 5.4 TB/s - the memory.  4 rows of 8192, 32 heads on 2:
 // 9.6 us in 64 parts and 3.9 to join them, 34 MB - the launches and one pass of latency.  A row of 512 tokens, 16 heads on 8: 7.9 us, chain of list, pages, K, V alone.
-// A chunk of 1024 rows of 2048 tokens, 16 heads on 8: 125 us, 17 GFLOP (26 with the weights' second term): tiles of 16 rows meet all that any of them lists, some
+// A chunk of 1024 rows of 2048 tokens, 16 heads on 8: 140 us, 17 GFLOP (34 with the weights' three terms): tiles of 16 rows meet all that any of them lists, some
 // 3.5 times one row's list, and a tile's tokens are masked, weighed and moved by vector instructions for 32 columns only.
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -915,9 +916,15 @@ __device__ __forceinline__ float vmax(float x, float y) {            // (fmaxf o
     asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(x), "v"(y));
     return r;
 }
-// the weights of T tiles of scores, as two 16-bit terms (one: the first, not zero where the weight is not); o and l go to a new base if they have to
+// A weight as a sum of 16-bit terms that has its 24 bits: three of bf16, or two of fp16, whose sum is off by 2^-23 of it at most (half a step of half a step of half a step)
+template <int F16>
+struct Terms {
+    static constexpr int N = F16 ? 2 : 3;
+    uint4 w[N];
+};
+// the weights of T tiles of scores in terms (one: the first, not zero where the weight is not); o and l go to a new base if they have to
 template <int F16, int D, int T, bool CAREFUL>
-__device__ __forceinline__ void weigh(f32x4 (&s4)[T], const int (&sees)[T], float scale2, float& m, float& l, f32x4 (&o)[D / 16], uint4 (&bh)[T / 2], uint4 (&bl)[T / 2], uint4 (&one)[T / 2]) {
+__device__ __forceinline__ void weigh(f32x4 (&s4)[T], const int (&sees)[T], float scale2, float& m, float& l, f32x4 (&o)[D / 16], Terms<F16> (&b)[T / 2], uint4 (&one)[T / 2]) {
     const float inf = __uint_as_float(0x7f800000u);
     bool part = CAREFUL;
 #pragma unroll
@@ -952,40 +959,47 @@ __device__ __forceinline__ void weigh(f32x4 (&s4)[T], const int (&sees)[T], floa
     for (int x = 0; x < T; ++x) l += sum[x];
 #pragma unroll
     for (int y = 0; y < T / 2; ++y) {
-        const float* const w = p + 8 * y;
-        u32 ph[4], pl[4];
+        float w[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            ph[i] = pack2<F16>(w[2 * i], w[2 * i + 1]);
-            pl[i] = pack2<F16>(w[2 * i] - elem_f<F16>((bf16_t)ph[i]), w[2 * i + 1] - elem_f<F16>((bf16_t)(ph[i] >> 16)));
-        }
-        bh[y] = make_uint4(ph[0], ph[1], ph[2], ph[3]);
-        bl[y] = make_uint4(pl[0], pl[1], pl[2], pl[3]);
-        if constexpr (CAREFUL) {
+        for (int i = 0; i < 8; ++i) w[i] = p[8 * y + i];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) ph[i] |= (w[2 * i] > 0.0f && !(ph[i] & 0xffffu) ? 1u : 0u) | (w[2 * i + 1] > 0.0f && !(ph[i] >> 16) ? 0x10000u : 0u);
-            one[y] = make_uint4(ph[0], ph[1], ph[2], ph[3]);
+        for (int n = 0; n < Terms<F16>::N; ++n) {
+            u32 t[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                t[i] = pack2<F16>(w[2 * i], w[2 * i + 1]);
+                if (n + 1 < Terms<F16>::N) {                         // (what a term leaves is exact)
+                    w[2 * i] -= elem_f<F16>((bf16_t)t[i]);
+                    w[2 * i + 1] -= elem_f<F16>((bf16_t)(t[i] >> 16));
+                }
+            }
+            b[y].w[n] = make_uint4(t[0], t[1], t[2], t[3]);
+            if constexpr (CAREFUL) if (n == 0) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) t[i] |= (p[8 * y + 2 * i] > 0.0f && !(t[i] & 0xffffu) ? 1u : 0u) | (p[8 * y + 2 * i + 1] > 0.0f && !(t[i] >> 16) ? 0x10000u : 0u);
+                one[y] = make_uint4(t[0], t[1], t[2], t[3]);
+            }
         }
     }
 }
 // o += V^T P^T over a pair of tiles; vt(t): channel CPL c + t of the lane's eight tokens
 template <int F16, int D, bool CAREFUL, class V>
-__device__ __forceinline__ void weighted(V vt, const uint4& bh, const uint4& bl, const uint4& one, f32x4 (&o)[D / 16]) {
+__device__ __forceinline__ void weighted(V vt, const Terms<F16>& b, const uint4& one, f32x4 (&o)[D / 16]) {
     if constexpr (CAREFUL) {
 #pragma unroll
         for (int t = 0; t < D / 16; ++t) {
             const uint4 a = vt(t), odd = make_uint4(a.x & halves_not_finite<F16>(a.x), a.y & halves_not_finite<F16>(a.y), a.z & halves_not_finite<F16>(a.z), a.w & halves_not_finite<F16>(a.w));
             const uint4 fine = make_uint4(a.x ^ odd.x, a.y ^ odd.y, a.z ^ odd.z, a.w ^ odd.w);
             o[t] = mma32<F16>(odd, one, o[t]);
-            o[t] = mma32<F16>(fine, bh, o[t]);
-            o[t] = mma32<F16>(fine, bl, o[t]);
+#pragma unroll
+            for (int n = 0; n < Terms<F16>::N; ++n) o[t] = mma32<F16>(fine, b.w[n], o[t]);
         }
     } else {
 #pragma unroll
         for (int t = 0; t < D / 16; ++t) {
             const uint4 a = vt(t);
-            o[t] = mma32<F16>(a, bh, o[t]);
-            o[t] = mma32<F16>(a, bl, o[t]);
+#pragma unroll
+            for (int n = 0; n < Terms<F16>::N; ++n) o[t] = mma32<F16>(a, b.w[n], o[t]);
         }
     }
 }
@@ -1164,10 +1178,11 @@ __global__ __launch_bounds__(64 * W, 1) void k_block_attn_row(BlockAttnArgs a) {
 #pragma unroll
                 for (int x = 0; x < T; ++x)
                     if (tok[x] + 16 > n) f.drop_v(x, n - tok[x], g);
-                uint4 bh[T / 2], bl[T / 2], one[T / 2];
-                weigh<F16, D, T, CAREFUL>(s4, sees, a.scale2, m, l, o, bh, bl, one);
+                Terms<F16> b[T / 2];
+                uint4 one[T / 2];
+                weigh<F16, D, T, CAREFUL>(s4, sees, a.scale2, m, l, o, b, one);
 #pragma unroll
-                for (int y = 0; y < T / 2; ++y) weighted<F16, D, CAREFUL>([&](int t) { return f.vt(y, t); }, bh[y], bl[y], one[y], o);
+                for (int y = 0; y < T / 2; ++y) weighted<F16, D, CAREFUL>([&](int t) { return f.vt(y, t); }, b[y], one[y], o);
             }
         };
         if (__builtin_expect(careful, 0)) go(std::true_type{});
@@ -1359,9 +1374,10 @@ __global__ __launch_bounds__(64 * W, 2) void k_block_attn_rows(BlockAttnArgs a) 
                             int sees[2];
 #pragma unroll
                             for (int x = 0; x < 2; ++x) sees[x] = rows[x] >> (n * rpt + rc) & 1 ? own[n] - tok[x] - 4 * g : 0;
-                            uint4 bh[1], bl[1], one[1];
-                            weigh<F16, D, 2, CAREFUL>(s4[n], sees, a.scale2, m[n], l[n], o[n], bh, bl, one);
-                            weighted<F16, D, CAREFUL>([&](int t) { return f.vt(0, t); }, bh[0], bl[0], one[0], o[n]);
+                            Terms<F16> b[1];
+                            uint4 one[1];
+                            weigh<F16, D, 2, CAREFUL>(s4[n], sees, a.scale2, m[n], l[n], o[n], b, one);
+                            weighted<F16, D, CAREFUL>([&](int t) { return f.vt(0, t); }, b[0], one[0], o[n]);
                         }
                     }
                     dma_wait();                                      // (nothing may land in LDS that is used anew)

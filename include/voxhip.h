@@ -13,7 +13,8 @@
  *   - all calls only ENQUEUE work on the given stream (safe inside hipGraph capture), allocate nothing
  *     after the context / engine was created, and return VOX_OK or an error code (vox_last_error()).
  *   - numerics follow the fixed-order contract written in DESIGN.md §"Numeric contract" (the same one
- *     oracle/voxref.c restates on the CPU): results do not depend on grid shape or batch size.
+ *     oracle/voxref.c restates on the CPU): results do not depend on grid shape or batch size
+ *     (vox_block_attention, which no engine calls, takes its sums in its launch's order).
  */
 #ifndef VOXHIP_H
 #define VOXHIP_H
@@ -122,7 +123,7 @@ typedef struct {
 typedef struct { /* rows of one ragged call (the plan arrays of vox_paged_attention) */
     const int32_t *q_req, *q_kvlen, *kv_indptr, *kv_indices;
     int32_t n_rows, n_req;  /* n_req: entries of kv_indptr minus one */
-    int32_t n_own;          /* how many requests have rows here (0: not known; the launch goes by it, the results do not) */
+    int32_t n_own;          /* how many requests have rows here (0: not known); the launch goes by it, the choice does not, an attention's fp32 sums are taken in its order */
     int32_t heads;          /* query heads: kv_heads times 1..64 */
     int32_t max_kvlen;      /* bounds q_kvlen (a longer row is taken as this long) */
 } vox_block_rows;
@@ -172,7 +173,9 @@ int vox_block_select_form(const vox_block_select_args* a);
 /* out[i, h] = softmax(scale q . K) V over the tokens < q_kvlen[i] of the blocks in row i's list of h's kv head; out [n_rows,heads,head_dim] contiguous.  An entry
  * counts if it is a block of the row and larger than every entry before it.  A row without any such entry is zero.  Scores, sums and
  * the output are fp32 until its one rounding (the softmax weights enter the matrix cores as three bf16 or two fp16 terms, which hold what fp32 does).  What a masked or unlisted
- * token holds, NaN and infinities included, does not reach a row. */
+ * token holds, NaN and infinities included, does not reach a row, nor do other rows' queries: not a bit of it changes.
+ * The order of a row's fp32 sums, and by that the rounding of its last bit, goes by the launch: by n_rows, n_own, heads, the type, top and block, and where rows go together
+ * by which blocks the neighbouring ones list.  It is the one exception here from results that do not depend on the batch; equal calls give equal bits. */
 typedef struct {
     vox_block_cache cache;   /* bounds and steps are not read */
     vox_block_rows rows;

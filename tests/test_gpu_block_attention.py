@@ -1011,3 +1011,23 @@ def test_weights_keep_their_bits(dev, dtype, hq, h, d, rows, top, form):
         if dtype == "bf16":
             seen |= bool((np.abs(np.einsum("bthg,bthd->hgd", in_terms(w, 2), v[m]) / total - want) > tol).any())
     assert seen or dtype != "bf16" or len(mine[0]) > 1       # two terms would be outside
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("hq,h,d", [(16, 8, 128), (8, 8, 64), (28, 4, 64), (32, 8, 64)])
+def test_rows_together_do_not_feel_each_others_keys(dev, dtype, hq, h, d):
+    """Neighbouring rows that list neighbouring blocks: whatever scores one row's blocks give it, its neighbours' results stay as they are, bit for bit."""
+    from vox_serve_amd import block_attention as B
+    s = Paged(dev, TYPES[dtype], h, d, 32, [1300], [280], seed=d)
+    lists = torch.tensor([[j for j in range(60) if not 16 <= j < 32 or j % 2 == i % 2] for i in range(s.n)], dtype=torch.int32, device=dev)[:, None].repeat(1, h, 1).contiguous()
+    assert attend_form(s, hq, 16, lists.shape[2], 1) > 1
+    q = s.rnd(s.n, hq, d)
+    clean = B.block_attention(q, s.kv, lists, *s.plan, block=16, n_req=1)
+    check_attend(s, q, clean, lists, 16, d ** -0.5, [0, 1, 17, 278, 279])
+    for factor in (10.0, 100.0, -1000.0):
+        kv = s.kv.clone()
+        for j in range(16, 32, 2):
+            kv[s.pages[0][j // 2], 0, :16] *= factor          # (an even block: the front half of its page)
+        got = B.block_attention(q, kv, lists, *s.plan, block=16, n_req=1)
+        assert torch.equal(got[1::2], clean[1::2])
+        assert not torch.equal(got[::2], clean[::2])

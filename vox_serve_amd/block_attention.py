@@ -229,7 +229,8 @@ def block_attention(q, kv_cache, blocks, q_req, q_kvlen, kv_indptr, kv_indices, 
     """softmax(scale q . K) V over the tokens that a row sees (its first q_kvlen) of the blocks in its lists, int32 [rows, kv heads, top] as of `select_blocks`.
 
     An entry counts if it is a block of the row and larger than the entries before it; a row without any is zero.  scale: 1 / sqrt(dim) if
-    it is not given.  n_req: how many requests have rows here, 0 if it is not known (which launch is taken goes by it)."""
+    it is not given.  n_req: how many requests have rows here, 0 if it is not known.  Sizes and n_req choose the launch, and by that the order of a
+    row's fp32 sums; what the tokens of other rows hold changes nothing, not a bit."""
     device = _cache(kv_cache)
     if device.index != torch.cuda.current_device():
         with torch.cuda.device(device):

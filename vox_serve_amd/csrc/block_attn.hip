@@ -906,7 +906,7 @@ struct VTiles {
 };
 // A tile of columns against T tiles of tokens.  sees[x]: how many of the lane's tokens 4 g, 4 g + 1, .. of tile x its column sees (any number: 4 and more are all).
 // m: the exponent's base, in powers of two.  It need not be the maximum, only near enough that no weight passes 2^8: a lane looks at its own scores alone, and the
-// column's lanes meet only when one of them is that far above (the first time, and a few times more).  A tile is masked as a whole, by the base, unless the
+// columns' lanes meet only when one of them is that far above (the first time, and a few times more); a column without such a lane keeps its base and its sums.  A tile is masked as a whole, by the base, unless the
 // column's last token lies in it.  What was a third more vector instructions a tile is the same to fp32 rounding.  CAREFUL: every score is masked, and
 // V that is not finite meets the weight as one term.
 #define ATTN_AHEAD 8.0f
@@ -940,7 +940,8 @@ __device__ __forceinline__ void weigh(f32x4 (&s4)[T], const int (&sees)[T], floa
     for (int x = 0; x < T; ++x) top = vmax(top, sees[x] > 0 ? vmax(vmax(s4[x][0], s4[x][1]), vmax(s4[x][2], s4[x][3])) : -inf);
     top *= scale2;
     if (__ballot(top > m + ATTN_AHEAD)) {
-        const float now = vmax(m, xor_max<32>(xor_max<16>(top))), keep = __builtin_amdgcn_exp2f(m - (now == -inf ? 0.0f : now));
+        // (only the columns that ask for it: a column's base, and with it the rounding of its weights, goes by its own scores alone)
+        const float most = xor_max<32>(xor_max<16>(top)), now = most > m + ATTN_AHEAD ? most : m, keep = __builtin_amdgcn_exp2f(m - (now == -inf ? 0.0f : now));
         m = now;
         l *= keep;
 #pragma unroll

@@ -153,3 +153,16 @@ def test_bounds_and_steps_come_together():
     for pair in ((bounds, None), (None, steps)):
         with pytest.raises(ValueError, match="come together"):
             B._bounds_of(kv, *pair)
+
+
+@pytest.mark.parametrize("rows,own", [(0, 0), (0, 3), (3, 0)])
+@pytest.mark.parametrize("top,block", [(8, 16), (16, 128), (1024, 128), (0, 16)])
+def test_sizes_without_rows(rows, own, top, block):
+    """What a call of no rows asks for: no workspace, a launch of some kind - and an answer, whatever its lists' length."""
+    L, wrong = N.lib(), dict(n_rows=rows, n_own=own, top=top, block=block, page_size=256)
+    attend, select = (B._ATTEND.pack(*dict(ATTEND, **wrong).values()), B._SELECT.pack(*dict(SELECT, **dict(wrong, top=max(top, 3)), max_kvlen=400).values()))
+    long = B._SELECT.pack(*dict(SELECT, **dict(wrong, top=max(top, 3)), max_kvlen=16 * 5000).values())
+    assert L.vox_block_attention_form(attend) != 0 and L.vox_block_select_form(select) != 0 and L.vox_block_select_form(long) != 0
+    for room in (L.vox_block_attention_workspace_bytes(attend), L.vox_block_select_workspace_bytes(select), L.vox_block_select_workspace_bytes(long)):
+        assert room == 0 if rows == 0 else room >= 0
+    assert B._attend_room(rows, own, 16, 2, 128, 0, 256, block, top) >= 0

@@ -1031,3 +1031,19 @@ def test_rows_together_do_not_feel_each_others_keys(dev, dtype, hq, h, d):
         got = B.block_attention(q, kv, lists, *s.plan, block=16, n_req=1)
         assert torch.equal(got[1::2], clean[1::2])
         assert not torch.equal(got[::2], clean[::2])
+
+
+def test_no_rows_with_long_lists(dev):
+    from vox_serve_amd import block_attention as B
+    s = Paged(dev, torch.bfloat16, 2, 64, 128, [300], [1])
+    none, plan = s.rnd(1, 8, 64)[:0], (s.q_req[:0], s.q_kvlen[:0], s.indptr, s.indices)
+    bounds, steps = B.new_bounds(s.kv, 128)
+    before = s.kv.clone()
+    for n_req in (0, 1):
+        blocks = B.select_blocks(none, bounds, steps, *plan, block=128, top=1000, max_kvlen=300000, n_req=n_req)
+        assert blocks.shape == (0, 2, 1000)
+        assert B.block_attention(none, s.kv, blocks, *plan, block=128, n_req=n_req).shape == (0, 8, 64)
+        empty = s.q_req[:0]
+        assert B.rope_append(none, none[:, :2], none[:, :2], s.kv, None, empty, empty, empty, bounds=bounds, steps=steps, n_req=n_req).shape == (0, 8, 64)
+    B.update_bounds(s.kv, bounds, steps, s.q_req[:0], s.q_req[:0])
+    assert torch.equal(s.kv, before) and not bounds.any()

@@ -1640,7 +1640,7 @@ static AttnShape attn_shape(const vox_block_attention_args* a, int cus) {
     // A row's list over several blocks of threads, one for each CU that has none, 256 tokens at least; a second launch joins them (some 3 us of host time, so not for 1024
     // tokens, 11.4 / 9.4).  us in a captured graph, one block of threads a row / parts: 16 heads on 8 of 128, 1 row of 2048 tokens 19.4 / 10.2, 4 rows 25.8 / 16.7, 16 rows
     // 39.1 / 36.5; 32 on 2, 1 row of 4096 28.4 / 9.6, 4 rows of 8192 57 / 16.6, 16 rows 92 / 35 (two for each CU: 40); 32 on 8 of 64, 8 rows of 2048 21.2 / 16.9.
-    if (tokens > 1024) {
+    if (tokens > 1024 && blocks > 0) {                               // (a call of no rows asks for its workspace too)
         const long z = (cus + blocks - 1) / blocks, most = (tokens + 255) / 256, parts = z < most ? z : most;
         s.splits = (int)(parts < 1 ? 1 : parts > 64 ? 64 : parts);
     }

@@ -1047,3 +1047,59 @@ def test_no_rows_with_long_lists(dev):
         assert B.rope_append(none, none[:, :2], none[:, :2], s.kv, None, empty, empty, empty, bounds=bounds, steps=steps, n_req=n_req).shape == (0, 8, 64)
     B.update_bounds(s.kv, bounds, steps, s.q_req[:0], s.q_req[:0])
     assert torch.equal(s.kv, before) and not bounds.any()
+
+
+def choose_by_scores(q, bounds, steps, pages, n, block, top, first, last):
+    """The oracle's choice with all of a row's scores at once: q [heads, dim], bounds [pages, kv heads, per, 2, dim] of whole numbers."""
+    h, per, have = bounds.shape[1], bounds.shape[2], -(-n // block)
+    j = np.arange(first, have - last)
+    page, out = np.asarray(pages)[j // per], np.zeros((h, top), np.int64)
+    for g in range(h):
+        mine = q[g * (q.shape[0] // h):(g + 1) * (q.shape[0] // h)]
+        a = np.clip(np.rint(mine / R.step_of(mine)), -127, 127).astype(np.int64)
+        b = bounds[page, g, j % per].astype(np.int64)
+        whole = sum(np.maximum(row * b[:, 0], row * b[:, 1]).sum(1) for row in a)
+        score = whole.astype(np.float32) * steps[page, g, j % per]
+        best = j[np.argsort(-score, kind="stable")[:top - first - last]]
+        out[g] = np.sort(np.concatenate([np.arange(first), best, np.arange(have - last, have)]))
+    return out
+
+
+@pytest.mark.parametrize("kinds", [0, 1, 9])
+@pytest.mark.parametrize("lens,rows,form", [
+    # blocks of 16 tokens; a row alone in parts, whose choice has up to 2, 4, 8 and 32 keys a lane
+    ([1500], 1, -6), ([2051], 1, -9), ([2052], 1, -9), ([4099], 1, -17), ([4100], 1, -17), ([6000], 1, -24), ([8195], 1, -33), ([8196], 1, -33), ([20001], 1, -79), ([32768], 1, -128),
+    # eight waves a row: 2, 4 and 8 keys a lane
+    ([900, 1027, 1028, 2051, 2052, 3333, 4096], 70, 1),
+    # sixteen: 2, 4, 8, 16 and 32
+    ([700, 2051, 2052, 4099, 4100, 8195, 8196, 16387, 16388, 25000, 32768], 66, 1),
+    # rows of a chunk together, a wave a row: 2 to 16 of up to 1024 blocks, 2 to 64 of up to 4096
+    ([35, 131, 132, 259, 260, 515, 516, 1024], 330, 16), ([40, 131, 132, 260, 515, 516, 1027, 1028, 2051, 2052, 4096], 330, 8),
+])
+def test_select_among_many_thousands(dev, kinds, lens, rows, form):
+    """Each number of keys a lane that a choice has, at its borders, with all scores different, all the same, and of a few kinds: equal ones on both sides of waves."""
+    from vox_serve_amd import block_attention as B
+    from vox_serve_amd import _native as N
+    hq, h, d, block, per, top = 4, 2, 64, 16, 8, 29
+    g = np.random.default_rng(sum(lens) + kinds)
+    most = max(lens)
+    pages = -(-most // per) if not kinds else kinds
+    b = np.sort(g.integers(-127, 128, (pages, h, per, 2, d)), axis=3)[..., ::-1, :].astype(np.int8)
+    st = (2.0 ** g.integers(-3, 2, (pages, h, per))).astype(np.float32)
+    if kinds:
+        b[:], st[:] = b[:, :, :1], st[:, :, :1]
+    table_ = g.permutation(pages) if not kinds else g.integers(0, pages, -(-most // per))
+    blocks = [lens[i % len(lens)] for i in range(rows)]
+    kvlen = [n * block - int(x) for n, x in zip(blocks, g.integers(0, block, rows))]
+    q = torch.from_numpy(g.standard_normal((rows, hq, d))).to(torch.bfloat16).to(dev)
+    i32 = lambda x: torch.tensor(np.asarray(x), dtype=torch.int32, device=dev)
+    bounds, steps = torch.from_numpy(b.copy()).to(dev), torch.from_numpy(st).to(dev)
+    args, n_req = (i32([0] * rows), i32(kvlen), i32([0, len(table_)]), i32(table_)), 1 if form > 1 else rows
+    sizes = B._SELECT.pack(0, 16, 16, pages, per * block, block, h, d, 0, 16, 16, 16, 16, rows, 1, n_req, hq, max(kvlen), 0, 16, 16, 0, 0, 0, top, 1, 2)
+    assert N.lib().vox_block_select_form(sizes) == form
+    got = B.select_blocks(q, bounds, steps, *args, block=block, top=top, max_kvlen=max(kvlen), n_req=n_req).cpu().numpy()
+    for i in range(min(rows, 2 * len(lens))):
+        assert np.array_equal(got[i], choose_by_scores(f64(q[i]), b, st, table_, kvlen[i], block, top, 1, 2)), (i, kvlen[i])
+    small = min(range(rows), key=lambda i: kvlen[i])
+    if blocks[small] < 3000:
+        assert np.array_equal(got[small], R.select(f64(q[small]), b, st, table_.tolist(), kvlen[small], block, top, 1, 2))

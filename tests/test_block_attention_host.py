@@ -166,3 +166,39 @@ def test_sizes_without_rows(rows, own, top, block):
     for room in (L.vox_block_attention_workspace_bytes(attend), L.vox_block_select_workspace_bytes(select), L.vox_block_select_workspace_bytes(long)):
         assert room == 0 if rows == 0 else room >= 0
     assert B._attend_room(rows, own, 16, 2, 128, 0, 256, block, top) >= 0
+
+
+def test_graph_memory_goes_with_its_graph(monkeypatch):
+    """What captured calls make is held for their graph's sake until vox_graph_destroy, by a capture whose stream the call is on; what an eager call makes is not."""
+    import gc
+    import weakref
+    destroyed = []
+    monkeypatch.setattr(N, "_graph_memory", {})
+    monkeypatch.setattr(N, "_parted", [])
+    monkeypatch.setattr(N, "_capturing", {})
+
+    class Capture:
+        def __init__(self, records):
+            self.held, self.records = [], lambda: records
+
+    t = torch.zeros(8)
+    assert N.hold(t) is t                                    # no capture
+    for records in (False, True):
+        N._capturing[t.device.index] = cap = Capture(records)
+        assert N.hold(t) is t and len(cap.held) == records
+        del N._capturing[t.device.index]
+    refs = [weakref.ref(cap.held[0])]
+    N._graph_memory[77] = cap.held
+    del t, cap
+    gc.collect()
+    assert refs[0]() is not None
+    N._destroy(destroyed.append, 5)                          # another graph: nothing of ours
+    assert refs[0]() is not None
+    handle = N.c_void_p(77)
+    N._capturing[None] = Capture(True)                       # inside a capture: the memory waits for its end
+    N._destroy(destroyed.append, handle)
+    assert destroyed == [5, handle] and not N._graph_memory and len(N._parted) == 1 and refs[0]() is not None
+    N._let_go(N._parted.pop())
+    gc.collect()
+    assert refs[0]() is None
+    assert not hasattr(B, "_kept")

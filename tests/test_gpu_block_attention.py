@@ -1103,3 +1103,66 @@ def test_select_among_many_thousands(dev, kinds, lens, rows, form):
     small = min(range(rows), key=lambda i: kvlen[i])
     if blocks[small] < 3000:
         assert np.array_equal(got[small], R.select(f64(q[small]), b, st, table_.tolist(), kvlen[small], block, top, 1, 2))
+
+
+def test_graphs_give_their_memory_back(dev):
+    """Captured, replayed and destroyed again and again: what is allocated stays what it was; so does it behind a body that raises, and for eager calls during a capture."""
+    import threading
+
+    from vox_serve_amd import _native as N
+    from vox_serve_amd import block_attention as B
+    s = Paged(dev, torch.bfloat16, 2, 128, 128, [9000, 9000], [1, 1], seed=6)
+    q, plan = s.rnd(2, 32, 256)[:, :, :128], [x.long() for x in s.plan]
+    bounds, steps = B.new_bounds(s.kv, 128)
+    B.update_bounds(s.kv, bounds, steps, torch.arange(s.kv.shape[0], device=dev), torch.full((s.kv.shape[0],), 127, device=dev))
+
+    def run():
+        return B.block_attention(q, s.kv, B.select_blocks(q, bounds, steps, *plan, block=128, top=60, max_kvlen=9000, n_req=2), *plan, block=128, n_req=2)
+
+    want, sizes = run(), []
+    for i in range(8):
+        with N.graph_capture() as cap:
+            got = run()
+        assert N._graph_memory[cap.graph.value]
+        for _ in range(3):
+            got.zero_()
+            N.check(N.lib().vox_graph_launch(cap.graph, N.stream()))
+            assert torch.equal(got, want)
+        # a body that raises behind its calls
+        with pytest.raises(KeyError):
+            with N.graph_capture() as failed:
+                run()
+                raise KeyError(i)
+        assert not failed.held
+        N.lib().vox_graph_destroy(cap.graph)
+        assert not N._graph_memory and not N._capturing
+        del got, cap, failed
+        torch.cuda.synchronize()
+        sizes.append(torch.cuda.memory_allocated())
+    assert len(set(sizes)) == 1
+    # another thread's eager calls while this one captures, and a stream forked from the capture
+    done, side = [], torch.cuda.Stream()
+
+    def other():
+        with torch.cuda.device(dev), torch.cuda.stream(torch.cuda.Stream()):
+            done.append(run())
+            torch.cuda.current_stream().synchronize()
+
+    with N.graph_capture() as cap:
+        first = run()
+        held = len(cap.held)
+        worker = threading.Thread(target=other)
+        worker.start()
+        worker.join()
+        assert len(cap.held) == held and torch.is_tensor(done[0])
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            second = run()
+        torch.cuda.current_stream().wait_stream(side)
+        assert len(cap.held) == 2 * held
+    assert torch.equal(done[0], want)
+    for _ in range(3):
+        first.zero_(), second.zero_()
+        N.check(N.lib().vox_graph_launch(cap.graph, N.stream()))
+        assert torch.equal(first, want) and torch.equal(second, want)
+    N.lib().vox_graph_destroy(cap.graph)

@@ -126,7 +126,9 @@ _SIGS = {
 _OPTIONAL_SIGS = {}
 
 _lib = None
-_capturing = set()   # devices with a stream capture in progress (graph_capture)
+_capturing = {}     # device -> the graph_capture in progress there
+_graph_memory = {}  # graph handle -> tensors that its captured calls made (hold), until vox_graph_destroy
+_parted = []        # those of graphs that were destroyed while a capture was in progress on their device
 _ctxs = {}          # one context per HIP device of this process (the LM's GPU; a detokenizer on a second GPU gets its own)
 
 
@@ -150,6 +152,8 @@ def lib():
             if fn is None:
                 continue
             fn.restype, fn.argtypes = res, args
+        native = L.vox_graph_destroy
+        L.vox_graph_destroy = lambda graph: _destroy(native, graph)
         if L.vox_abi_version() != 1:
             raise VoxError("libvoxhip ABI version mismatch")
         _lib = L
@@ -204,6 +208,34 @@ def stream():
 _capture_streams = {}
 
 
+def hold(t):
+    """A tensor that an operator makes for itself or its caller.  Eagerly the allocator's stream order makes it safe to let go of behind the call; one that a call records
+    into a `graph_capture` stays until that graph is destroyed, so that no replay writes to memory that another graph or an eager call has by then (torch's own
+    graphs keep theirs by their pool).  Calls on streams that are not being captured, of this or another thread, are eager ones."""
+    cap = _capturing.get(t.device.index)
+    if cap is not None and cap.records():
+        cap.held.append(t)
+    return t
+
+
+def _destroy(native, graph):
+    """vox_graph_destroy, and what the graph held.  A replay may still be running: its memory waits for it."""
+    held = _graph_memory.pop(getattr(graph, "value", graph), None)
+    native(graph)
+    if held:
+        if held[0].device.index in _capturing:      # (no synchronization inside a capture: when that one ends)
+            _parted.append(held)
+        else:
+            _let_go(held)
+
+
+def _let_go(held):
+    if held[0].is_cuda:
+        import torch
+        torch.cuda.synchronize(held[0].device)
+    held.clear()
+
+
 class graph_capture:
     """`with graph_capture() as cap: <enqueue on N.stream()>` -> `cap.graph` (a vox_graph handle).
 
@@ -214,7 +246,10 @@ class graph_capture:
     leaves behind until the graph finishes) makes the command processor alternate between the queues, and every dependent
     dispatch of the running graph costs about 1.3 us more on an MI355X — 0.5 ms of a 3.3 ms Qwen3-TTS frame of ~510 dependent
     kernels (profiles/round3_queue_fence.txt).  Whoever wants two graphs side by side (LM frame + codec chunk) puts them on
-    two streams itself and orders them with events it waits for on the HOST."""
+    two streams itself and orders them with events it waits for on the HOST.
+
+    Workspaces, converted plans and results that operators make inside the body (`hold`) belong to the graph until
+    `vox_graph_destroy`; those of a body that raised are let go of at once."""
 
     def __init__(self):
         import torch
@@ -224,14 +259,19 @@ class graph_capture:
             _capture_streams[d] = torch.cuda.Stream(device=d)
         self.cs = _capture_streams[d]
         self.graph = None
+        self.held = []
+
+    def records(self):
+        """Whether the current stream is being captured: the capture's own, or one that was forked from it."""
+        return self._torch.cuda.is_current_stream_capturing()
 
     def __enter__(self):
         torch = self._torch
         d = torch.cuda.current_device()
         if d in _capturing:      # the capture stream is one per device and not re-entrant
             raise VoxError("graph_capture: a capture is already active on this device (nested or concurrent captures are not supported)")
-        _capturing.add(d)
         self._dev = d
+        _capturing[d] = self
         self.cur = torch.cuda.current_stream()
         self.cs.wait_stream(self.cur)
         self._ctx = torch.cuda.stream(self.cs)
@@ -240,7 +280,7 @@ class graph_capture:
             check(lib().vox_graph_begin(ctx(), stream()))
         except Exception:
             self._ctx.__exit__(None, None, None)
-            _capturing.discard(self._dev)
+            _capturing.pop(self._dev, None)
             raise
         return self
 
@@ -251,10 +291,16 @@ class graph_capture:
         finally:
             self._ctx.__exit__(None, None, None)
             self.cur.wait_stream(self.cs)
-            _capturing.discard(self._dev)
+            _capturing.pop(self._dev, None)
+            held, self.held = self.held, []
+            for x in [x for x in _parted if x[0].device.index == self._dev]:
+                _parted.remove(x)
+                _let_go(x)
         if et is None:
             check(status)
             self.graph = gh
+            if held:
+                _graph_memory[gh.value] = held
         else:
             # the body raised: its exception propagates; a graph that was instantiated all the same is released, and a failed
             # end-of-capture is at least reported

@@ -34,18 +34,6 @@ def _on(device):
     return N._ctxs.get(device.index) or N.ctx(), torch._C._cuda_getCurrentRawStream(device.index)
 
 
-_kept = []                               # what captured graphs go back to
-
-
-def _hold(t):
-    """A tensor that a call makes for itself or its caller.  Eagerly the allocator's stream order makes it safe to let go of behind the call; one that a
-    `graph_capture` records is kept for good, so that no graph ever writes to memory that another graph or an eager call has by then (torch's own graphs
-    keep theirs by their pool)."""
-    if t.device.index in N._capturing:
-        _kept.append(t)
-    return t
-
-
 @functools.lru_cache(maxsize=4096)
 def _attend_room(*sizes):
     """Bytes of workspace that a call of these sizes asks for: a function of the sizes alone."""
@@ -76,8 +64,8 @@ def _ints(t, shape, device, name):
     if t.dtype is not torch.int32:
         if t.dtype is not torch.int64:
             raise TypeError(f"{name} is {t.dtype}: int32 or int64 is wanted")
-        t = _hold(t.to(torch.int32))
-    return t if t.is_contiguous() else _hold(t.contiguous())
+        t = N.hold(t.to(torch.int32))
+    return t if t.is_contiguous() else N.hold(t.contiguous())
 
 
 def _heads(t, rows, dim, like, name):
@@ -88,7 +76,7 @@ def _heads(t, rows, dim, like, name):
     if t.dtype is not like.dtype or t.device != like.device:
         raise ValueError(f"{name} is {t.dtype} on {t.device}, {like.dtype} on {like.device} is wanted")
     _, apart, unit = t.stride()
-    return t if unit == 1 and (apart == dim or shape[1] == 1) else _hold(t.contiguous())
+    return t if unit == 1 and (apart == dim or shape[1] == 1) else N.hold(t.contiguous())
 
 
 def _cache(kv):
@@ -124,7 +112,7 @@ def _bounds_of(kv, bounds, steps):
 
 def _out(out, shape, like, device, name="out"):
     if out is None:
-        return _hold(torch.empty(shape, dtype=like, device=device))      # (rows that are passed over hold what the allocator left)
+        return N.hold(torch.empty(shape, dtype=like, device=device))      # (rows that are passed over hold what the allocator left)
     if out.shape != shape or out.dtype is not like or out.device != device or not out.is_contiguous():
         raise ValueError(f"{name} is {out.dtype} {tuple(out.shape)} on {out.device}: a contiguous {like} {tuple(shape)} on {device} is wanted")
     return out
@@ -162,7 +150,7 @@ def rope_append(q, k, v, kv_cache, cos_sin, positions, pages, slots, *, interlea
     if cos_sin is not None:
         if cos_sin.dim() != 3 or cos_sin.shape[2] != 2 or cos_sin.dtype is not torch.float32 or cos_sin.device != device:
             raise ValueError(f"cos_sin is {cos_sin.dtype} {tuple(cos_sin.shape)} on {cos_sin.device}: float32 [positions, turning channels / 2, 2] on {device} is wanted")
-        cos_sin = cos_sin if cos_sin.is_contiguous() else _hold(cos_sin.contiguous())
+        cos_sin = cos_sin if cos_sin.is_contiguous() else N.hold(cos_sin.contiguous())
         rot, table, length = 2 * cos_sin.shape[1], cos_sin.data_ptr(), cos_sin.shape[0]
     where = (0, 0, page) if bounds is None and steps is None else _bounds_of(kv_cache, bounds, steps)
     out = _out(out, q.shape, kv_cache.dtype, device)
@@ -216,7 +204,7 @@ def select_blocks(q, bounds, steps, q_req, q_kvlen, kv_indptr, kv_indices, *, bl
     plan = _plan(q_req, q_kvlen, kv_indptr, kv_indices, rows, device)
     out = _out(out, (rows, h, top), torch.int32, device)
     room = _select_room(rows, n_req, q.shape[1], h, d, _DTYPES[q.dtype], per * block, block, top, first, last, max_kvlen)
-    ws = _hold(torch.empty(room, dtype=torch.uint8, device=device)) if room else None
+    ws = N.hold(torch.empty(room, dtype=torch.uint8, device=device)) if room else None
     ctx, stream = _on(device)
     N.check(N.lib().vox_block_select(ctx, stream, _SELECT.pack(
         0, bounds.data_ptr(), steps.data_ptr(), n_pages, per * block, block, h, d, _DTYPES[q.dtype], plan[0].data_ptr(), plan[1].data_ptr(), plan[2].data_ptr(),
@@ -246,7 +234,7 @@ def block_attention(q, kv_cache, blocks, q_req, q_kvlen, kv_indptr, kv_indices, 
     out = _out(out, q.shape, kv_cache.dtype, device)
     ctx, stream = _on(device)
     room = _attend_room(rows, n_req, q.shape[1], h, d, _DTYPES[kv_cache.dtype], page, block, top)
-    ws = _hold(torch.empty(room, dtype=torch.uint8, device=device)) if room else None
+    ws = N.hold(torch.empty(room, dtype=torch.uint8, device=device)) if room else None
     N.check(N.lib().vox_block_attention(ctx, stream, _ATTEND.pack(
         kv_cache.data_ptr(), 0, 0, n_pages, page, block, h, d, _DTYPES[kv_cache.dtype], plan[0].data_ptr(), plan[1].data_ptr(), plan[2].data_ptr(),
         plan[3].data_ptr(), rows, plan[2].shape[0] - 1, n_req, q.shape[1], 2 ** 31 - 1, 0, q.data_ptr(), blocks.data_ptr(), out.data_ptr(),

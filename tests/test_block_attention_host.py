@@ -202,3 +202,27 @@ def test_graph_memory_goes_with_its_graph(monkeypatch):
     gc.collect()
     assert refs[0]() is None
     assert not hasattr(B, "_kept")
+
+
+def test_plans_count_their_requests_when_asked():
+    """A plan for dense attention does no work for the operators beside it."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    from vox_serve_amd.flashinfer_utils import FlashInferDecodeWrapper, FlashInferPrefillWrapper
+    ops = []
+
+    class Count(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            ops.append(func.overloadpacket.__name__)
+            return func(*args, **(kwargs or {}))
+
+    w = FlashInferPrefillWrapper(None, 4, 2, 256, 16, device="cpu")
+    with Count():
+        w.plan(torch.tensor([0, 5, 5, 6]), torch.tensor([0, 1, 2, 4]), torch.arange(4).int(), torch.tensor([5, 6, 7]))
+    assert "gt" not in ops and ops.count("sum") == 1          # (the rows' number)
+    assert w._n_own() == 2 and w._n_own() == 2
+    w.plan(torch.tensor([0, 1, 2]), torch.tensor([0, 1, 2]), torch.arange(2).int(), torch.tensor([1, 1]))
+    assert w._n_own() == 2
+    d = FlashInferDecodeWrapper(None, 4, 2, 256, 16, device="cpu")
+    d.plan(torch.tensor([0, 1, 2, 4]), torch.arange(4).int(), torch.tensor([5, 6, 7]))
+    assert d._n_own() == 3

@@ -100,11 +100,18 @@ class _PagedBase:
                                       N.ptr(slot), k.shape[0], kv_cache.shape[2], self.n_kv_head, self.head_dim))
 
     # ---- long contexts: the operators of block_attention, with this plan's rows
+    def _n_own(self):
+        """How many requests have rows: counted when an operator asks for it, not in every plan."""
+        m = self._meta
+        if "n_own" not in m:
+            m["n_own"] = int((m["lens"] > 0).sum())
+        return m["n_own"]
+
     def set_kv_cache_rope(self, kv_cache, q, k, v, position_ids, cos_sin, interleave=False, bounds=None, steps=None, out=None):
         """apply_rope_pos_ids and set_kv_cache in one call, from slices of one projection's output if need be; returns the rotated q."""
         m = self._meta
         return block_attention.rope_append(q, k, v, kv_cache, cos_sin, position_ids, m["page"], m["slot"], interleave=interleave, bounds=bounds, steps=steps,
-                                           n_req=m["n_own"], out=out)
+                                           n_req=self._n_own(), out=out)
 
     def update_bounds(self, kv_cache, bounds, steps):
         """The bounds of the blocks that the planned rows complete, behind set_kv_cache."""
@@ -113,12 +120,12 @@ class _PagedBase:
     def select_blocks(self, q, bounds, steps, top, first=1, last=2, out=None):
         m = self._meta
         return block_attention.select_blocks(q, bounds, steps, m["q_req"], m["q_kvlen"], m["indptr"], m["indices"], block=self.page_size // bounds.shape[2], top=top,
-                                             max_kvlen=m["max_kvlen"], first=first, last=last, n_req=m["n_own"], out=out)
+                                             max_kvlen=m["max_kvlen"], first=first, last=last, n_req=self._n_own(), out=out)
 
     def run_blocks(self, q, kv_cache, blocks, block, out=None):
         """Attention as `run`, over the listed blocks of `block` tokens only."""
         m = self._meta
-        return block_attention.block_attention(q, kv_cache, blocks, m["q_req"], m["q_kvlen"], m["indptr"], m["indices"], block=block, n_req=m["n_own"], out=out)
+        return block_attention.block_attention(q, kv_cache, blocks, m["q_req"], m["q_kvlen"], m["indptr"], m["indices"], block=block, n_req=self._n_own(), out=out)
 
 
 class FlashInferPrefillWrapper(_PagedBase):
@@ -168,7 +175,7 @@ class FlashInferPrefillWrapper(_PagedBase):
         self._meta = dict(q_req=q_req.to(dev), q_kvlen=q_kvlen.to(dev), page=page32, slot=slot32,
                           indptr=paged_kv_indptr.to(device=dev, dtype=torch.int32),
                           indices=paged_kv_indices.to(device=dev, dtype=torch.int32),
-                          max_kvlen=int(kv_len.max()) if n_req else 1, n_req=n_req, n_own=int((lens > 0).sum()))
+                          max_kvlen=int(kv_len.max()) if n_req else 1, n_req=n_req, lens=lens)
 
     def run(self, q, kv_cache):
         return self._run(q, kv_cache)

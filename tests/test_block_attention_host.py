@@ -226,3 +226,20 @@ def test_plans_count_their_requests_when_asked():
     d = FlashInferDecodeWrapper(None, 4, 2, 256, 16, device="cpu")
     d.plan(torch.tensor([0, 1, 2, 4]), torch.arange(4).int(), torch.tensor([5, 6, 7]))
     assert d._n_own() == 3
+
+
+def test_rope_table():
+    """The angles that a caller hands to set_kv_cache_rope: those of apply_rope_pos_ids, for as many positions as are asked for."""
+    from vox_serve_amd import flashinfer_utils as F
+    t = F.rope_table(20000, 64, rope_theta=1e6, device="cpu")
+    assert t.shape == (20000, 32, 2) and t.dtype is torch.float32 and t.is_contiguous()
+    assert torch.equal(t[:8192], F._rope_table(torch.device("cpu"), 8192, 64, 1e6, 1.0, None))
+    angle = torch.arange(20000, dtype=torch.float32)[:, None] * (1e6 ** (-torch.arange(32, dtype=torch.float64) / 32)).float()
+    assert (t - torch.stack([angle.double().cos(), angle.double().sin()], -1)).abs().max() < 20000 * 2.0 ** -22     # (a step of a frequency, and of its product)
+    far = F.rope_table(64, 128, rope_scale=8.0, rope_theta=5e5, device="cpu", low_freq_factor=1.0, high_freq_factor=4.0, old_context_len=8192)
+    assert torch.equal(far, F._rope_table(torch.device("cpu"), 64, 128, 5e5, 8.0, (1.0, 4.0, 8192)))
+    for bad in ((0, 64), (10, 63), (10, 0)):
+        with pytest.raises(ValueError, match="rope_table"):
+            F.rope_table(*bad, device="cpu")
+    with pytest.raises(TypeError, match="unexpected"):
+        F.rope_table(10, 64, device="cpu", theta=1.0)

@@ -1166,3 +1166,25 @@ def test_graphs_give_their_memory_back(dev):
         N.check(N.lib().vox_graph_launch(cap.graph, N.stream()))
         assert torch.equal(first, want) and torch.equal(second, want)
     N.lib().vox_graph_destroy(cap.graph)
+
+
+def test_rope_append_far_positions(dev):
+    """Positions behind apply_rope_pos_ids' own 8192, by a table of the caller's length; behind that one's end its last row."""
+    from vox_serve_amd.flashinfer_utils import FlashInferDecodeWrapper, apply_rope_pos_ids, rope_table
+    hq, h, d, page, kv_lens = 8, 2, 64, 128, [5000, 131072, 9000]
+    need = [-(-n // page) for n in kv_lens]
+    g = torch.Generator().manual_seed(2)
+    q, k, v = (torch.randn(3, x, d, generator=g).bfloat16().to(dev) for x in (hq, h, h))
+    kv = torch.zeros(sum(need), 2, page, h, d, dtype=torch.bfloat16, device=dev)
+    w = FlashInferDecodeWrapper(None, hq, h, hq * d, page, device=dev)
+    i32 = lambda a: torch.tensor(a, dtype=torch.int32)
+    w.plan(i32([0] + list(np.cumsum(need))), torch.randperm(sum(need), generator=g).int(), i32([n - (m - 1) * page for n, m in zip(kv_lens, need)]), torch.bfloat16)
+    cs = rope_table(131072, d, rope_theta=1e6, device=dev)
+    for pos in (torch.tensor(kv_lens, device=dev) - 1, torch.tensor([8191, 8192, 200000], device=dev)):
+        got = w.set_kv_cache_rope(kv, q, k, v, pos, cs)
+        want = R.rotate(f64(q), cs.cpu().numpy(), pos.cpu().numpy(), False)
+        assert (np.abs(f64(got) - want) <= 2.0 ** -8 * np.abs(want) * (1 + 2.0 ** -8) + 2.0 ** -22 * np.abs(f64(q)).max(-1, keepdims=True)).all()
+        near = pos < 8192
+        qr, kr = apply_rope_pos_ids(q, k, pos, rope_theta=1e6)
+        assert torch.equal(got[near], qr[near]) and torch.equal(kv[w._meta["page"].long(), 0, w._meta["slot"].long()][near], kr[near])
+        assert not torch.equal(got[~near], qr[~near])

@@ -131,9 +131,9 @@ def rope_append(q, k, v, kv_cache, cos_sin, positions, pages, slots, *, interlea
     """Rotate q [rows, heads, dim] and k [rows, kv heads, dim] by their rows' positions and append k and v to the cache at (pages, slots).
     Returns the rotated q (`out` if it is given; q itself serves if it is contiguous).
 
-    q, k and v may be slices of one projection's output.  cos_sin: fp32 [positions, channels that turn / 2, 2] (`engine.rope_table`: plain,
-    scaled and llama-3.1 angles; fewer channels than dim: the others stay), or None: nothing turns.  The results are those of
-    `apply_rope_pos_ids` and `set_kv_cache`, bit for bit.  With `bounds` and `steps` (`new_bounds`), also those of the blocks that the
+    q, k and v may be slices of one projection's output.  cos_sin: fp32 [positions, channels that turn / 2, 2] (`flashinfer_utils.rope_table`:
+    plain, scaled and llama-3.1 angles; fewer channels than dim: the others stay), or None: nothing turns.  Positions are clamped to the table.  By the same table the
+    results are those of `apply_rope_pos_ids`, whose own has 8192 positions, and `set_kv_cache`, bit for bit.  With `bounds` and `steps` (`new_bounds`), also those of the blocks that the
     rows complete.  n_req: how many requests have rows here, 0 if it is not known; as many as rows: a token of each, one launch."""
     device = _cache(kv_cache)
     if device.index != torch.cuda.current_device():

@@ -9,7 +9,7 @@ FlashInfer, no Triton.
   FlashInferDecodeWrapper     flashinfer_utils.py:149-244 (plan / run / set_kv_cache, .kv_cache_locations)
 
 Beyond the reference, both wrappers hand the same plan to the operators of `block_attention`: set_kv_cache_rope (rotate and append in one
-call), update_bounds, select_blocks and run_blocks (attention over the blocks that were chosen).
+call, by the angles of rope_table), update_bounds, select_blocks and run_blocks (attention over the blocks that were chosen).
 
 plan() takes CPU int32 tensors like the reference and uploads them with an async copy; unlike the
 reference it needs no device synchronisation afterwards (the caller's `torch.cuda.synchronize()` is
@@ -29,10 +29,31 @@ def _rope_table(device, max_pos, rot, theta, scale, llama31):
     key = (str(device), max_pos, rot, float(theta), float(scale), llama31)
     t = _ROPE_TABLES.get(key)
     if t is None:
-        from .engine import StackCfg, rope_table
+        from .engine import StackCfg, rope_table as table
         c = StackCfg(0, 0, 0, 0, rot, 0, rope_theta=theta, rope_scale=scale, rope_dim=rot, rope_llama31=llama31)
-        t = _ROPE_TABLES[key] = rope_table(max_pos, c, device)
+        t = _ROPE_TABLES[key] = table(max_pos, c, device)
     return t
+
+
+def _llama31(kwargs):
+    """llama-3.1's factors out of keyword arguments: (low, high, old context) or None, and the other arguments."""
+    llama31 = {k: kwargs[k] for k in ("low_freq_factor", "high_freq_factor", "old_context_len") if k in kwargs}
+    other = {k: v for k, v in kwargs.items() if k not in llama31}
+    if not llama31:
+        return None, other
+    return (float(llama31.get("low_freq_factor", 1.0)), float(llama31.get("high_freq_factor", 4.0)), int(llama31.get("old_context_len", 8192))), other
+
+
+def rope_table(max_pos: int, rotary_dim: int, rope_scale: float = 1.0, rope_theta: float = 10000.0, device="cuda", **kwargs):
+    """The angles that `set_kv_cache_rope` and `block_attention.rope_append` turn by: fp32 [max_pos, rotary_dim / 2, 2] (cos, sin), the ones of
+    apply_rope_pos_ids with the same arguments (its own table ends at 8192 positions).  As long as the contexts: positions behind the last row take that row's angles."""
+    l31, other = _llama31(kwargs)
+    if other:
+        raise TypeError(f"rope_table() got unexpected keyword arguments {sorted(other)}")
+    if max_pos <= 0 or rotary_dim <= 0 or rotary_dim % 2:
+        raise ValueError(f"rope_table: {max_pos} positions of {rotary_dim} channels (an even number)")
+    from .engine import StackCfg, rope_table as table
+    return table(max_pos, StackCfg(0, 0, 0, 0, rotary_dim, 0, rope_theta=rope_theta, rope_scale=rope_scale, rope_dim=rotary_dim, rope_llama31=l31), device)
 
 
 def rms_norm(hidden_states: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6) -> torch.Tensor:
@@ -46,8 +67,7 @@ def rms_norm(hidden_states: torch.Tensor, weight: torch.Tensor, eps: float = 1e-
 
 def apply_rope_pos_ids(query_states, key_states, position_ids, rope_scale: float = 1.0, rope_theta: float = 10000.0,
                        interleave: bool = False, **kwargs):
-    llama31 = {k: kwargs[k] for k in ("low_freq_factor", "high_freq_factor", "old_context_len") if k in kwargs}
-    other = {k: v for k, v in kwargs.items() if k not in llama31}
+    l31, other = _llama31(kwargs)
     unknown = set(other) - {"rotary_dim"}
     if unknown:
         raise TypeError(f"apply_rope_pos_ids() got unexpected keyword arguments {sorted(unknown)}")
@@ -55,10 +75,6 @@ def apply_rope_pos_ids(query_states, key_states, position_ids, rope_scale: float
     n, hq, d = q.shape
     hkv = k.shape[1]
     rot = other.get("rotary_dim") or d
-    l31 = None
-    if llama31:
-        l31 = (float(llama31.get("low_freq_factor", 1.0)), float(llama31.get("high_freq_factor", 4.0)),
-               int(llama31.get("old_context_len", 8192)))
     max_pos = 8192
     cs = _rope_table(q.device, max_pos, rot, rope_theta, rope_scale, l31)
     qo, ko = torch.empty_like(q), torch.empty_like(k)
@@ -108,7 +124,7 @@ class _PagedBase:
         return m["n_own"]
 
     def set_kv_cache_rope(self, kv_cache, q, k, v, position_ids, cos_sin, interleave=False, bounds=None, steps=None, out=None):
-        """apply_rope_pos_ids and set_kv_cache in one call, from slices of one projection's output if need be; returns the rotated q."""
+        """apply_rope_pos_ids and set_kv_cache in one call, from slices of one projection's output if need be; returns the rotated q.  cos_sin: `rope_table`."""
         m = self._meta
         return block_attention.rope_append(q, k, v, kv_cache, cos_sin, position_ids, m["page"], m["slot"], interleave=interleave, bounds=bounds, steps=steps,
                                            n_req=self._n_own(), out=out)

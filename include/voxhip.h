@@ -185,7 +185,7 @@ typedef struct {
     void* workspace;
     int64_t workspace_bytes, q_stride;
     int32_t top;
-    float scale;
+    float scale;             /* of any sign, -2e38 to 2e38 */
 } vox_block_attention_args;
 int64_t vox_block_attention_workspace_bytes(const vox_block_attention_args* a);
 int vox_block_attention(vox_ctx* ctx, void* stream, const vox_block_attention_args* a);

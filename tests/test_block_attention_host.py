@@ -243,3 +243,10 @@ def test_rope_table():
             F.rope_table(*bad, device="cpu")
     with pytest.raises(TypeError, match="unexpected"):
         F.rope_table(10, 64, device="cpu", theta=1.0)
+
+
+@pytest.mark.parametrize("scale", [2.4e38, -3.4e38])
+def test_scales_whose_exponents_overflow_are_refused(scale):
+    """Scores are taken in powers of two: a scale that is not finite times log2 e would make every weight NaN."""
+    assert call("vox_block_attention", B._ATTEND, ATTEND, scale=scale) == 1
+    assert b"scale" in N.lib().vox_last_error()

@@ -1188,3 +1188,23 @@ def test_rope_append_far_positions(dev):
         qr, kr = apply_rope_pos_ids(q, k, pos, rope_theta=1e6)
         assert torch.equal(got[near], qr[near]) and torch.equal(kv[w._meta["page"].long(), 0, w._meta["slot"].long()][near], kr[near])
         assert not torch.equal(got[~near], qr[~near])
+
+
+@pytest.mark.parametrize("scale", [0.0, 2.0 ** -110, -(2.0 ** -104), 1e38])
+@pytest.mark.parametrize("rows", [1, 240])
+def test_attention_scales_of_all_sizes(dev, rows, scale):
+    """Scores of 2^105 under no scale, under scales that bring them to about one, and scores of 2^-117 under the largest one: what the formula gives."""
+    from vox_serve_amd import block_attention as B
+    h, d = 8, 64
+    s = Paged(dev, torch.bfloat16, h, d, 32, [400], [rows], seed=rows)
+    q = s.rnd(rows, 2 * h, d)
+    if abs(scale) < 1:                                       # (powers of two: exact)
+        q *= 2.0 ** 52
+        s.kv[:, 0] *= 2.0 ** 50
+    else:
+        q *= 2.0 ** -60
+        s.kv[:, 0] *= 2.0 ** -60
+    blocks = torch.arange(10, dtype=torch.int32, device=dev).repeat(rows, h, 1).contiguous()
+    assert (attend_form(s, 2 * h, 16, 10, 1) > 1) == (rows > 1)
+    got = B.block_attention(q, s.kv, blocks, *s.plan, block=16, scale=scale, n_req=1)
+    check_attend(s, q, got, blocks, 16, float(np.float32(scale)), [0] if rows == 1 else [0, 100, 239])

@@ -807,10 +807,12 @@ struct BlockAttnArgs {
     bf16_t* out;
     float *part_o, *part_ml;             // splits > 1: [row][head][split][D], [row][head][split][2]
     long q_stride;
-    float scale2;                        // |scale| log2 e, a little above zero (a lower score is a larger one where the scale is negative: q changes its sign)
+    float scale2;                        // |scale| log2 e, LEAST_SCALE2 at least (a lower score is a larger one where the scale is negative: q changes its sign)
     int n_rows, n_req, Hq, Hkv, max_kvlen, n_pages, page_size, block, top;
     int splits, head_tiles, cols, q_al, out_al, negate, k_at;      // k_at: byte of the waves' K in LDS (rows of several)      // cols: columns of a wave in the merge's LDS
 };
+// The smallest number above zero: a masked score, -infinity, times it is what zero would not make of it, and the largest score times it is nothing (2^-21).
+#define LEAST_SCALE2 1.4012984643e-45f
 #define ATTN_WINDOW 4096                 // blocks whose rows' bits lie in LDS at a time (rows of several: 8 KB)
 
 // The entries of a row's list that count, 64 at a time, by one wave: f(j, counts) for every lane.  first: the lane's entry of the first 64.
@@ -1611,6 +1613,7 @@ static int check_attention(const vox_block_attention_args* a) {
     VOX_TRY(check_rows("block_attention", a->cache, a->rows));
     if (a->top < 0 || a->top > VOX_BLOCK_TOP_MAX) return vox_fail(VOX_ERR_INVALID, "block_attention: lists of %d blocks (up to %d)", a->top, VOX_BLOCK_TOP_MAX);
     if (a->q_stride < 0) return vox_fail(VOX_ERR_INVALID, "block_attention: a stride is negative");
+    if (!(fabsf(a->scale) <= 2e38f)) return vox_fail(VOX_ERR_INVALID, "block_attention: a scale of %g (finite, and so times log2 e)", (double)a->scale);
     return VOX_OK;
 }
 // How a call's rows are laid out: rows a tile, and the parts that a row's list is split into.
@@ -1669,7 +1672,6 @@ int vox_block_attention(vox_ctx* ctx, void* stream, const vox_block_attention_ar
         return vox_fail(VOX_ERR_INVALID, "block_attention: a workspace of %lld bytes on 16, %lld are wanted", (long long)(a->workspace ? a->workspace_bytes : 0), (long long)(rows * (c.head_dim + 2) * 4));
     const int64_t grid = (int64_t)((r.n_rows + z.per_tile - 1) / z.per_tile) * z.splits * z.head_tiles * c.kv_heads;
     if (grid > 0x7fffffff) return vox_fail(VOX_ERR_INVALID, "block_attention: %d rows of %d heads are more than a launch holds", r.n_rows, r.heads);
-    if (!(fabsf(a->scale) < 3e38f)) return vox_fail(VOX_ERR_INVALID, "block_attention: the scale is not finite");
     const bool one = z.tiles == 0;
     const float scale2 = fabsf(a->scale) * 1.44269504088896340736f;
     const int W = z.W, G = r.heads / c.kv_heads, cols = one && G < 16 ? G : 16;
@@ -1678,7 +1680,7 @@ int vox_block_attention(vox_ctx* ctx, void* stream, const vox_block_attention_ar
     const size_t lists = one ? (big ? ((size_t)a->top * 8 + 15 & ~(size_t)15) : 0) : ATTN_WINDOW * 2 + ((entries < ATTN_WINDOW ? entries : ATTN_WINDOW) * 8 + 15 & ~(size_t)15);
     const size_t keys = (size_t)W * 128 * c.head_dim, lds = one ? lists + (merge > keys ? merge : keys) : merge > lists + keys ? merge : lists + keys;
     BlockAttnArgs s{(const bf16_t*)a->q, (const bf16_t*)c.kv, r.q_req, r.q_kvlen, r.kv_indptr, r.kv_indices, a->blocks, (bf16_t*)a->out, (float*)a->workspace,
-                    (float*)a->workspace + rows * c.head_dim, (long)a->q_stride, scale2 > 1e-30f ? scale2 : 1e-30f, r.n_rows, r.n_req, r.heads, c.kv_heads, r.max_kvlen, c.n_pages,
+                    (float*)a->workspace + rows * c.head_dim, (long)a->q_stride, scale2 > LEAST_SCALE2 ? scale2 : LEAST_SCALE2, r.n_rows, r.n_req, r.heads, c.kv_heads, r.max_kvlen, c.n_pages,
                     c.page_size, c.block, a->top, z.splits, z.head_tiles, cols, ((size_t)a->q & 15) == 0 && a->q_stride % 8 == 0, ((size_t)a->out & 7) == 0, a->scale < 0.0f, (int)lists};
 #define ATTN_OF(KERN, ...) (c.dtype == VOX_DTYPE_F16 ? (c.head_dim == 128 ? (const void*)KERN<1, 128, __VA_ARGS__> : (const void*)KERN<1, 64, __VA_ARGS__>) \
                                                      : (c.head_dim == 128 ? (const void*)KERN<0, 128, __VA_ARGS__> : (const void*)KERN<0, 64, __VA_ARGS__>))

@@ -250,3 +250,18 @@ def test_scales_whose_exponents_overflow_are_refused(scale):
     """Scores are taken in powers of two: a scale that is not finite times log2 e would make every weight NaN."""
     assert call("vox_block_attention", B._ATTEND, ATTEND, scale=scale) == 1
     assert b"scale" in N.lib().vox_last_error()
+
+
+def test_sizes_beyond_a_launch_are_refused():
+    """Rows whose number comes near 2^31, heads whose channels do: refused, not wrapped around on the way to a launch."""
+    most = 2 ** 31 - 1
+    wide = dict(kv_heads=65535, heads=65535, n_pages=1, n_rows=most, head_dim=64)
+    for own in (0, 1):
+        assert call("vox_block_select", B._SELECT, SELECT, **dict(wide, n_own=own)) == 1
+        assert b"more than a launch" in N.lib().vox_last_error()
+        assert call("vox_block_attention", B._ATTEND, ATTEND, **dict(wide, n_own=own)) == 1
+        assert b"more than a launch" in N.lib().vox_last_error()
+    assert call("vox_rope_append", B._APPEND, APPEND, heads=most) == 1
+    assert call("vox_rope_append", B._APPEND, APPEND, heads=most, bounds=0) == 1
+    assert call("vox_rope_append", B._APPEND, APPEND, heads=2 ** 24, head_dim=512, bounds=0, rot=0) == 1
+    assert b"heads" in N.lib().vox_last_error()

@@ -1471,7 +1471,7 @@ __global__ __launch_bounds__(256) void k_block_attn_merge(BlockAttnArgs a) {
 static int launch_bounds(hipStream_t st, const vox_block_cache& c, const int* page, const int* slot, int n_rows) {
     if (n_rows == 0) return VOX_OK;
     BoundsArgs b{(const bf16_t*)c.kv, c.bounds, c.steps, page, slot, n_rows, c.n_pages, c.page_size, c.block, c.kv_heads};
-    return launch(BY_TYPE_AND_DIM(k_block_bounds, c), dim3((n_rows + 63) / 64, c.kv_heads), 256, 0, st, b);
+    return launch(BY_TYPE_AND_DIM(k_block_bounds, c), dim3((unsigned)(((int64_t)n_rows + 63) / 64), c.kv_heads), 256, 0, st, b);
 }
 
 extern "C" {
@@ -1493,6 +1493,7 @@ int vox_rope_append(vox_ctx* ctx, void* stream, const vox_rope_append_args* a) {
     if (c.bounds) VOX_TRY(check_bounds("rope_append", c));
     const int D = c.head_dim;
     if (D < 2 || D % 2 || D > 512) return vox_fail(VOX_ERR_INVALID, "rope_append: head_dim %d (even, 2 to 512)", D);
+    if (((int64_t)a->heads + 2 * c.kv_heads) * D > 0x7fffffff) return vox_fail(VOX_ERR_INVALID, "rope_append: %d heads of %d channels are 2^31 or more", a->heads, D);
     if (a->n_rows < 0 || a->n_own < 0 || a->heads <= 0) return vox_fail(VOX_ERR_INVALID, "rope_append: %d rows of %d requests, %d heads", a->n_rows, a->n_own, a->heads);
     if (a->rot < 0 || a->rot % 2 || a->rot > D) return vox_fail(VOX_ERR_INVALID, "rope_append: %d of %d channels turn", a->rot, D);
     if (a->n_rows == 0) return VOX_OK;
@@ -1591,7 +1592,7 @@ int vox_block_select(vox_ctx* ctx, void* stream, const vox_block_select_args* a)
     SelectArgs s{(const bf16_t*)a->q, c.bounds, c.steps, r.q_req, r.q_kvlen, r.kv_indptr, r.kv_indices, a->blocks, (long)a->q_stride,
                  r.n_rows, r.n_req, r.heads, c.kv_heads, r.max_kvlen, c.n_pages, c.page_size, c.block, a->top, a->first, a->last, z.stride,
                  ((size_t)a->q & 15) == 0 && a->q_stride % 8 == 0, z.splits, (int)lds, (u32*)a->workspace, per > 1 ? (u32)((1ull << 32) / per + 1) : 0u};
-    const int64_t grid = (int64_t)((r.n_rows + qt - 1) / qt) * c.kv_heads * z.splits;
+    const int64_t grid = ((int64_t)r.n_rows + qt - 1) / qt * c.kv_heads * z.splits;
     if (grid > 0x7fffffff) return vox_fail(VOX_ERR_INVALID, "block_select: %d rows of %d kv heads are more than a launch holds", r.n_rows, c.kv_heads);
 #define SELECT_OF(QT, W, SPLIT, NT) (c.dtype == VOX_DTYPE_F16 ? (c.head_dim == 128 ? (const void*)k_block_select<1, 128, QT, W, SPLIT, NT> : (const void*)k_block_select<1, 64, QT, W, SPLIT, NT>) \
                                                              : (c.head_dim == 128 ? (const void*)k_block_select<0, 128, QT, W, SPLIT, NT> : (const void*)k_block_select<0, 64, QT, W, SPLIT, NT>))
@@ -1670,7 +1671,7 @@ int vox_block_attention(vox_ctx* ctx, void* stream, const vox_block_attention_ar
     const size_t rows = (size_t)r.n_rows * r.heads * z.splits;
     if (z.splits > 1 && (!a->workspace || (size_t)a->workspace & 15 || a->workspace_bytes < (int64_t)(rows * (c.head_dim + 2) * 4)))
         return vox_fail(VOX_ERR_INVALID, "block_attention: a workspace of %lld bytes on 16, %lld are wanted", (long long)(a->workspace ? a->workspace_bytes : 0), (long long)(rows * (c.head_dim + 2) * 4));
-    const int64_t grid = (int64_t)((r.n_rows + z.per_tile - 1) / z.per_tile) * z.splits * z.head_tiles * c.kv_heads;
+    const int64_t grid = ((int64_t)r.n_rows + z.per_tile - 1) / z.per_tile * z.splits * z.head_tiles * c.kv_heads;
     if (grid > 0x7fffffff) return vox_fail(VOX_ERR_INVALID, "block_attention: %d rows of %d heads are more than a launch holds", r.n_rows, r.heads);
     const bool one = z.tiles == 0;
     const float scale2 = fabsf(a->scale) * 1.44269504088896340736f;

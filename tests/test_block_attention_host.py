@@ -265,3 +265,13 @@ def test_sizes_beyond_a_launch_are_refused():
     assert call("vox_rope_append", B._APPEND, APPEND, heads=most, bounds=0) == 1
     assert call("vox_rope_append", B._APPEND, APPEND, heads=2 ** 24, head_dim=512, bounds=0, rot=0) == 1
     assert b"heads" in N.lib().vox_last_error()
+
+
+def test_wrappers_refuse_bounds_of_other_pages():
+    from vox_serve_amd.flashinfer_utils import FlashInferDecodeWrapper
+    w = FlashInferDecodeWrapper(None, 4, 2, 256, 128, device="cpu")
+    w.plan(torch.tensor([0, 1]), torch.arange(1).int(), torch.tensor([5]))
+    q = torch.zeros(1, 4, 64, dtype=torch.bfloat16)
+    for shape in ((1, 2, 3, 2, 64), (1, 2, 0, 2, 64), (1, 2, 256, 2, 64), (1, 2, 2, 64)):
+        with pytest.raises(ValueError, match="pages of 128 tokens"):
+            w.select_blocks(q, torch.zeros(shape, dtype=torch.int8), torch.zeros(shape[:3]), top=4)

@@ -135,7 +135,10 @@ class _PagedBase:
 
     def select_blocks(self, q, bounds, steps, top, first=1, last=2, out=None):
         m = self._meta
-        return block_attention.select_blocks(q, bounds, steps, m["q_req"], m["q_kvlen"], m["indptr"], m["indices"], block=self.page_size // bounds.shape[2], top=top,
+        per = bounds.shape[2] if bounds.dim() == 5 else 0
+        if per == 0 or self.page_size % per:
+            raise ValueError(f"bounds {tuple(bounds.shape)} are not those of pages of {self.page_size} tokens")
+        return block_attention.select_blocks(q, bounds, steps, m["q_req"], m["q_kvlen"], m["indptr"], m["indices"], block=self.page_size // per, top=top,
                                              max_kvlen=m["max_kvlen"], first=first, last=last, n_req=self._n_own(), out=out)
 
     def run_blocks(self, q, kv_cache, blocks, block, out=None):

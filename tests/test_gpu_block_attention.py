@@ -1208,3 +1208,46 @@ def test_attention_scales_of_all_sizes(dev, rows, scale):
     assert (attend_form(s, 2 * h, 16, 10, 1) > 1) == (rows > 1)
     got = B.block_attention(q, s.kv, blocks, *s.plan, block=16, scale=scale, n_req=1)
     check_attend(s, q, got, blocks, 16, float(np.float32(scale)), [0] if rows == 1 else [0, 100, 239])
+
+
+def test_threads_at_once(dev):
+    """Calls of several threads, each on its own stream: the same kernels with more and less LDS, parts and none."""
+    import threading
+
+    from vox_serve_amd import block_attention as B
+    h, d, hq = 2, 128, 32
+    s = Paged(dev, torch.bfloat16, h, d, 128, [70000, 70000], [1, 1], seed=3)
+    q = s.rnd(2, hq, d)
+    bounds, steps = B.new_bounds(s.kv, 16)
+    pages = torch.arange(s.kv.shape[0], device=dev).repeat_interleave(8)
+    B.update_bounds(s.kv, bounds, steps, pages, torch.arange(15, 128, 16, device=dev).repeat(s.kv.shape[0]))
+
+    def run(top, rows):
+        qs, req = q.repeat(rows, 1, 1), s.q_req.repeat(rows)
+        lens = torch.minimum(s.q_kvlen.repeat(rows), torch.full((2 * rows,), 1000 * top, dtype=torch.int32, device=dev))
+        most = min(70000, 1000 * top)
+        b = B.select_blocks(qs, bounds, steps, req, lens, s.indptr, s.indices, block=16, top=top, max_kvlen=most)
+        return b, B.block_attention(qs, s.kv, b, req, lens, s.indptr, s.indices, block=16)
+
+    kinds = [(10, 80), (70, 1), (66, 70), (400, 1), (1000, 3), (62, 66)]
+    want = [run(*k) for k in kinds]
+    torch.cuda.synchronize()
+    errors = []
+
+    def loop(first):
+        try:
+            with torch.cuda.device(dev), torch.cuda.stream(torch.cuda.Stream()):
+                for i in range(40):
+                    k = (first + i) % len(kinds)
+                    got = run(*kinds[k])
+                    torch.cuda.current_stream().synchronize()
+                    assert torch.equal(got[0], want[k][0]) and torch.equal(got[1], want[k][1]), kinds[k]
+        except BaseException as e:
+            errors.append(e)
+
+    threads = [threading.Thread(target=loop, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors

@@ -777,7 +777,8 @@ __global__ __launch_bounds__(64 * W) void k_block_choose(SelectArgs a) {
 // again one by one in the same order with V's masked tokens as zero, and a value that is not finite multiplied by the weight as one term (an infinity times
 // several of them would be inf - inf).  Rows that see no such value come out bit for bit as if it were not there.
 // What bounds it, and measured (bf16, dim 128, unless said): 64 rows of 2048 tokens, 32 heads on 8 of 64, fp16: 50 us for 268 MB, 5.4 TB/s - the memory.  4 rows of 8192, 32 heads on 2:
-// 9.6 us in 64 parts and 3.9 to join them, 34 MB - the launches and one pass of latency.  A row of 512 tokens, 16 heads on 8: 7.9 us, chain of list, pages, K, V alone.
+// 9.7 us in 32 parts and 3.9 to join them, 34 MB - the launches and one pass of latency.  A row of 512 tokens, 16 heads on 8: 7.9 us - 262 KB for each of eight CUs, which at
+// the 35 bytes a ns that one draws are 7.5.
 // A chunk of 1024 rows of 2048 tokens, 16 heads on 8: 140 us, 17 GFLOP (34 with the weights' three terms): tiles of 16 rows meet all that any of them lists, some
 // 3.5 times one row's list, and a tile's tokens are masked, weighed and moved by vector instructions for 32 columns only.
 typedef short s16x8 __attribute__((ext_vector_type(8)));
@@ -918,7 +919,7 @@ __device__ __forceinline__ float vmax(float x, float y) {            // (fmaxf o
     asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(x), "v"(y));
     return r;
 }
-// A weight as a sum of 16-bit terms that has its 24 bits: three of bf16, or two of fp16, whose sum is off by 2^-23 of it at most (half a step of half a step of half a step)
+// A weight as a sum of 16-bit terms that has its 24 bits: three of bf16, or two of fp16, whose sum is off by 2^-23 of it at most (the half step of what is no more than a half step)
 template <int F16>
 struct Terms {
     static constexpr int N = F16 ? 2 : 3;
@@ -1041,7 +1042,7 @@ __device__ __forceinline__ bool merge_columns(const float* s_o, const float2* s_
     }
     return fabsf(sum) < inf && fabsf(acc[0]) < inf && fabsf(acc[1]) < inf && fabsf(acc[2]) < inf && fabsf(acc[3]) < inf;
 }
-// acc / sum (by one reciprocal: 2^-23 more beside the output's 2^-9), or zero where a row lists nothing
+// acc / sum (by one reciprocal: 2^-23 more beside the output's half step, 2^-8 or 2^-11), or zero where a row lists nothing
 template <int F16>
 __device__ __forceinline__ void store_columns(bf16_t* dst, int aligned, bool seen, float sum, const float (&acc)[4]) {
     const float r = 1.0f / sum;
@@ -1419,7 +1420,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_block_attn_rows(BlockAttnArgs a) 
 }
 
 // the splits of a row and head, a block of threads each: four channels a thread, the splits over the groups of D / 4 threads, all loads on their way at once (128 rows and heads
-// of 64 splits: 3.9 us, 4.3 MB; a launch of nothing is 2)
+// of 32 splits: 3.9 us, 2.1 MB; a launch of nothing is 2)
 template <int F16, int D>
 __global__ __launch_bounds__(256) void k_block_attn_merge(BlockAttnArgs a) {
     constexpr int LPD = D / 4, GROUPS = 256 / LPD, MOST = 64 / GROUPS;
@@ -1551,7 +1552,8 @@ static SelectShape select_shape(const vox_block_select_args* a) {
     // rows a tile: 16 while their keys take half a CU's LDS, 8 while they take most of it (4096 blocks), else (and for rows of different requests) one; together only
     // where there are enough of them, the more the more channels a row has to bring to matrix rows first.  us in a captured graph, a row / 16 rows together, 256 blocks, for
     // 64, 128, 256 and 512 rows: 16 heads on 8 of 128 10.6 / 12.3, 13.6 / 12.8, 21 / 13, 37 / 13.3; 32 on 8 10 / 13.6, 12.5 / 13.7, 21.5 / 13.8, 37 / 14.3; 32 on 2 8.8 / 19.4,
-    // 8.8 / 19.8, 10.3 / 19.9, 14.1 / 20; 8 on 8 of 64 9.7 / 11.3, 10.6 / 11.3, 15.2 / 11.4, 25.2 / 11.8.
+    // 8.8 / 19.8, 10.3 / 19.9, 14.1 / 20; 8 on 8 of 64 9.7 / 11.3, 10.6 / 11.3, 15.2 / 11.4, 25.2 / 11.8.  Of other numbers of blocks, a call of the fewest rows that go together: 24 blocks
+    // 11.0 / 11.4, 10.9 / 11.4, 13.5 / 17.1, 11.1 / 11.2 in the same order, 1000 24 / 16, 26 / 18, 46 / 24, 15.7 / 14.9, 3000 65 / 33, 84 / 33, 141 / 36, 32 / 23.
     const int G = r.heads / a->cache.kv_heads;
     const bool many = r.n_own > 0 && r.n_rows >= 2 * (int64_t)r.n_own && (int64_t)r.n_rows * a->cache.kv_heads >= 576 + G * a->cache.head_dim / 2;
     SelectShape s{many && most <= 1024 ? 16 : many && most <= 4096 ? 8 : 1, 8, 1, 0};
@@ -1626,7 +1628,8 @@ static AttnShape attn_shape(const vox_block_attention_args* a, int cus) {
     // Rows together pay once there are enough of them: a tile's block of threads goes through what all its rows list, however few of them there are, a row's through its own list, 15 to
     // the us once the card is full; what R neighbouring rows list between them is some R^0.4 lists.  us, a row / rows together, lists of 2048 tokens, for 96, 128, 192 and 512 rows: 16 heads on
     // 8 of 128 55 / 74, 70 / 73, 98 / 74, 242 / 77; 32 on 8 51 / 56, 65 / 56, 94 / 57, 235 / 93; 8 on 8 of 64 38 / 55, 49 / 54, 70 / 56, 175 / 58; 14 on 2 of 64 24 / 35, 19 / 35, 28 / 36,
-    // 52 / 37; 32 on 2 of 128, 256 rows 38 / 40, 384 53 / 57, 512 70 / 60.
+    // 52 / 37; 32 on 2 of 128, 328 rows 54 / 61, 420 70 / 61, 600 87 / 95, 900 136 / 116.  From lists of 64 tokens to ones of 8192 the crossings hold within a sixth: at the smallest number
+    // of rows that goes together, 16 heads on 8 of 128 30 / 19 and 251 / 207, 32 on 8 24 / 18 and 196 / 154, 8 on 8 of 64 25 / 16 and 181 / 129, 32 on 2 20.5 / 18.6 and 149 / 175.
     // Eight waves a tile while that is a block of threads a CU, four where there are two (4 / 8 waves: 16 heads on 8, 512 rows 102 / 77, 1024 141 / 151; 8 on 8 of 64, 700 rows 66 / 70).
     if (r.n_own > 0 && r.n_rows >= 2 * (int64_t)r.n_own && G <= 16) {
         const int tiles = G > 1 ? 2 : 1, per_tile = tiles * (16 / G);

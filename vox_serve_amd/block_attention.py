@@ -10,8 +10,8 @@ reference has no sparse form); its wrappers hand their plan to the functions her
 
 A cache layer is [pages, 2, page, kv heads, dim] in bf16 or fp16, dim 64 or 128, a page whole blocks of 16, 32, 64 or 128 tokens.  `bounds`
 (int8 [pages, kv heads, blocks a page, 2, dim]) holds the largest and the smallest key of a complete block per channel, as whole numbers of
-`steps` (fp32 [pages, kv heads, blocks a page], powers of two).  Integer plan arrays are int32 (int64 is converted).  Rows whose page is
-negative, or that see no token, are passed over: what would have been written for them stays as it was.
+`steps` (fp32 [pages, kv heads, blocks a page], powers of two).  Integer plan arrays are int32 (int64 is converted, its
+values have to fit).  Rows whose page is negative, or that see no token, are passed over: what would have been written for them stays as it was.
 """
 import functools
 import struct
@@ -132,9 +132,11 @@ def rope_append(q, k, v, kv_cache, cos_sin, positions, pages, slots, *, interlea
     Returns the rotated q (`out` if it is given; q itself serves if it is contiguous).
 
     q, k and v may be slices of one projection's output.  cos_sin: fp32 [positions, channels that turn / 2, 2] (`flashinfer_utils.rope_table`:
-    plain, scaled and llama-3.1 angles; fewer channels than dim: the others stay), or None: nothing turns.  Positions are clamped to the table.  By the same table the
-    results are those of `apply_rope_pos_ids`, whose own has 8192 positions, and `set_kv_cache`, bit for bit.  With `bounds` and `steps` (`new_bounds`), also those of the blocks that the
-    rows complete.  n_req: how many requests have rows here, 0 if it is not known; as many as rows: a token of each, one launch."""
+    plain, scaled and llama-3.1 angles; fewer channels than dim: the others stay), or None: nothing turns.  Positions are clamped to the table.
+    By the same table the results are those of `apply_rope_pos_ids` (whose own has 8192 positions) and `set_kv_cache`, bit for bit.  With `bounds`
+    and `steps` (`new_bounds`), also those of the blocks that the rows complete, by their last token (behind a row that overwrites an earlier one:
+    `update_bounds` with that block's last slot).  n_req: how many requests have rows here, 0 if it is not known; as many as rows: a token of
+    each, one launch."""
     device = _cache(kv_cache)
     if device.index != torch.cuda.current_device():
         with torch.cuda.device(device):

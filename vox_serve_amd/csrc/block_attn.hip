@@ -1627,10 +1627,10 @@ static AttnShape attn_shape(const vox_block_attention_args* a, int cus) {
     AttnShape s{0, 1, 1, (G + 15) / 16, 8};
     // Rows together pay once there are enough of them: a tile's block of threads goes through what all its rows list, however few of them there are, a row's through its own list, 15 to
     // the us once the card is full; what R neighbouring rows list between them is some R^0.4 lists.  us, a row / rows together, lists of 2048 tokens, for 96, 128, 192 and 512 rows: 16 heads on
-    // 8 of 128 55 / 74, 70 / 73, 98 / 74, 242 / 77; 32 on 8 51 / 56, 65 / 56, 94 / 57, 235 / 93; 8 on 8 of 64 38 / 55, 49 / 54, 70 / 56, 175 / 58; 14 on 2 of 64 24 / 35, 19 / 35, 28 / 36,
-    // 52 / 37; 32 on 2 of 128, 328 rows 54 / 61, 420 70 / 61, 600 87 / 95, 900 136 / 116.  From lists of 64 tokens to ones of 8192 the crossings hold within a sixth: at the smallest number
+    // 8 of 128 59 / 80, 74 / 80, 104 / 79, 251 / 80; 32 on 8 52 / 58, 69 / 58, 98 / 59, 245 / 99; 8 on 8 of 64 39 / 55, 51 / 55, 74 / 56, 184 / 57; 14 on 2 of 64 (128 rows on) 18 / 35, 28 / 36,
+    // 53 / 37; 32 on 2 of 128, 256 rows 39 / 42, 328 54 / 61, 420 69 / 60, 600 87 / 95, 900 136 / 116.  From lists of 64 tokens to ones of 8192 the crossings hold within a sixth: at the smallest number
     // of rows that goes together, 16 heads on 8 of 128 30 / 19 and 251 / 207, 32 on 8 24 / 18 and 196 / 154, 8 on 8 of 64 25 / 16 and 181 / 129, 32 on 2 20.5 / 18.6 and 149 / 175.
-    // Eight waves a tile while that is a block of threads a CU, four where there are two (4 / 8 waves: 16 heads on 8, 512 rows 102 / 77, 1024 141 / 151; 8 on 8 of 64, 700 rows 66 / 70).
+    // Eight waves a tile while that is a block of threads a CU, four where there are two (4 / 8 waves: 16 heads on 8, 512 rows 113 / 80, 1024 140 / 154; 8 on 8 of 64, 700 rows 97 / 102).
     if (r.n_own > 0 && r.n_rows >= 2 * (int64_t)r.n_own && G <= 16) {
         const int tiles = G > 1 ? 2 : 1, per_tile = tiles * (16 / G);
         const bool room = a->cache.head_dim == 64 || (int64_t)a->top * per_tile <= 2048;      // (eight waves' K at dim 128 are 128 of a CU's 160 KB, their lists 8 KB and 8 bytes an entry)

@@ -1251,3 +1251,23 @@ def test_threads_at_once(dev):
     for t in threads:
         t.join()
     assert not errors, errors
+
+
+@pytest.mark.parametrize("fill", [float("nan"), float("inf"), 1e4])
+@pytest.mark.parametrize("hq,h,d,rows,top", [(16, 8, 128, 230, 30), (8, 8, 64, 230, 30), (12, 4, 64, 3, 30), (32, 2, 128, 1, 120), (40, 1, 64, 2, 40)])
+def test_queries_of_others_change_nothing(dev, hq, h, d, rows, top, fill):
+    """A row's, and a head's, results are the same bits whatever queries the others have: NaN and infinities that send their tile through the second pass, scores that are large."""
+    from vox_serve_amd import block_attention as B
+    for dtype in (torch.bfloat16, torch.float16):
+        s = Paged(dev, dtype, h, d, 32, [2000], [rows], seed=top)
+        q, blocks = s.rnd(rows, hq, d), random_lists(s, h, 16, top, 3)
+        blocks[0, :, :] = torch.arange(top, dtype=torch.int32, device=dev)
+        clean = B.block_attention(q, s.kv, blocks, *s.plan, block=16, n_req=1)
+        bad = torch.zeros(rows, hq, dtype=torch.bool, device=dev)
+        bad[::3, ::2] = True
+        q2 = q.clone()
+        q2[bad] *= fill
+        got = B.block_attention(q2, s.kv, blocks, *s.plan, block=16, n_req=1)
+        assert torch.equal(got[~bad], clean[~bad])
+        seen = (blocks >= 0).any(-1).repeat_interleave(hq // h, 1) & bad
+        assert seen.any() and (torch.isnan(got[seen]).any(-1).all() if not fill < 1e9 else not torch.equal(got[seen], clean[seen]))
